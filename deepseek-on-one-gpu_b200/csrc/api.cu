@@ -73,13 +73,14 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 2-D row-major map: `rows` x `cols` elements, box `box_rows` x `box_cols`.
-int make_map(CUtensorMap* m, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t cols, uint64_t rows,
-             uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw) {
+// 2-D row-major map: `rows` x `cols` elements in rows of `row_bytes` bytes, box
+// `box_rows` x `box_cols`.
+int make_map_strided(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
+                     uint64_t rows, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(DSMOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {cols * static_cast<uint64_t>(elem_bytes)};
+  cuuint64_t strides[1] = {row_bytes};
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
@@ -88,6 +89,11 @@ int make_map(CUtensorMap* m, CUtensorMapDataType dt, int elem_bytes, const void*
     return fail(DSMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): rows=%llu cols=%llu box=%ux%u", int(r),
                 (unsigned long long)rows, (unsigned long long)cols, box_rows, box_cols);
   return DSMOE_OK;
+}
+
+int make_map(CUtensorMap* m, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t cols, uint64_t rows,
+             uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw) {
+  return make_map_strided(m, dt, cols * static_cast<uint64_t>(elem_bytes), base, cols, rows, box_cols, box_rows, sw);
 }
 
 int num_sms() {
@@ -277,8 +283,7 @@ int run_gemm(const GemmJob& j, cudaStream_t s) {
   gp.sx = j.sx;
   gp.y = j.y;
   gp.status = j.status;
-  const int ctas = g_gemm_ctas > 0 && g_gemm_ctas < num_sms() ? g_gemm_ctas : num_sms();
-  DSMOE_CUDA(launch_grouped_gemm(m_w0, m_w1, m_x, m_x32, gp, j.tile, ctas, s));
+  DSMOE_CUDA(launch_grouped_gemm(m_w0, m_w1, m_x, m_x32, gp, j.tile, gemm_grid(), s));
   return DSMOE_OK;
 }
 
@@ -361,6 +366,13 @@ int do_experts(const dsmoe_moe_config_t* c, const dsmoe_layer_weights_t* wt, con
 }  // namespace
 
 int set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
+
+int make_tma_map(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
+                 uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
+  return make_map_strided(m, dt, row_bytes, base, cols, rows, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int sm_count() { return num_sms(); }
+int gemm_grid() { return g_gemm_ctas > 0 && g_gemm_ctas < num_sms() ? g_gemm_ctas : num_sms(); }
 
 }  // namespace dsmoe
 

@@ -10,6 +10,11 @@ namespace dsmoe {
 
 // Records `msg` as the calling thread's dsmoe_last_error() and returns `code`.
 int set_last_error(int code, const char* msg);
+// 2-D row-major TMA map with a 128-byte swizzle; returns a DSMOE_* code.
+int make_tma_map(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
+                 uint64_t rows, uint32_t box_cols, uint32_t box_rows);
+int sm_count();   // SMs of the current device
+int gemm_grid();  // CTAs of a persistent GEMM launch (dsmoe_set_gemm_sm_limit)
 // Device address of the current device's allocation-free scratch status word
 // (noalloc.cu); nullptr with the reason in *err on failure.
 void* noalloc_status_word(const char** err);

@@ -1,0 +1,111 @@
+// Internal interface of the MXFP4 operators (mxfp4_quant.cu, mxfp4_prep.cu,
+// mxfp4_gemm.cu, mxfp4_api.cu).
+//
+// MXFP4: a row of K numbers is K e2m1 codes (two per byte, the even element
+// in the low nibble) and one e8m0 scale byte b = 2^(b - 127) per 32
+// consecutive numbers; byte 255 is NaN.
+//
+// The tensor core takes bf16 activations as two e4m3 terms that share one
+// power-of-two scale per 32 numbers: with 2^7 <= amax * 2^-e < 2^8,
+//   hi = e4m3(x * 2^-e),  lo = e4m3(x * 2^-e - hi).
+// hi keeps 4 of a bf16's 8 significant bits and the remainder fits lo's 4
+// exactly, as long as its last bit is not below e4m3's smallest step 2^-9:
+// numbers down to 2^-9 of the block's amax are exact, smaller ones are off by
+// at most 2^-10 * 2^e <= 2^-17 of the amax.
+//
+// Scale factors are stored as the 512-byte atoms tcgen05.cp takes: rows
+// 32j + l (j < 4, l < 32) of a 128-row tile and one K block of 128 numbers;
+// bytes l * 16 + j * 4 .. + 3 hold row 32j + l's four scales of that block.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace dsmoe {
+namespace mx {
+
+constexpr int kMaxGroups = 512;
+constexpr int kEpiWarps = 16;
+
+// Token tiles of the product kernels: columns of one work unit, and 512-byte
+// scale atoms per token tile and K block.
+constexpr int tile_atoms(int bn) { return bn > 64 ? 2 : 1; }
+
+// bf16 activations: columns of a tile that run hi and lo side by side in one
+// MMA (rounded to 32, hi columns then lo columns), or 0 where hi and lo are
+// two MMAs. Side by side the MMA is twice as wide, which pays while a narrow
+// one does not fill the tensor pipe; the accumulators then take 4 columns of
+// TMEM per token, which caps it at 96.
+__host__ __device__ constexpr int side_by_side(int bn, int ncols) {
+  const int n32 = (ncols + 31) & ~31;
+  return bn <= 64 ? n32 : (n32 <= 96 ? n32 : 0);
+}
+
+enum { kTypeBf16 = 0, kTypeF16 = 1, kTypeF32 = 2, kTypeE4m3 = 3 };
+
+// Group tables of a product: group g has counts[g] rows from row_start[g] on
+// and owns token tiles [tile_start[g], tile_start[g + 1]).
+struct Groups {
+  const int32_t* counts;      // NULL: one group of `rows` rows
+  const int32_t* row_start;
+  const int32_t* tile_start;
+  int n;
+  int rows;
+};
+
+struct GemmArgs {
+  Groups g;
+  int M;                 // features of one weight matrix
+  int K;
+  int P;                 // first lo row of the split activations
+  int ksplit;            // parts of K per tile (1 unless g.counts == NULL)
+  const uint8_t* sfa0;   // scale atoms of the weights [group][ceil(M/128)][K/128][512]
+  const uint8_t* sfa1;   // up projection (SwiGLU), else == sfa0
+  const uint8_t* sfb;    // scale atoms of the rows [tile][K/128][tile_atoms][512]
+  __nv_bfloat16* y;      // [row][M]
+  uint8_t* hq;           // SwiGLU: split rows [2][P][M] and their atoms
+  uint8_t* hsf;
+  float* partial;        // ksplit > 1: [tile unit][ksplit][column][256]
+  int32_t* arrived;      // ksplit > 1: [tile unit][kEpiWarps], zero before the launch
+  int* status;
+};
+
+// -------------------------------------------------------- mxfp4_quant.cu
+cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long long row_stride, const float* scale_inv,
+                            long long rows_per_mat, uint8_t* codes, uint8_t* scales, cudaStream_t s);
+cudaError_t launch_dequantize(const uint8_t* codes, const uint8_t* scales, long long blocks, int type, void* out,
+                              cudaStream_t s);
+// Scales [mats][N][K/32] -> atoms [mats][ceil(N/tile)][K/128][atoms][512].
+// zero (optional): n_zero counters cleared by the same launch.
+cudaError_t launch_tile_scales(const uint8_t* scales, int mats, int N, int K, int tile, int atoms, uint8_t* out,
+                               int32_t* zero, int n_zero, cudaStream_t s);
+
+// --------------------------------------------------------- mxfp4_prep.cu
+// Segments of rows sorted by expert from offsets[n + 1].
+cudaError_t launch_segments(const int32_t* offsets, int n, int rows, int tile, int32_t* counts, int32_t* row_start,
+                            int32_t* tile_start, int* status, cudaStream_t s);
+// Segments from a routing: pos[T][top_k] is the row of each (token, k), in
+// token order inside an expert, -1 for an id outside [0, n_routed).
+cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed, int shared, int tile,
+                              int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* pos, cudaStream_t s);
+// bf16 rows [T][K] -> hi/lo rows and scale atoms. pos == NULL: row t is row t
+// of g (zero_out, optional: rows of y outside every segment are cleared);
+// else token t goes to the rows pos names (and to row t of group 0 with shared).
+cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
+                         const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
+                         __nv_bfloat16* zero_out, int M, int32_t* zero, int n_zero, cudaStream_t s);
+// out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
+cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
+                           int shared, float scale, __nv_bfloat16* out, cudaStream_t s);
+
+// --------------------------------------------------------- mxfp4_gemm.cu
+// Largest K split of a single-group product that keeps its grid within one
+// wave; units: (feature tile pair, token tile) pairs.
+int pick_ksplit(int units, int kblocks, int sms);
+cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
+                        const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s);
+
+}  // namespace mx
+}  // namespace dsmoe

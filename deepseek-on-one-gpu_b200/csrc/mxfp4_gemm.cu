@@ -1,0 +1,591 @@
+// MXFP4 products on tcgen05 block-scaled MMA (sm_100a).
+//
+// For every group g, row r of its segment and feature m:
+//   Y[r, m] = sum_k  W_g[m, k] X[r, k]
+// W_g MXFP4; X either bf16 held as two e4m3 terms with shared scales (see
+// mxfp4.cuh; kind::mxf8f6f4, W * hi + W * lo) or MXFP4 itself (kind::mxf4).
+// The tensor core multiplies both sides' scales in, so the accumulators stay
+// in TMEM over the whole of K and are read once per work unit.
+//
+// Weights are the 128-row operand A, rows of X the N operand, so that few
+// rows waste little. A work unit is two A tiles (256 features, or 128 gate and
+// the same 128 up features for the SwiGLU form) times one token tile: the
+// token tile is read from L2 once for both, and a thread of the epilogue
+// holds gate and up of the same feature and token.
+//
+// 4-bit weights next to 8-bit activations: TMA widens 16 codes (8 bytes) to
+// 16 bytes of shared memory (8 bytes of padding), the layout kind::mxf8f6f4
+// reads, so a 128-number K block of one row is 128 bytes on both sides.
+//
+// Warp roles (one CTA per SM, persistent):
+//   warp 0     TMA producer (one thread)
+//   warp 1     TMEM allocator, MMA issuer (one thread): per stage it copies the
+//              scale atoms to TMEM (tcgen05.cp) and issues the MMAs behind them
+//   warp 3     unit planner, a shared-memory ring of decoded units
+//   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 16-column chunks
+// TMEM: two halves of accumulator columns, then one set of scale columns per
+// stage (a stage's scales are overwritten only after its MMAs released it). A
+// unit that fits a half alternates between them, so its epilogue overlaps the
+// next unit's MMAs; a larger one takes both.
+#include "common.cuh"
+#include "mxfp4.cuh"
+
+namespace dsmoe {
+namespace mx {
+namespace {
+
+constexpr int BM = 128;
+constexpr int RING = 4;
+constexpr int PLAN_WARP = 3;
+constexpr int EPI_WARP0 = 4;
+constexpr int NUM_CG = kEpiWarps / 4;
+constexpr int CHUNK = 16;
+constexpr int THREADS = (EPI_WARP0 + kEpiWarps) * 32;
+
+struct Unit {
+  int32_t ncols;   // valid rows of the token tile
+  int32_t row0;    // first row
+  int32_t tile;    // token tile index (scale atoms)
+  int32_t group;
+  int32_t m0, m1;  // first feature of each A tile; m1 < 0: one A tile only
+  int32_t n;       // MMA N of one term
+  int32_t both;    // hi and lo side by side (N = 2 n)
+  int32_t kb0, kb1;
+  int32_t part;    // K part
+  int32_t id;      // tile unit (split-K bookkeeping)
+};
+
+template <bool FP4_, int BN_, int STAGES_>
+struct Cfg {
+  static constexpr bool FP4 = FP4_;
+  static constexpr int BN = BN_;
+  static constexpr int STAGES = STAGES_;
+  static constexpr int KB_STAGE = FP4 ? 2 : 1;  // 128-number K blocks per stage (128 bytes of a row)
+  static constexpr int TERMS = FP4 ? 1 : 2;
+  static constexpr int ATOMS = tile_atoms(BN);
+  static constexpr int A_BYTES = BM * 128;
+  // What an A tile's copy counts on its mbarrier: the packed bytes it reads,
+  // without the padding it writes between them.
+  static constexpr int A_TX = FP4 ? A_BYTES : A_BYTES / 2;
+  static constexpr int B_OFF = 2 * A_BYTES;
+  static constexpr int B_BYTES = TERMS * BN * 128;
+  static constexpr int SFA_BYTES = KB_STAGE * 512;
+  static constexpr int SFB_BYTES = KB_STAGE * ATOMS * 512;
+  // Operand tiles start on 1024 bytes (128-byte swizzle), so the scale atoms
+  // of all stages live behind the operands of all stages.
+  static constexpr int OP_BYTES = B_OFF + B_BYTES;
+  static constexpr int SF_BYTES = 2 * SFA_BYTES + SFB_BYTES;
+  static constexpr int SF0 = STAGES * OP_BYTES;
+  // TMEM columns
+  static constexpr int SF_COLS = KB_STAGE * (2 + ATOMS) * 4;
+  static constexpr int SF_TOTAL = STAGES * SF_COLS <= 64 ? 64 : 128;
+  static constexpr int HALF = (512 - SF_TOTAL) / 2;
+  static constexpr int SF_BASE = 2 * HALF;
+  static constexpr int BAR_OFF = STAGES * (OP_BYTES + SF_BYTES);
+  // full[S], empty[S], tfull[2], tempty[2], done, ufull[RING], uempty[RING]
+  static constexpr int NUM_BARS = 2 * STAGES + 5 + 2 * RING;
+  static constexpr int MISC_OFF = BAR_OFF + 8 * NUM_BARS;
+  static constexpr int PLAN_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
+  static constexpr int SMEM = PLAN_OFF + RING * static_cast<int>(sizeof(Unit)) + 1024;
+  static_assert(SMEM <= 232448, "shared memory");
+  static_assert(OP_BYTES % 1024 == 0, "operand alignment");
+  static_assert(STAGES * SF_COLS <= SF_TOTAL, "scale columns");
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 512-byte scale atom (32 rows of 16 bytes, unswizzled) -> 4 TMEM columns,
+// repeated in all four lane quadrants.
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t saddr) {
+  uint64_t d = static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(128 >> 4) << 32;  // 8 rows of 16 bytes to the next 8
+  d |= static_cast<uint64_t>(1) << 46;
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
+}
+
+template <bool FP4>
+__device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                           uint32_t sfb, uint32_t acc) {
+  if constexpr (FP4)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+
+// Instruction descriptor of the block-scaled kinds: D fp32, both operands
+// K-major, e8m0 scales; A e2m1, B e4m3 (mxf8f6f4) or e2m1 (mxf4). `sf` is the
+// byte of the 32-bit scale word this MMA's K starts at.
+template <bool FP4>
+__device__ __forceinline__ uint32_t idesc_scaled(int n, int sf) {
+  const uint32_t at = FP4 ? 1u : 5u, bt = FP4 ? 1u : 0u;
+  return (static_cast<uint32_t>(sf) << 4) | (at << 7) | (bt << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(BM >> 7) << 27) | (static_cast<uint32_t>(sf) << 29);
+}
+
+template <class C, bool SWIGLU>
+__device__ __forceinline__ Unit decode(int u, const GemmArgs& p) {
+  Unit e;
+  const int per = SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
+  const int id = p.ksplit > 1 ? u / p.ksplit : u;
+  e.id = id;
+  e.part = u - id * p.ksplit;
+  int g = 0, rows = p.g.rows, row_start = 0, tile0 = 0, ntiles;
+  if (p.g.counts) {
+    int lo = 0, hi = p.g.n;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(p.g.tile_start + mid) * per <= id) lo = mid; else hi = mid;
+    }
+    g = lo;
+    rows = __ldg(p.g.counts + g);
+    row_start = __ldg(p.g.row_start + g);
+    tile0 = __ldg(p.g.tile_start + g);
+  }
+  ntiles = (rows + C::BN - 1) / C::BN;
+  const int local = id - tile0 * per;
+  const int mt = local / ntiles, nt = local - mt * ntiles;
+  e.group = g;
+  e.ncols = min(C::BN, rows - nt * C::BN);
+  e.row0 = row_start + nt * C::BN;
+  e.tile = tile0 + nt;
+  e.m0 = mt * (SWIGLU ? BM : 2 * BM);
+  e.m1 = SWIGLU ? e.m0 : (e.m0 + BM < p.M ? e.m0 + BM : -1);
+  const int n32 = C::FP4 ? 0 : side_by_side(C::BN, e.ncols);
+  e.both = n32 > 0;
+  e.n = n32 ? n32 : (e.ncols + 15) & ~15;
+  const int KB = p.K / 128;
+  e.kb0 = 0;
+  e.kb1 = KB;
+  if (p.ksplit > 1) {
+    // whole stages per part
+    const int st = (KB + C::KB_STAGE - 1) / C::KB_STAGE;
+    e.kb0 = static_cast<int>(static_cast<long long>(st) * e.part / p.ksplit) * C::KB_STAGE;
+    e.kb1 = min(KB, static_cast<int>(static_cast<long long>(st) * (e.part + 1) / p.ksplit) * C::KB_STAGE);
+  }
+  return e;
+}
+
+__device__ __forceinline__ int unit_count(const GemmArgs& p, int bn, bool swiglu) {
+  const int per = swiglu ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
+  const int tiles = p.g.counts ? __ldg(p.g.tile_start + p.g.n) : (p.g.rows + bn - 1) / bn;
+  return tiles * per * p.ksplit;
+}
+
+// bf16 pairs of features: an even lane stores features (lane, lane + 1) of
+// token c, its odd neighbour those of token c + 1.
+__device__ __forceinline__ void store_pairs(const float* v, int c0, int ncols, int feat_ok, __nv_bfloat16* y,
+                                            size_t ld, int lane) {
+  const int odd = lane & 1;
+#pragma unroll
+  for (int c = 0; c < CHUNK; c += 2) {
+    const unsigned short a = __bfloat16_as_ushort(__float2bfloat16_rn(v[c]));
+    const unsigned short b = __bfloat16_as_ushort(__float2bfloat16_rn(v[c + 1]));
+    const uint32_t mine = odd ? b : a;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(odd ? a : b), 1);
+    const uint32_t pair = odd ? (other | (mine << 16)) : (mine | (other << 16));
+    const int tok = c0 + c + odd;
+    if (tok < ncols && feat_ok) *reinterpret_cast<uint32_t*>(y + tok * ld) = pair;
+  }
+}
+
+template <class C, bool SWIGLU>
+__global__ void __launch_bounds__(THREADS, 1)
+mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1,
+               const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
+               const GemmArgs p) {
+  constexpr bool FP4 = C::FP4;
+  constexpr int BN = C::BN, STAGES = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* done_bar = tempty + 2;
+  uint64_t* ufull = done_bar + 1;
+  uint64_t* uempty = ufull + RING;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + C::MISC_OFF);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(smem + C::MISC_OFF + 4);
+  Unit* plan = reinterpret_cast<Unit*>(smem + C::PLAN_OFF);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], kEpiWarps);
+    }
+    mbar_init(done_bar, 1);
+    for (int r = 0; r < RING; ++r) {
+      mbar_init(&ufull[r], 1);
+      mbar_init(&uempty[r], 2 + kEpiWarps);  // producer, issuer, epilogue warps
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_w0);
+    prefetch_tmap(&tm_w1);
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_x32);
+  }
+  if (warp == 1) tmem_alloc(s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  const uint32_t tmem = *s_tmem;
+  const int total = unit_count(p, BN, SWIGLU);
+  const int KB = p.K / 128;
+  const int MT = (p.M + BM - 1) / BM;
+
+  if (warp == PLAN_WARP) {
+    // ------------------------------------------------------------- planner
+    if (lane == 0) {
+      int i = 0;
+      for (int u = blockIdx.x; u < total; u += gridDim.x, ++i) {
+        const Unit e = decode<C, SWIGLU>(u, p);
+        const int ri = i % RING;
+        if (!mbar_wait(&uempty[ri], ((i / RING) & 1) ^ 1, p.status, kDevTimeoutProducer, s_abort)) break;
+        plan[ri] = e;
+        mbar_arrive(&ufull[ri]);
+      }
+    }
+  } else if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
+      int stage = 0, issued = 0, i = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+        const int ri = i % RING;
+        if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutProducer, s_abort)) break;
+        const Unit e = plan[ri];
+        mbar_arrive(&uempty[ri]);
+        const int wrow = e.group * p.M;
+        const bool two = e.m1 >= 0;
+        const uint8_t* fa0 = p.sfa0 + (static_cast<size_t>(e.group) * MT + e.m0 / BM) * KB * 512;
+        const uint8_t* fa1 = p.sfa1 + (static_cast<size_t>(e.group) * MT + (two ? e.m1 : 0) / BM) * KB * 512;
+        const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
+        const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
+        for (int kb = e.kb0; kb < e.kb1; kb += C::KB_STAGE) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.status, kDevTimeoutProducer, s_abort)) { ok = false; break; }
+          uint8_t* st = smem + stage * C::OP_BYTES;
+          uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
+          const int nkb = min(C::KB_STAGE, e.kb1 - kb);  // an odd last K block: only its scales exist
+          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * (C::A_TX + nkb * 512) + xbytes + nkb * C::ATOMS * 512);
+          const int kx = FP4 ? kb * 64 : kb * 128;  // coordinate: bytes of packed codes, or numbers
+          tma_load_2d(st, &tm_w0, &full[stage], kx, wrow + e.m0, pol_w);
+          if (two) tma_load_2d(st + C::A_BYTES, &tm_w1, &full[stage], kx, wrow + e.m1, pol_w);
+          if (!FP4 && e.both) {
+            for (int s = 0; s < e.n; s += 32) {
+              tma_load_2d(st + C::B_OFF + s * 128, &tm_x32, &full[stage], kx, e.row0 + s, pol_x);
+              tma_load_2d(st + C::B_OFF + (e.n + s) * 128, &tm_x32, &full[stage], kx, p.P + e.row0 + s, pol_x);
+            }
+          } else {
+            tma_load_2d(st + C::B_OFF, &tm_x, &full[stage], kx, e.row0, pol_x);
+            if (!FP4) tma_load_2d(st + C::B_OFF + BN * 128, &tm_x, &full[stage], kx, p.P + e.row0, pol_x);
+          }
+          bulk_load(sf, fa0 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
+          if (two) bulk_load(sf + C::SFA_BYTES, fa1 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
+          bulk_load(sf + 2 * C::SFA_BYTES, fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512,
+                    &full[stage]);
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      // The last copies must have landed before the CTA may exit.
+      const int n_drain = issued < STAGES ? issued : STAGES;
+      for (int d = 0; d < n_drain; ++d) {
+        if (--stage < 0) { stage = STAGES - 1; phase ^= 1; }
+        mbar_wait_settle(&full[stage], phase, p.status, kDevTimeoutProducer);
+      }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (lane == 0) {
+      int stage = 0, nb = 0, i = 0;
+      uint32_t phase = 0, tphase = 0;  // tphase: one bit per half
+      bool ok = true;
+      for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+        const int ri = i % RING;
+        if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutMma, s_abort)) break;
+        const Unit e = plan[ri];
+        mbar_arrive(&uempty[ri]);
+        const int nn = e.both ? 2 * e.n : e.n;  // columns of one accumulator
+        const bool big = 2 * nn > C::HALF;
+        const int b0 = big ? 0 : nb, b1 = big ? 1 : nb;
+        for (int b = b0; b <= b1 && ok; ++b) {
+          ok = mbar_wait(&tempty[b], ((tphase >> b) & 1) ^ 1, p.status, kDevTimeoutMma, s_abort);
+          tphase ^= 1u << b;
+        }
+        if (!ok) break;
+        const uint32_t d0 = tmem + b0 * C::HALF, d1 = d0 + nn;
+        const bool two = e.m1 >= 0;
+        for (int kb = e.kb0; kb < e.kb1; kb += C::KB_STAGE) {
+          if (!mbar_wait(&full[stage], phase, p.status, kDevTimeoutMma, s_abort)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + stage * C::OP_BYTES);
+          const uint32_t sf = smem_u32(smem + C::SF0 + stage * C::SF_BYTES);
+          const uint32_t tsa = tmem + C::SF_BASE + stage * C::SF_COLS;
+          const uint32_t tsb = tsa + C::KB_STAGE * 8;
+          const int nkb = min(C::KB_STAGE, e.kb1 - kb);
+          for (int h = 0; h < nkb; ++h) {
+            copy_scales(tsa + h * 8, sf + h * 512);
+            if (two) copy_scales(tsa + h * 8 + 4, sf + C::SFA_BYTES + h * 512);
+#pragma unroll
+            for (int a = 0; a < C::ATOMS; ++a)
+              copy_scales(tsb + (h * C::ATOMS + a) * 4, sf + 2 * C::SFA_BYTES + (h * C::ATOMS + a) * 512);
+          }
+          const uint64_t da0 = umma_desc_sw128(st), da1 = umma_desc_sw128(st + C::A_BYTES);
+          const uint64_t db = umma_desc_sw128(st + C::B_OFF), dl = umma_desc_sw128(st + C::B_OFF + BN * 128);
+          const int steps = FP4 ? 2 * nkb : 4;  // 32 bytes of a row each
+          for (int kk = 0; kk < steps; ++kk) {
+            const uint32_t id = FP4 ? idesc_scaled<true>(nn, (kk & 1) * 2) : idesc_scaled<false>(nn, kk);
+            const uint32_t a0 = tsa + (FP4 ? (kk >> 1) * 8 : 0);
+            const uint32_t sb = tsb + (FP4 ? (kk >> 1) * C::ATOMS * 4 : 0);
+            const uint32_t acc = kb > e.kb0 || kk > 0;
+            mma_scaled<FP4>(d0, da0 + 2 * kk, db + 2 * kk, id, a0, sb, acc);
+            if (!FP4 && !e.both) mma_scaled<FP4>(d0, da0 + 2 * kk, dl + 2 * kk, id, a0, sb, 1);
+            if (two) {
+              mma_scaled<FP4>(d1, da1 + 2 * kk, db + 2 * kk, id, a0 + 4, sb, acc);
+              if (!FP4 && !e.both) mma_scaled<FP4>(d1, da1 + 2 * kk, dl + 2 * kk, id, a0 + 4, sb, 1);
+            }
+          }
+          mma_commit(&empty[stage]);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        for (int b = b0; b <= b1; ++b) mma_commit(&tfull[b]);
+        if (!big) nb ^= 1;
+      }
+      // Every MMA ends before TMEM is freed, also after an abort.
+      mma_commit(done_bar);
+      mbar_wait_settle(done_bar, 0, p.status, kDevTimeoutMma);
+    }
+  } else if (warp >= EPI_WARP0) {
+    // ------------------------------------------------------------ epilogue
+    const int quad = warp & 3;
+    const int cg = (warp - EPI_WARP0) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    int nb = 0, i = 0;
+    uint32_t tphase = 0;  // one bit per half
+    bool ok = true;
+    for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+      const int ri = i % RING;
+      if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutEpilogue, s_abort)) break;
+      const Unit e = plan[ri];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&uempty[ri]);
+      const int nn = e.both ? 2 * e.n : e.n;
+      const bool big = 2 * nn > C::HALF;
+      const int b0 = big ? 0 : nb, b1 = big ? 1 : nb;
+      for (int b = b0; b <= b1 && ok; ++b) {
+        ok = mbar_wait(&tfull[b], (tphase >> b) & 1, p.status, kDevTimeoutEpilogue, s_abort);
+        tphase ^= 1u << b;
+      }
+      if (!ok) break;
+      if (!big) nb ^= 1;
+      tc_fence_after();
+      const uint32_t d0 = tmem + lanes + b0 * C::HALF, d1 = d0 + nn;
+      // 16 columns from column c on of one accumulator, hi + lo
+      auto load = [&](uint32_t d, int c, float* v) {
+        tmem_ld16(d + c, v);
+        if (!FP4 && e.both) {
+          float l[CHUNK];
+          tmem_ld16(d + e.n + c, l);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] += l[j];
+        } else {
+          tmem_ld_wait();
+        }
+      };
+      if constexpr (SWIGLU) {
+        const int f0 = e.m0 + quad * 32;  // this warp's 32 features: one scale block
+        const int KB2 = p.M / 128;
+        for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+          float h[CHUNK];
+          {
+            float up[CHUNK];
+            load(d0, c0, h);
+            load(d1, c0, up);
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) h[j] = __fdividef(h[j], 1.0f + __expf(-h[j])) * up[j];
+          }
+#pragma unroll
+          for (int j = 0; j < CHUNK; j += 4) {
+            uint32_t hi4 = 0, lo4 = 0, bytes = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const float v = h[j + t];
+              const uint32_t ef = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu) >> 23;
+              const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
+              const float inv = ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23);
+              const float q = v * inv;
+              const uint32_t hb = f32x2_to_e4m3x2(q, 0.f) & 0xff;
+              const uint32_t lb = f32x2_to_e4m3x2(q - e4m3_to_f32(static_cast<uint8_t>(hb)), 0.f) & 0xff;
+              hi4 |= hb << (8 * t);
+              lo4 |= lb << (8 * t);
+              bytes |= byte << (8 * t);
+            }
+            // 4x4 byte transpose over groups of 4 lanes: lane l then holds 4
+            // features of token j + l % 4
+            auto transpose = [&](uint32_t v) {
+              uint32_t o = __shfl_xor_sync(0xffffffffu, v, 1);
+              v = __byte_perm(v, o, lane & 1 ? 0x3715 : 0x6240);
+              o = __shfl_xor_sync(0xffffffffu, v, 2);
+              return __byte_perm(v, o, lane & 2 ? 0x3276 : 0x5410);
+            };
+            hi4 = transpose(hi4);
+            lo4 = transpose(lo4);
+            const int col = c0 + j + (lane & 3);
+            if (col < e.ncols) {
+              const size_t off = static_cast<size_t>(e.row0 + col) * p.M + f0 + (lane & ~3);
+              *reinterpret_cast<uint32_t*>(p.hq + off) = hi4;
+              *reinterpret_cast<uint32_t*>(p.hq + static_cast<size_t>(p.P) * p.M + off) = lo4;
+              if (lane < 4) {
+                uint8_t* sf = p.hsf + (static_cast<size_t>(e.tile) * KB2 + e.m0 / 128) * (C::ATOMS * 512) + quad;
+                const uint8_t byte = static_cast<uint8_t>(bytes >> (8 * lane));
+                auto spot = [](int c) { return (c >> 7) * 512 + (c & 31) * 16 + ((c >> 5) & 3) * 4; };
+                sf[spot(col)] = byte;
+                if (e.both) sf[spot(col + e.n)] = byte;
+              }
+            }
+          }
+        }
+      } else {
+        const bool two = e.m1 >= 0;
+        const int ld_feat = quad * 32 + (lane & ~1);
+        if (p.ksplit == 1) {
+          for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+            float v[CHUNK];
+            __nv_bfloat16* y = p.y + static_cast<size_t>(e.row0) * p.M + ld_feat;
+            load(d0, c0, v);
+            store_pairs(v, c0, e.ncols, e.m0 + ld_feat < p.M, y + e.m0, p.M, lane);
+            if (two) {
+              load(d1, c0, v);
+              store_pairs(v, c0, e.ncols, e.m1 + ld_feat < p.M, y + e.m1, p.M, lane);
+            }
+          }
+        } else {
+          // Every part leaves its sums in `partial`; the warp that arrives
+          // last on its (tile, quadrant, column group) adds the parts up in
+          // part order, so the result does not depend on who that is.
+          const size_t part_sz = static_cast<size_t>(C::BN) * 2 * BM;
+          float* all = p.partial + static_cast<size_t>(e.id) * p.ksplit * part_sz + quad * 32 + lane;
+          float* mine = all + e.part * part_sz;
+          for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+            float v[CHUNK];
+            for (int a = 0; a < (two ? 2 : 1); ++a) {
+              load(a ? d1 : d0, c0, v);
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j)
+                if (c0 + j < e.ncols) mine[(c0 + j) * 2 * BM + a * BM] = v[j];
+            }
+          }
+          __threadfence();
+          __syncwarp();
+          int last = 0;
+          if (lane == 0) last = atomicAdd(p.arrived + e.id * kEpiWarps + warp - EPI_WARP0, 1) == p.ksplit - 1;
+          last = __shfl_sync(0xffffffffu, last, 0);
+          if (last) {
+            __threadfence();
+            for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+              for (int a = 0; a < (two ? 2 : 1); ++a) {
+                float v[CHUNK];
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) v[j] = 0.f;
+                for (int s = 0; s < p.ksplit; ++s)
+#pragma unroll
+                  for (int j = 0; j < CHUNK; ++j)
+                    if (c0 + j < e.ncols) v[j] += __ldcg(all + s * part_sz + (c0 + j) * 2 * BM + a * BM);
+                const int m = a ? e.m1 : e.m0;
+                store_pairs(v, c0, e.ncols, m + ld_feat < p.M, p.y + static_cast<size_t>(e.row0) * p.M + m + ld_feat,
+                            p.M, lane);
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0)
+        for (int b = b0; b <= b1; ++b) mbar_arrive(&tempty[b]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+template <class C, bool SWIGLU>
+cudaError_t launch(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& x32,
+                   const GemmArgs& a, int grid, cudaStream_t s) {
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!attr[dev]) {
+    e = cudaFuncSetAttribute(mx_gemm_kernel<C, SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    attr[dev] = true;
+  }
+  mx_gemm_kernel<C, SWIGLU><<<grid, THREADS, C::SMEM, s>>>(w0, w1, x, x32, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int pick_ksplit(int units, int kblocks, int sms) {
+  int s = sms / (units > 0 ? units : 1);
+  if (s > kblocks / 4) s = kblocks / 4;  // at least four K blocks a part
+  if (s > 16) s = 16;
+  return s < 1 ? 1 : s;
+}
+
+cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
+                        const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s) {
+  if (fp4) {
+    switch (tile) {
+      case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
+      case 192: return launch<Cfg<true, 192, 3>, false>(w0, w1, x, x32, a, grid, s);
+      default: return cudaErrorInvalidValue;
+    }
+  }
+  switch (tile) {
+    case 32:
+      return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, a, grid, s)
+                    : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, a, grid, s);
+    case 64:
+      return swiglu ? launch<Cfg<false, 64, 4>, true>(w0, w1, x, x32, a, grid, s)
+                    : launch<Cfg<false, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
+    case 160:
+      return swiglu ? launch<Cfg<false, 160, 3>, true>(w0, w1, x, x32, a, grid, s)
+                    : launch<Cfg<false, 160, 3>, false>(w0, w1, x, x32, a, grid, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+}  // namespace mx
+}  // namespace dsmoe

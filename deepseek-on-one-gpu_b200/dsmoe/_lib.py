@@ -27,7 +27,10 @@ EXPORTED = (
     "dsmoe_moe_layer_ffn", "dsmoe_read_ranges", "dsmoe_ep_plan", "dsmoe_ep_push", "dsmoe_moe_local_peer",
     "dsmoe_ep_meta_bytes", "dsmoe_ipc_alloc", "dsmoe_ipc_open", "dsmoe_ipc_close", "dsmoe_ipc_free",
     "dsmoe_sample_top_p", "dsmoe_slotcache_state_bytes", "dsmoe_slotcache_step", "dsmoe_map_host_pointers",
-    "dsmoe_clock_probe",
+    "dsmoe_clock_probe", "dsmoe_mxfp4_quantize", "dsmoe_mxfp4_dequantize", "dsmoe_mxfp4_scale_atoms_bytes",
+    "dsmoe_mxfp4_scale_atoms", "dsmoe_mxfp4_linear_workspace_size", "dsmoe_mxfp4_linear",
+    "dsmoe_mxfp4_matmul_workspace_size", "dsmoe_mxfp4_matmul", "dsmoe_mxfp4_grouped_linear_workspace_size",
+    "dsmoe_mxfp4_grouped_linear", "dsmoe_mxfp4_moe_workspace_size", "dsmoe_mxfp4_moe",
 )
 
 
@@ -47,6 +50,16 @@ class LayerWeights(ctypes.Structure):
         ("w_up", ctypes.c_void_p), ("s_up", ctypes.c_void_p),
         ("w_down", ctypes.c_void_p), ("s_down", ctypes.c_void_p),
         ("slot_of_expert", ctypes.c_void_p),
+    ]
+
+
+class MXFP4ExpertsDesc(ctypes.Structure):
+    """``dsmoe_mxfp4_experts_t`` (include/dsmoe.h)."""
+    _fields_ = [
+        ("hidden", ctypes.c_int32), ("inter", ctypes.c_int32), ("n_routed", ctypes.c_int32),
+        ("shared", ctypes.c_int32),
+        ("gate_codes", ctypes.c_void_p), ("gate_atoms", ctypes.c_void_p), ("up_codes", ctypes.c_void_p),
+        ("up_atoms", ctypes.c_void_p), ("down_codes", ctypes.c_void_p), ("down_atoms", ctypes.c_void_p),
     ]
 
 
@@ -122,6 +135,26 @@ def lib() -> ctypes.CDLL:
                 L.dsmoe_map_host_pointers.argtypes = [u64p, i32, u64p]
                 L.dsmoe_read_ranges.argtypes = [i32, ctypes.POINTER(ctypes.c_char_p), u64p, u64p,
                                                 ctypes.POINTER(vp), i32]
+                i64, f32 = ctypes.c_int64, ctypes.c_float
+                L.dsmoe_mxfp4_quantize.argtypes = [vp, i32, i64, i32, i64, vp, i64, vp, vp, vp]
+                L.dsmoe_mxfp4_dequantize.argtypes = [vp, vp, i64, i32, vp, vp]
+                L.dsmoe_mxfp4_scale_atoms_bytes.argtypes = [i32, i32, i32]
+                L.dsmoe_mxfp4_scale_atoms_bytes.restype = sz
+                L.dsmoe_mxfp4_scale_atoms.argtypes = [vp, i32, i32, i32, vp, vp]
+                L.dsmoe_mxfp4_linear_workspace_size.argtypes = [i32, i32, i32]
+                L.dsmoe_mxfp4_linear_workspace_size.restype = sz
+                L.dsmoe_mxfp4_linear.argtypes = [vp, i64, i32, i32, i32, vp, vp, vp, vp, sz, vp, vp]
+                L.dsmoe_mxfp4_matmul_workspace_size.argtypes = [i32, i32, i32]
+                L.dsmoe_mxfp4_matmul_workspace_size.restype = sz
+                L.dsmoe_mxfp4_matmul.argtypes = [vp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp, vp]
+                L.dsmoe_mxfp4_grouped_linear_workspace_size.argtypes = [i32, i32, i32, i32]
+                L.dsmoe_mxfp4_grouped_linear_workspace_size.restype = sz
+                L.dsmoe_mxfp4_grouped_linear.argtypes = [vp, i64, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp, sz, vp,
+                                                         vp]
+                L.dsmoe_mxfp4_moe_workspace_size.argtypes = [i32, i32, i32, i32, i32, i32]
+                L.dsmoe_mxfp4_moe_workspace_size.restype = sz
+                L.dsmoe_mxfp4_moe.argtypes = [vp, i64, i32, ctypes.POINTER(MXFP4ExpertsDesc), vp, vp, i32, f32, vp, vp,
+                                              sz, vp, vp]
                 for name in EXPORTED:
                     getattr(L, name).restype = getattr(L, name).restype or ctypes.c_int
                 _lib = L

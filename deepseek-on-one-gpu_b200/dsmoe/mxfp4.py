@@ -1,0 +1,378 @@
+"""MXFP4 experts and projections: 4-bit weights with a power-of-two scale per
+32 numbers (the OCP microscaling format), 17/32 of the FP8 checkpoint's bytes.
+
+The reference knows FP8 weights only (``inference/ops.py:15-44``); these
+operators stand beside ``fp8_linear``, ``expert_ffn`` and ``moe_block`` for
+users who halve the expert memory and the bytes a decode step reads:
+
+  * ``mxfp4_quantize`` / ``mxfp4_dequantize``  tensors to and from MXFP4, also
+    straight from the checkpoint's ``(weight, weight_scale_inv)``;
+  * ``MXFP4Weight``            a weight (or a stack of experts) laid out for
+    the products, once;
+  * ``mxfp4_linear``           bf16 activations times an MXFP4 weight;
+  * ``mxfp4_matmul``           MXFP4 activations times an MXFP4 weight;
+  * ``mxfp4_grouped_linear``   rows sorted by expert times each expert's weight;
+  * ``MXFP4Experts`` / ``mxfp4_moe``  the routed FFN after ``route``.
+
+``GPUTransfer(..., expert_format="mxfp4")`` makes ``moe_block`` and
+``moe_layer_ffn`` run on 4-bit experts. Every call goes through
+``libdsmoe.so`` on the current stream of the tensors' device, with scratch
+from torch's allocator (private to the call, also in a captured graph). There
+is no CPU path and no backward: tensors that require a gradient are rejected.
+"""
+from __future__ import annotations
+
+import ctypes
+import threading
+
+import torch
+
+from . import _lib
+from ._lib import check, lib, ptr, stream_handle
+
+BLOCK = 32
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
+_status: dict[int, torch.Tensor] = {}
+_status_lock = threading.Lock()
+
+
+def _device_status(device: torch.device) -> torch.Tensor:
+    """The device error word of this module's kernels (int32, first error wins)."""
+    t = _status.get(device.index)
+    if t is None:
+        with _status_lock:
+            t = _status.get(device.index)
+            if t is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first MXFP4 call on a device must come before a graph capture")
+                t = torch.zeros(1, dtype=torch.int32, device=device)
+                torch.cuda.current_stream(device).synchronize()
+                _status[device.index] = t
+    return t
+
+
+def mxfp4_status(device) -> int:
+    """Read (synchronously) and clear the device error code of the MXFP4
+    kernels: 0, or the first error since the last read (6: offsets of
+    ``mxfp4_grouped_linear`` that decrease or leave the rows)."""
+    t = _device_status(_index(torch.device(device)))
+    torch.cuda.synchronize(t.device)
+    code = int(t.item())
+    if code:
+        t.zero_()
+    return code
+
+
+def _index(device: torch.device) -> torch.device:
+    return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+def _require(what: str, *tensors: torch.Tensor) -> None:
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what} expects tensors")
+        if not t.is_cuda:
+            raise RuntimeError("dsmoe runs on CUDA tensors only (no CPU fallback)")
+        if dev is not None and t.device != dev:
+            raise RuntimeError(f"{what}: tensors on different devices ({dev}, {t.device})")
+        dev = t.device
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{what} has no backward: detach the inputs or call it under torch.no_grad()")
+
+
+def _rows(x: torch.Tensor, align: int) -> torch.Tensor:
+    """``x`` as (rows, K) with unit column stride, rows that do not overlap
+    and start on ``align`` bytes; a copy only where the strides need one."""
+    K = x.shape[-1]
+    x2 = x.reshape(-1, K)
+    if x2.stride(1) != 1 and K > 1:
+        return x2.contiguous()
+    if x2.data_ptr() % align or (x2.shape[0] > 1 and (x2.stride(0) < K or x2.stride(0) * x2.element_size() % align)):
+        return x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % align else t
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _quantize_into(x: torch.Tensor, scale_inv: torch.Tensor | None, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    K = x.shape[-1]
+    fp8 = x.dtype == torch.float8_e4m3fn
+    x2 = _rows(x, 8 if fp8 else 16)
+    per = x.shape[-2] if fp8 else 1
+    with torch.cuda.device(x.device):
+        check(lib().dsmoe_mxfp4_quantize(ptr(x2), _DTYPES[x.dtype], x2.shape[0], K, x2.stride(0), ptr(scale_inv),
+                                         max(per, 1), ptr(codes), ptr(scales), stream_handle(x.device)),
+              "dsmoe_mxfp4_quantize")
+
+
+def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x`` [..., K] (K a multiple of 32) -> codes uint8 [..., K/2] and scales
+    uint8 [..., K/32]. Per block of 32 numbers with largest magnitude a:
+    scale 2^(floor(log2 a) - 2), codes rounded to nearest even, saturating at
+    6; a block with an infinity or a NaN becomes NaN.
+
+    ``x`` is bf16, fp16 or fp32, or e4m3 [..., O, I] with the checkpoint's
+    ``scale_inv`` fp32 [..., ceil(O/128), ceil(I/128)] (the products are
+    rounded as exact numbers)."""
+    _require("mxfp4_quantize", x, scale_inv)
+    if x.dtype not in _DTYPES:
+        raise TypeError("mxfp4_quantize expects bf16, fp16, fp32 or e4m3")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
+        raise ValueError(f"the last dimension must be a multiple of {BLOCK}")
+    K = x.shape[-1]
+    if x.dtype == torch.float8_e4m3fn:
+        if scale_inv is None or scale_inv.dtype != torch.float32:
+            raise TypeError("e4m3 needs fp32 scale_inv")
+        if x.dim() < 2:
+            raise ValueError("e4m3 weights are (..., out, in)")
+        want = (*x.shape[:-2], -(-x.shape[-2] // 128), -(-K // 128))
+        if tuple(scale_inv.shape) != want:
+            raise ValueError(f"scale_inv must be {want}, is {tuple(scale_inv.shape)}")
+        scale_inv = scale_inv.contiguous()
+    elif scale_inv is not None:
+        raise TypeError("scale_inv goes with e4m3 only")
+    codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-1], K // BLOCK, dtype=torch.uint8, device=x.device)
+    if x.numel():
+        _quantize_into(x, scale_inv, codes, scales)
+    return codes, scales
+
+
+def _check_pair(what: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
+    _require(what, codes, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError(f"{what} expects uint8 codes and scales")
+    if codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1] or \
+            codes.shape[-1] != 16 * scales.shape[-1]:
+        raise ValueError(f"{what}: codes [..., K/2] {tuple(codes.shape)} do not go with scales [..., K/32] "
+                         f"{tuple(scales.shape)}")
+    return 2 * codes.shape[-1]
+
+
+def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
+                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers MXFP4 data stands for, in bf16 or fp32 (exact) or fp16
+    (rounded; beyond its range infinite)."""
+    K = _check_pair("mxfp4_dequantize", codes, scales)
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError("mxfp4_dequantize produces bf16, fp16 or fp32")
+    codes, scales = _dense(codes, 4), scales.contiguous()
+    out = torch.empty(*codes.shape[:-1], K, dtype=out_dtype, device=codes.device)
+    if out.numel():
+        with torch.cuda.device(codes.device):
+            check(lib().dsmoe_mxfp4_dequantize(ptr(codes), ptr(scales), scales.numel(), _DTYPES[out_dtype], ptr(out),
+                                               stream_handle(codes.device)), "dsmoe_mxfp4_dequantize")
+    return out
+
+
+class MXFP4Weight:
+    """An MXFP4 weight ``[out, in]`` or a stack of experts ``[E, out, in]``,
+    held for the products: the codes as they are (not copied when dense and
+    32-byte aligned) and the scales in the tensor core's layout. in features
+    a multiple of 128, out features of 8."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        K = _check_pair("MXFP4Weight", codes, scales)
+        if codes.dim() not in (2, 3):
+            raise ValueError("a weight is (out, in/2) or (experts, out, in/2)")
+        self.in_features, self.out_features = K, codes.shape[-2]
+        self.experts = codes.shape[0] if codes.dim() == 3 else None
+        self.device = codes.device
+        mats = 1 if self.experts is None else self.experts
+        nbytes = lib().dsmoe_mxfp4_scale_atoms_bytes(mats, self.out_features, K)
+        if nbytes == 0:
+            raise ValueError("MXFP4Weight: in features must be a multiple of 128 up to 32768, out features a multiple "
+                             "of 8, with at least one expert")
+        self.codes = _dense(codes, 32)
+        self.atoms = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self.status = _device_status(self.device)
+        self._pack(_dense(scales, 4), 0, mats)
+
+    def _pack(self, scales: torch.Tensor, first: int, mats: int) -> None:
+        per = self.atoms.numel() // (1 if self.experts is None else self.experts)
+        with torch.cuda.device(self.device):
+            check(lib().dsmoe_mxfp4_scale_atoms(ptr(scales), mats, self.out_features, self.in_features,
+                                                ptr(self.atoms) + first * per, stream_handle(self.device)),
+                  "dsmoe_mxfp4_scale_atoms")
+
+    @classmethod
+    def quantize(cls, weight: torch.Tensor, scale_inv: torch.Tensor | None = None) -> "MXFP4Weight":
+        """From a bf16, fp16 or fp32 weight, or the checkpoint's e4m3 weight
+        with its ``weight_scale_inv``."""
+        return cls(*mxfp4_quantize(weight, scale_inv))
+
+    @classmethod
+    def _empty(cls, experts: int, out_features: int, in_features: int, device) -> "MXFP4Weight":
+        """A stack to be filled slot by slot (``_set``)."""
+        self = cls.__new__(cls)
+        self.in_features, self.out_features, self.experts = in_features, out_features, experts
+        self.device = _index(torch.device(device))
+        self.codes = torch.zeros(experts, out_features, in_features // 2, dtype=torch.uint8, device=self.device)
+        self.atoms = torch.zeros(lib().dsmoe_mxfp4_scale_atoms_bytes(experts, out_features, in_features),
+                                 dtype=torch.uint8, device=self.device)
+        self.status = _device_status(self.device)
+        return self
+
+    def _set(self, slot: int, weight: torch.Tensor, scale_inv: torch.Tensor | None) -> None:
+        scales = torch.empty(self.out_features, self.in_features // BLOCK, dtype=torch.uint8, device=self.device)
+        _quantize_into(weight, scale_inv, self.codes[slot], scales)
+        self._pack(scales, slot, 1)
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.atoms.numel()
+
+
+def _check_weight(what: str, w: MXFP4Weight, stacked: bool) -> None:
+    if not isinstance(w, MXFP4Weight):
+        raise TypeError(f"{what} expects an MXFP4Weight")
+    if (w.experts is not None) != stacked:
+        raise ValueError(f"{what} expects " + ("a stack of experts" if stacked else "a single weight (out, in)"))
+
+
+def _check_x(what: str, x: torch.Tensor, K: int, *others: torch.Tensor) -> None:
+    _require(what, x, *others)
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects bf16 activations")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"{what}: activations end in {x.shape[-1] if x.dim() else 'no'} features, the weight has {K}")
+
+
+def mxfp4_linear(x: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
+    """``bf16(x @ W.T)`` for bf16 ``x`` [..., in], fp32 sums. A row with an
+    infinity or a NaN comes out as NaN."""
+    _check_weight("mxfp4_linear", weight, False)
+    _check_x("mxfp4_linear", x, weight.in_features, weight.codes)
+    x2 = _rows(x, 16)
+    T, K, N = x2.shape[0], weight.in_features, weight.out_features
+    out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
+    if T:
+        with torch.cuda.device(x.device):
+            ws = _scratch(lib().dsmoe_mxfp4_linear_workspace_size(T, K, N), x.device)
+            check(lib().dsmoe_mxfp4_linear(ptr(x2), x2.stride(0), T, K, N, ptr(weight.codes), ptr(weight.atoms),
+                                           ptr(out), ptr(ws), ws.numel(), ptr(weight.status),
+                                           stream_handle(x.device)), "dsmoe_mxfp4_linear")
+    return out
+
+
+def mxfp4_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
+    """``bf16(x @ W.T)`` for MXFP4 activations (``mxfp4_quantize``'s codes
+    [..., in/2] and scales [..., in/32]), fp32 sums."""
+    _check_weight("mxfp4_matmul", weight, False)
+    K = _check_pair("mxfp4_matmul", codes, scales)
+    _require("mxfp4_matmul", codes, weight.codes)
+    if K != weight.in_features:
+        raise ValueError(f"mxfp4_matmul: activations have {K} features, the weight {weight.in_features}")
+    shape, N = codes.shape[:-1], weight.out_features
+    c2, s2 = _dense(codes.reshape(-1, K // 2), 16), _dense(scales.reshape(-1, K // BLOCK), 4)
+    T = c2.shape[0]
+    out = torch.empty(*shape, N, dtype=torch.bfloat16, device=codes.device)
+    if T:
+        with torch.cuda.device(codes.device):
+            ws = _scratch(lib().dsmoe_mxfp4_matmul_workspace_size(T, K, N), codes.device)
+            check(lib().dsmoe_mxfp4_matmul(ptr(c2), ptr(s2), T, K, N, ptr(weight.codes), ptr(weight.atoms), ptr(out),
+                                           ptr(ws), ws.numel(), ptr(weight.status), stream_handle(codes.device)),
+                  "dsmoe_mxfp4_matmul")
+    return out
+
+
+def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Tensor,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows sorted by expert: rows ``offsets[e] .. offsets[e + 1]`` of ``x``
+    [R, in] (bf16) times expert e's weight -> bf16 [R, out]. ``offsets`` is
+    int32 [E + 1] on the device, never read by the host. Rows outside every
+    segment are zero in a new output and left as they are in ``out`` (dense
+    bf16 [R, out], which must not overlap ``x``)."""
+    _check_weight("mxfp4_grouped_linear", weight, True)
+    _check_x("mxfp4_grouped_linear", x, weight.in_features, offsets, out, weight.codes)
+    if x.dim() != 2:
+        raise ValueError("mxfp4_grouped_linear expects (rows, in) activations")
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != weight.experts + 1:
+        raise ValueError(f"offsets must be int32 with {weight.experts + 1} entries")
+    R, K, N = x.shape[0], weight.in_features, weight.out_features
+    clear = out is None
+    if clear:
+        out = torch.empty(R, N, dtype=torch.bfloat16, device=x.device)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (R, N) or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a dense, 16-byte aligned bf16 tensor ({R}, {N})")
+    if R:
+        x2, off = _rows(x, 16), offsets.contiguous()
+        with torch.cuda.device(x.device):
+            need = lib().dsmoe_mxfp4_grouped_linear_workspace_size(R, K, N, weight.experts)
+            ws = _scratch(need, x.device)
+            check(lib().dsmoe_mxfp4_grouped_linear(ptr(x2), x2.stride(0), R, K, N, weight.experts, ptr(off),
+                                                   ptr(weight.codes), ptr(weight.atoms), ptr(out), int(clear),
+                                                   ptr(ws) or None, ws.numel(), ptr(weight.status),
+                                                   stream_handle(x.device)), "dsmoe_mxfp4_grouped_linear")
+    return out
+
+
+class MXFP4Experts:
+    """The expert weights of one MoE layer: stacks ``gate`` and ``up``
+    [G, inter, hidden] and ``down`` [G, hidden, inter]; with ``shared`` matrix
+    0 is the shared expert and 1 + e routed expert e."""
+
+    def __init__(self, gate: MXFP4Weight, up: MXFP4Weight, down: MXFP4Weight, shared: bool = True):
+        for w in (gate, up, down):
+            _check_weight("MXFP4Experts", w, True)
+        self.hidden, self.inter = gate.in_features, gate.out_features
+        if (up.in_features, up.out_features) != (self.hidden, self.inter) or \
+                (down.in_features, down.out_features) != (self.inter, self.hidden) or \
+                not gate.experts == up.experts == down.experts:
+            raise ValueError("MXFP4Experts: gate and up are (G, inter, hidden), down is (G, hidden, inter)")
+        if not gate.device == up.device == down.device:
+            raise RuntimeError("MXFP4Experts: weights on different devices")
+        self.shared = bool(shared)
+        self.n_routed = gate.experts - int(self.shared)
+        if self.n_routed < 1:
+            raise ValueError("MXFP4Experts: no routed expert")
+        self.gate, self.up, self.down, self.device = gate, up, down, gate.device
+        self.desc = _lib.MXFP4ExpertsDesc(
+            hidden=self.hidden, inter=self.inter, n_routed=self.n_routed, shared=int(self.shared),
+            gate_codes=ptr(gate.codes), gate_atoms=ptr(gate.atoms), up_codes=ptr(up.codes), up_atoms=ptr(up.atoms),
+            down_codes=ptr(down.codes), down_atoms=ptr(down.atoms))
+
+    @property
+    def nbytes(self) -> int:
+        return self.gate.nbytes + self.up.nbytes + self.down.nbytes
+
+
+def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, experts: MXFP4Experts,
+              scale: float = 1.0) -> torch.Tensor:
+    """The routed FFN of a MoE layer on ``route``'s result (``topk_idx`` int64
+    and ``topk_w`` fp32, [..., top_k], top_k <= 8):
+    ``bf16(scale * sum_k w_k E_k(hidden) + E_shared(hidden))``,
+    ``E(x) = down(silu(gate(x)) * up(x))``, for bf16 ``hidden`` [..., hidden].
+    silu and the sum over experts are fp32; each expert's output row is
+    rounded to bf16. An id outside the routed experts adds nothing."""
+    if not isinstance(experts, MXFP4Experts):
+        raise TypeError("mxfp4_moe expects MXFP4Experts")
+    _check_x("mxfp4_moe", hidden, experts.hidden, topk_idx, topk_w, experts.gate.codes)
+    if topk_idx.dtype != torch.int64 or topk_w.dtype != torch.float32:
+        raise TypeError("mxfp4_moe expects int64 indices and fp32 weights")
+    lead = tuple(hidden.shape[:-1])
+    if topk_idx.dim() < 1 or topk_idx.shape != topk_w.shape or tuple(topk_idx.shape[:-1]) != lead:
+        raise ValueError(f"mxfp4_moe: indices {tuple(topk_idx.shape)} and weights {tuple(topk_w.shape)} do not go with "
+                         f"hidden {tuple(hidden.shape)}")
+    x2 = _rows(hidden, 16)
+    T, H, K = x2.shape[0], experts.hidden, topk_idx.shape[-1]
+    out = torch.empty(*lead, H, dtype=torch.bfloat16, device=hidden.device)
+    if T:
+        idx, w = topk_idx.contiguous(), topk_w.contiguous()
+        with torch.cuda.device(hidden.device):
+            ws = _scratch(lib().dsmoe_mxfp4_moe_workspace_size(T, H, experts.inter, experts.n_routed,
+                                                               int(experts.shared), K), hidden.device)
+            check(lib().dsmoe_mxfp4_moe(ptr(x2), x2.stride(0), T, ctypes.byref(experts.desc), ptr(idx), ptr(w), K,
+                                        float(scale), ptr(out), ptr(ws) or None, ws.numel(), ptr(experts.gate.status),
+                                        stream_handle(hidden.device)), "dsmoe_mxfp4_moe")
+    return out

@@ -417,6 +417,109 @@ DSMOE_API int dsmoe_sample_top_p(const float* logits, int32_t rows, int32_t voca
                                  float temperature, float top_p, const float* uniforms, int64_t* tokens,
                                  int32_t* nucleus_sizes, dsmoe_stream_t stream);
 
+/*
+ * MXFP4 (no counterpart in the reference, whose experts are FP8): the OCP
+ * microscaling format with 4-bit elements. A row of K numbers is K e2m1 codes
+ * (0, .5, 1, 1.5, 2, 3, 4, 6 and negatives; bit 3 is the sign; two per byte,
+ * the even element in the low nibble) and K/32 e8m0 scale bytes, one per 32
+ * consecutive numbers: byte b stands for 2^(b - 127), 255 for NaN. An expert
+ * takes 17/32 of its FP8 bytes.
+ *
+ * The entry points below enqueue on `stream`, allocate nothing and keep no
+ * state. `workspace` is scratch of at least the *_workspace_size bytes, 256-byte
+ * aligned, uninitialised, private to the call until it has run: calls that may
+ * run at the same time (two streams, two captured graphs) need two. Kernel
+ * errors (code of dsmoe_read_status) go to *device_status, a device int32 that
+ * starts at 0 and keeps the first error until the caller clears it. Row strides
+ * are in elements.
+ */
+enum { DSMOE_BF16 = 0, DSMOE_F16 = 1, DSMOE_F32 = 2, DSMOE_E4M3 = 3 };
+
+/*
+ * x [rows][row_stride], cols (% 32 == 0) numbers per row -> codes [rows][cols/2],
+ * scales [rows][cols/32]. Per block of 32, with a = max|v|:
+ * scale = 2^max(floor(log2 a) - 2, -127), codes rounded to nearest even and
+ * saturated at 6. A block with an infinity or a NaN gets scale byte 255 and
+ * codes 0, a zero block scale byte 0. DSMOE_E4M3 takes the checkpoint's form:
+ * scale_inv fp32 [rows / rows_per_matrix][ceil(rows_per_matrix/128)][ceil(cols/128)]
+ * multiplies 128x128 blocks, and the exact products are rounded (a product
+ * beyond fp32's largest number saturates there). Rows start on 16 bytes (e4m3: 8).
+ */
+DSMOE_API int dsmoe_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t row_stride,
+                                   const float* scale_inv, int64_t rows_per_matrix, void* codes, void* scales,
+                                   dsmoe_stream_t stream);
+/* blocks of 32 codes (16 bytes) and one scale byte -> 32 numbers of `dtype` (bf16, fp16, fp32), 16-byte aligned. */
+DSMOE_API int dsmoe_mxfp4_dequantize(const void* codes, const void* scales, int64_t blocks, int32_t dtype, void* out,
+                                     dsmoe_stream_t stream);
+
+/*
+ * The products read a weight's scales as 512-byte atoms (128 rows x 128
+ * numbers): scales [matrices][out][in/32] -> atoms, once per weight.
+ */
+DSMOE_API size_t dsmoe_mxfp4_scale_atoms_bytes(int32_t matrices, int32_t out_features, int32_t in_features);
+DSMOE_API int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_features, int32_t in_features,
+                                      void* atoms, dsmoe_stream_t stream);
+
+/*
+ * out[t][o] = bf16( sum_i x[t][i] * weight[o][i] ), x bf16, weight MXFP4 (codes
+ * 32-byte aligned), fp32 sums. in features a multiple of 128 up to 32768, out
+ * features a multiple of 8. A row of x with an infinity or a NaN comes out as
+ * NaN. Numbers below 2^-9 of the largest of their block of 32 are taken with an
+ * error of at most 2^-17 of it, all others exactly.
+ */
+DSMOE_API size_t dsmoe_mxfp4_linear_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features);
+DSMOE_API int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_t in_features,
+                                 int32_t out_features, const void* codes, const void* atoms, void* out,
+                                 void* workspace, size_t workspace_bytes, int32_t* device_status,
+                                 dsmoe_stream_t stream);
+/* The same product with MXFP4 activations (x_codes, x_scales of dsmoe_mxfp4_quantize, dense). */
+DSMOE_API size_t dsmoe_mxfp4_matmul_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features);
+DSMOE_API int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens, int32_t in_features,
+                                 int32_t out_features, const void* codes, const void* atoms, void* out,
+                                 void* workspace, size_t workspace_bytes, int32_t* device_status,
+                                 dsmoe_stream_t stream);
+/*
+ * Ragged products by expert: rows [offsets[e], offsets[e+1]) of x (offsets:
+ * device int32 [n_experts + 1], non-decreasing in [0, rows]) times expert e's
+ * weight, codes [n_experts][out][in/2]. Rows outside every segment are left as
+ * they are in `out`, or cleared with clear_rest. Offsets that decrease or leave
+ * the rows are clamped and reported (code 6). Up to 512 experts.
+ */
+DSMOE_API size_t dsmoe_mxfp4_grouped_linear_workspace_size(int32_t rows, int32_t in_features, int32_t out_features,
+                                                           int32_t n_experts);
+DSMOE_API int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, int32_t in_features,
+                                         int32_t out_features, int32_t n_experts, const int32_t* offsets,
+                                         const void* codes, const void* atoms, void* out, int32_t clear_rest,
+                                         void* workspace, size_t workspace_bytes, int32_t* device_status,
+                                         dsmoe_stream_t stream);
+/*
+ * The routed FFN of a MoE layer after dsmoe_route, with MXFP4 experts:
+ *   out[t] = bf16( scale * sum_k topk_w[t][k] E_{topk_idx[t][k]}(hidden[t]) + E_shared(hidden[t]) ),
+ *   E(x) = down(silu(gate(x)) * up(x)).
+ * Matrices: the shared expert first (if shared == 1), then the routed experts.
+ * silu and the product stay in fp32 and are split like activations; each
+ * expert's output row is rounded to bf16, the sum over experts is fp32 in
+ * top-k order. An id outside [0, n_routed) adds nothing. top_k <= 8.
+ */
+typedef struct {
+  int32_t hidden;    /* multiples of 128 */
+  int32_t inter;
+  int32_t n_routed;  /* n_routed + shared <= 512 */
+  int32_t shared;    /* 0 or 1 */
+  const void* gate_codes; /* [n_routed + shared][inter][hidden/2] */
+  const void* gate_atoms;
+  const void* up_codes;
+  const void* up_atoms;
+  const void* down_codes; /* [n_routed + shared][hidden][inter/2] */
+  const void* down_atoms;
+} dsmoe_mxfp4_experts_t;
+DSMOE_API size_t dsmoe_mxfp4_moe_workspace_size(int32_t tokens, int32_t hidden, int32_t inter, int32_t n_routed,
+                                                int32_t shared, int32_t top_k);
+DSMOE_API int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens,
+                              const dsmoe_mxfp4_experts_t* weights, const int64_t* topk_idx, const float* topk_w,
+                              int32_t top_k, float scale, void* out, void* workspace, size_t workspace_bytes,
+                              int32_t* device_status, dsmoe_stream_t stream);
+
 /* Reads (synchronously) and clears the device error word kept in `workspace`.
  * workspace == NULL reads the error word of dsmoe_expert_ffn_noalloc's
  * library-owned scratch on the current device: that entry point has no
