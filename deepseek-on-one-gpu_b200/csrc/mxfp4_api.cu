@@ -40,7 +40,7 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Token tile of a product over `rows` rows of one group.
 int linear_tile(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 160; }
-int fp4_tile(int rows) { return rows <= 64 ? 64 : 192; }
+int fp4_tile(int rows) { return rows <= 64 ? 64 : 176; }
 // Token tile where `rows` rows spread over `groups` experts.
 int grouped_tile(long long rows, int groups) {
   const long long mean = (rows + groups - 1) / groups;

@@ -19,8 +19,9 @@
 //
 // Warp roles (one CTA per SM, persistent):
 //   warp 0     TMA producer (one thread)
-//   warp 1     TMEM allocator, MMA issuer (one thread): per stage it copies the
-//              scale atoms to TMEM (tcgen05.cp) and issues the MMAs behind them
+//   warps 1, 2 MMA issuers (one thread each; warp 1 also allocates TMEM), one
+//              for each A tile: per stage the thread copies the scale atoms to
+//              its TMEM columns (tcgen05.cp) and issues the MMAs behind them
 //   warp 3     unit planner, a shared-memory ring of decoded units
 //   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 16-column chunks
 // TMEM: two halves of accumulator columns, then one set of scale columns per
@@ -77,9 +78,9 @@ struct Cfg {
   static constexpr int SF_BYTES = 2 * SFA_BYTES + SFB_BYTES;
   static constexpr int SF0 = STAGES * OP_BYTES;
   // TMEM columns
-  static constexpr int SF_COLS = KB_STAGE * (2 + ATOMS) * 4;
-  static constexpr int SF_TOTAL = STAGES * SF_COLS <= 64 ? 64 : 128;
-  static constexpr int HALF = (512 - SF_TOTAL) / 2;
+  static constexpr int SF_COLS = KB_STAGE * (1 + ATOMS) * 4;  // of one issuer and stage
+  static constexpr int SF_TOTAL = STAGES * 2 * SF_COLS;
+  static constexpr int HALF = (512 - SF_TOTAL) / 2 / 16 * 16;
   static constexpr int SF_BASE = 2 * HALF;
   static constexpr int BAR_OFF = STAGES * (OP_BYTES + SF_BYTES);
   // full[S], empty[S], tfull[2], tempty[2], done, ufull[RING], uempty[RING]
@@ -89,7 +90,7 @@ struct Cfg {
   static constexpr int SMEM = PLAN_OFF + RING * static_cast<int>(sizeof(Unit)) + 1024;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(OP_BYTES % 1024 == 0, "operand alignment");
-  static_assert(STAGES * SF_COLS <= SF_TOTAL, "scale columns");
+  static_assert(HALF >= BN && (FP4 || 4 * (BN < 96 ? BN : 96) <= 2 * HALF), "accumulator columns");
 };
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -129,13 +130,26 @@ __device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, u
 }
 
 // Instruction descriptor of the block-scaled kinds: D fp32, both operands
-// K-major, e8m0 scales; A e2m1, B e4m3 (mxf8f6f4) or e2m1 (mxf4). `sf` is the
-// byte of the 32-bit scale word this MMA's K starts at.
+// K-major, e8m0 scales; A e2m1, B e4m3 (mxf8f6f4) or e2m1 (mxf4). sf_id is
+// the byte of the 32-bit scale words an MMA's K starts at.
 template <bool FP4>
-__device__ __forceinline__ uint32_t idesc_scaled(int n, int sf) {
+__device__ __forceinline__ uint32_t idesc_scaled(int n) {
   const uint32_t at = FP4 ? 1u : 5u, bt = FP4 ? 1u : 0u;
-  return (static_cast<uint32_t>(sf) << 4) | (at << 7) | (bt << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
-         (static_cast<uint32_t>(BM >> 7) << 27) | (static_cast<uint32_t>(sf) << 29);
+  return (at << 7) | (bt << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(BM >> 7) << 27);
+}
+__device__ __forceinline__ constexpr uint32_t sf_id(int sf) {
+  return (static_cast<uint32_t>(sf) << 4) | (static_cast<uint32_t>(sf) << 29);
+}
+struct True { static constexpr bool value = true; };
+struct False { static constexpr bool value = false; };
+
+// One thread of a converged warp. The compiler knows that a single thread is
+// active behind it, so that descriptors go to uniform registers once.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
 }
 
 template <class C, bool SWIGLU>
@@ -228,16 +242,16 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);  // both issuers
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&tfull[b], 1);
+      mbar_init(&tfull[b], 2);
       mbar_init(&tempty[b], kEpiWarps);
     }
-    mbar_init(done_bar, 1);
+    mbar_init(done_bar, 2);
     for (int r = 0; r < RING; ++r) {
       mbar_init(&ufull[r], 1);
-      mbar_init(&uempty[r], 2 + kEpiWarps);  // producer, issuer, epilogue warps
+      mbar_init(&uempty[r], 3 + kEpiWarps);  // producer, issuers, epilogue warps
     }
     *s_abort = 0;
     fence_mbar_init();
@@ -270,7 +284,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     }
   } else if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t pol_w = policy_evict_first(), pol_x = policy_evict_last();
       int stage = 0, issued = 0, i = 0;
       uint32_t phase = 0;
@@ -319,18 +333,22 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         mbar_wait_settle(&full[stage], phase, p.status, kDevTimeoutProducer);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 2) {
     // ----------------------------------------------------------------- MMA
-    if (lane == 0) {
+    if (elect_one()) {
+      const int me = warp - 1;  // this thread's A tile
+      const uint32_t op0 = smem_u32(smem) + me * C::A_BYTES;
+      const uint32_t sf0 = smem_u32(smem + C::SF0);
+      const uint32_t tsf0 = tmem + C::SF_BASE + me * C::SF_COLS;
       int stage = 0, nb = 0, i = 0;
       uint32_t phase = 0, tphase = 0;  // tphase: one bit per half
       bool ok = true;
       for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
         const int ri = i % RING;
         if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutMma, s_abort)) break;
-        const Unit e = plan[ri];
+        const int m1 = plan[ri].m1, n = plan[ri].n, both = plan[ri].both, kb0 = plan[ri].kb0, kb1 = plan[ri].kb1;
         mbar_arrive(&uempty[ri]);
-        const int nn = e.both ? 2 * e.n : e.n;  // columns of one accumulator
+        const int nn = both ? 2 * n : n;  // columns of one accumulator
         const bool big = 2 * nn > C::HALF;
         const int b0 = big ? 0 : nb, b1 = big ? 1 : nb;
         for (int b = b0; b <= b1 && ok; ++b) {
@@ -338,37 +356,43 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           tphase ^= 1u << b;
         }
         if (!ok) break;
-        const uint32_t d0 = tmem + b0 * C::HALF, d1 = d0 + nn;
-        const bool two = e.m1 >= 0;
-        for (int kb = e.kb0; kb < e.kb1; kb += C::KB_STAGE) {
+        const uint32_t d = tmem + b0 * C::HALF + me * nn;
+        const bool mine = me == 0 || m1 >= 0;
+        const uint32_t id0 = idesc_scaled<FP4>(nn);
+        // One stage: scale atoms to TMEM, then its MMAs, all in order.
+        auto issue = [&](int nkb, auto two_terms, uint32_t acc) {
+          const uint32_t st = op0 + stage * C::OP_BYTES;
+          const uint32_t sb = op0 - me * C::A_BYTES + stage * C::OP_BYTES + C::B_OFF;
+          const uint32_t sf = sf0 + stage * C::SF_BYTES;
+          const uint32_t ta = tsf0 + stage * (2 * C::SF_COLS), tb = ta + C::KB_STAGE * 4;
+          const uint64_t da = umma_desc_sw128(st), db = umma_desc_sw128(sb), dl = umma_desc_sw128(sb + BN * 128);
+#pragma unroll
+          for (int h = 0; h < C::KB_STAGE; ++h) {
+            if (h < nkb) {
+              copy_scales(ta + h * 4, sf + me * C::SFA_BYTES + h * 512);
+#pragma unroll
+              for (int a = 0; a < C::ATOMS; ++a)
+                copy_scales(tb + (h * C::ATOMS + a) * 4, sf + 2 * C::SFA_BYTES + (h * C::ATOMS + a) * 512);
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {  // 32 bytes of a row each
+            const int h = FP4 ? kk >> 1 : 0;
+            if (h < nkb) {
+              const uint32_t id = id0 | sf_id(FP4 ? (kk & 1) * 2 : kk);
+              const uint32_t va = ta + h * 4, vb = tb + h * C::ATOMS * 4;
+              mma_scaled<FP4>(d, da + 2 * kk, db + 2 * kk, id, va, vb, kk ? 1u : acc);
+              if constexpr (decltype(two_terms)::value) mma_scaled<FP4>(d, da + 2 * kk, dl + 2 * kk, id, va, vb, 1u);
+            }
+          }
+        };
+        for (int kb = kb0; kb < kb1; kb += C::KB_STAGE) {
           if (!mbar_wait(&full[stage], phase, p.status, kDevTimeoutMma, s_abort)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + stage * C::OP_BYTES);
-          const uint32_t sf = smem_u32(smem + C::SF0 + stage * C::SF_BYTES);
-          const uint32_t tsa = tmem + C::SF_BASE + stage * C::SF_COLS;
-          const uint32_t tsb = tsa + C::KB_STAGE * 8;
-          const int nkb = min(C::KB_STAGE, e.kb1 - kb);
-          for (int h = 0; h < nkb; ++h) {
-            copy_scales(tsa + h * 8, sf + h * 512);
-            if (two) copy_scales(tsa + h * 8 + 4, sf + C::SFA_BYTES + h * 512);
-#pragma unroll
-            for (int a = 0; a < C::ATOMS; ++a)
-              copy_scales(tsb + (h * C::ATOMS + a) * 4, sf + 2 * C::SFA_BYTES + (h * C::ATOMS + a) * 512);
-          }
-          const uint64_t da0 = umma_desc_sw128(st), da1 = umma_desc_sw128(st + C::A_BYTES);
-          const uint64_t db = umma_desc_sw128(st + C::B_OFF), dl = umma_desc_sw128(st + C::B_OFF + BN * 128);
-          const int steps = FP4 ? 2 * nkb : 4;  // 32 bytes of a row each
-          for (int kk = 0; kk < steps; ++kk) {
-            const uint32_t id = FP4 ? idesc_scaled<true>(nn, (kk & 1) * 2) : idesc_scaled<false>(nn, kk);
-            const uint32_t a0 = tsa + (FP4 ? (kk >> 1) * 8 : 0);
-            const uint32_t sb = tsb + (FP4 ? (kk >> 1) * C::ATOMS * 4 : 0);
-            const uint32_t acc = kb > e.kb0 || kk > 0;
-            mma_scaled<FP4>(d0, da0 + 2 * kk, db + 2 * kk, id, a0, sb, acc);
-            if (!FP4 && !e.both) mma_scaled<FP4>(d0, da0 + 2 * kk, dl + 2 * kk, id, a0, sb, 1);
-            if (two) {
-              mma_scaled<FP4>(d1, da1 + 2 * kk, db + 2 * kk, id, a0 + 4, sb, acc);
-              if (!FP4 && !e.both) mma_scaled<FP4>(d1, da1 + 2 * kk, dl + 2 * kk, id, a0 + 4, sb, 1);
-            }
+          if (mine) {
+            const uint32_t acc = kb > kb0;
+            if (FP4 || both) issue(min(C::KB_STAGE, kb1 - kb), False{}, acc);
+            else issue(1, True{}, acc);
           }
           mma_commit(&empty[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -377,7 +401,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         for (int b = b0; b <= b1; ++b) mma_commit(&tfull[b]);
         if (!big) nb ^= 1;
       }
-      // Every MMA ends before TMEM is freed, also after an abort.
+      // Every MMA of both issuers ends before TMEM is freed, also after an abort.
       mma_commit(done_bar);
       mbar_wait_settle(done_bar, 0, p.status, kDevTimeoutMma);
     }
@@ -569,7 +593,7 @@ cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUte
   if (fp4) {
     switch (tile) {
       case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
-      case 192: return launch<Cfg<true, 192, 3>, false>(w0, w1, x, x32, a, grid, s);
+      case 176: return launch<Cfg<true, 176, 3>, false>(w0, w1, x, x32, a, grid, s);
       default: return cudaErrorInvalidValue;
     }
   }
