@@ -28,6 +28,7 @@ namespace mx {
 
 constexpr int kMaxGroups = 512;
 constexpr int kEpiWarps = 16;
+constexpr int kMaxSplit = 8;  // CTAs of a cluster that share one tile's K
 
 // Token tiles of the product kernels: columns of one work unit, and 512-byte
 // scale atoms per token tile and K block.
@@ -60,15 +61,13 @@ struct GemmArgs {
   int M;                 // features of one weight matrix
   int K;
   int P;                 // first lo row of the split activations
-  int ksplit;            // parts of K per tile (1 unless g.counts == NULL)
+  int ksplit;            // parts of K per tile, a cluster's CTAs (1 unless g.counts == NULL)
   const uint8_t* sfa0;   // scale atoms of the weights [group][ceil(M/128)][K/128][512]
   const uint8_t* sfa1;   // up projection (SwiGLU), else == sfa0
   const uint8_t* sfb;    // scale atoms of the rows [tile][K/128][tile_atoms][512]
   __nv_bfloat16* y;      // [row][M]
   uint8_t* hq;           // SwiGLU: split rows [2][P][M] and their atoms
   uint8_t* hsf;
-  float* partial;        // ksplit > 1: [tile unit][ksplit][column][256]
-  int32_t* arrived;      // ksplit > 1: [tile unit][kEpiWarps], zero before the launch
   int* status;
 };
 
@@ -78,9 +77,8 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
 cudaError_t launch_dequantize(const uint8_t* codes, const uint8_t* scales, long long blocks, int type, void* out,
                               cudaStream_t s);
 // Scales [mats][N][K/32] -> atoms [mats][ceil(N/tile)][K/128][atoms][512].
-// zero (optional): n_zero counters cleared by the same launch.
 cudaError_t launch_tile_scales(const uint8_t* scales, int mats, int N, int K, int tile, int atoms, uint8_t* out,
-                               int32_t* zero, int n_zero, cudaStream_t s);
+                               cudaStream_t s);
 
 // --------------------------------------------------------- mxfp4_prep.cu
 // Segments of rows sorted by expert from offsets[n + 1].
@@ -95,15 +93,15 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 // else token t goes to the rows pos names (and to row t of group 0 with shared).
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
                          const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
-                         __nv_bfloat16* zero_out, int M, int32_t* zero, int n_zero, cudaStream_t s);
+                         __nv_bfloat16* zero_out, int M, cudaStream_t s);
 // out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
                            int shared, float scale, __nv_bfloat16* out, cudaStream_t s);
 
 // --------------------------------------------------------- mxfp4_gemm.cu
-// Largest K split of a single-group product that keeps its grid within one
-// wave; units: (feature tile pair, token tile) pairs.
-int pick_ksplit(int units, int kblocks, int sms);
+// K split of a single-group product of `units` (feature tile pair, token tile)
+// pairs on the current device.
+int pick_ksplit(bool fp4, int tile, int units, int kblocks);
 cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
                         const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s);
 

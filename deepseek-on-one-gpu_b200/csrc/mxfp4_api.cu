@@ -40,7 +40,7 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Token tile of a product over `rows` rows of one group.
 int linear_tile(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 160; }
-int fp4_tile(int rows) { return rows <= 64 ? 64 : 176; }
+int fp4_tile(int rows) { return rows <= 64 ? 64 : 160; }
 // Token tile where `rows` rows spread over `groups` experts.
 int grouped_tile(long long rows, int groups) {
   const long long mean = (rows + groups - 1) / groups;
@@ -48,8 +48,7 @@ int grouped_tile(long long rows, int groups) {
 }
 
 struct Plan {
-  size_t counts = 0, row_start = 0, tile_start = 0, pos = 0, xq = 0, sf = 0, hq = 0, hsf = 0, y = 0, partial = 0,
-         arrived = 0, total = 0;
+  size_t counts = 0, row_start = 0, tile_start = 0, pos = 0, xq = 0, sf = 0, hq = 0, hsf = 0, y = 0, total = 0;
   int tile = 32, P = 0, ksplit = 1, units = 0;
   long long tiles = 0;
   size_t take(size_t bytes) {
@@ -63,36 +62,28 @@ struct Plan {
     tile_start = take(4 * (static_cast<size_t>(groups) + 1));
   }
   size_t atoms(int K) const { return static_cast<size_t>(tiles) * (K / 128) * mx::tile_atoms(tile) * 512; }
-  void split_k(int N, int K, int kb_stage) {
+  void split_k(bool fp4, int N, int K) {
     units = static_cast<int>(tiles) * ceil_div(N, 256);
-    ksplit = mx::pick_ksplit(units, K / 128, sm_count());
-    if (ceil_div(K / 128, kb_stage) < ksplit) ksplit = ceil_div(K / 128, kb_stage);
-    if (ksplit > 1) {
-      partial = take(sizeof(float) * units * ksplit * static_cast<size_t>(tile) * 256);
-      arrived = take(4 * static_cast<size_t>(units) * mx::kEpiWarps);
-    }
+    ksplit = mx::pick_ksplit(fp4, tile, units, K / 128);
   }
-  int counters() const { return ksplit > 1 ? units * mx::kEpiWarps : 0; }
 };
 
-Plan plan_linear(int T, int K, int N) {
+Plan plan_linear(int T, int K) {
   Plan w;
   w.tile = linear_tile(T);
   w.P = T;
   w.tiles = ceil_div(T, w.tile);
   w.xq = w.take(2 * static_cast<size_t>(T) * K);
   w.sf = w.take(w.atoms(K));
-  w.split_k(N, K, 1);
   return w;
 }
 
-Plan plan_matmul(int T, int K, int N) {
+Plan plan_matmul(int T, int K) {
   Plan w;
   w.tile = fp4_tile(T);
   w.P = T;
   w.tiles = ceil_div(T, w.tile);
   w.sf = w.take(w.atoms(K));
-  w.split_k(N, K, 2);
   return w;
 }
 
@@ -173,7 +164,8 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
     if ((r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
     if ((r = make_tma_map(&m_x32, u8, a.K, x, a.K, rows, 128, 32))) return r;
   }
-  const int g = gemm_grid();
+  // A split tile is a cluster, one unit per CTA; otherwise persistent CTAs.
+  const int g = a.ksplit > 1 ? static_cast<int>(max_units) : gemm_grid();
   MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, a, tile, max_units < g ? static_cast<int>(max_units) : g, s));
   return DSMOE_OK;
 }
@@ -240,13 +232,13 @@ int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_fe
   if (matrices < 1 || !aligned(scales, 4) || !aligned(atoms, 16))
     return fail(DSMOE_ERR_INVALID, "mxfp4_scale_atoms: no matrix, or pointer NULL or unaligned");
   MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(scales), matrices, out_features, in_features, 128, 1,
-                                 static_cast<uint8_t*>(atoms), nullptr, 0, reinterpret_cast<cudaStream_t>(stream)));
+                                 static_cast<uint8_t*>(atoms), reinterpret_cast<cudaStream_t>(stream)));
   return DSMOE_OK;
 }
 
 size_t dsmoe_mxfp4_linear_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features) {
   if (check_shape("mxfp4_linear", tokens, in_features, out_features) || tokens == 0) return 0;
-  return plan_linear(tokens, in_features, out_features).total;
+  return plan_linear(tokens, in_features).total;
 }
 
 int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_t in_features, int32_t out_features,
@@ -260,8 +252,9 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: pointer NULL or not 16-byte aligned");
   if (tokens > 1 && (row_stride < in_features || row_stride % 8))
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: rows must not overlap and must start on 16 bytes");
-  const Plan L = plan_linear(tokens, in_features, out_features);
+  Plan L = plan_linear(tokens, in_features);
   if ((r = check_ws("mxfp4_linear", workspace, workspace_bytes, L.total))) return r;
+  L.split_k(false, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   mx::GemmArgs a{};
   a.g.n = 1;
@@ -273,19 +266,16 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
   a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
-  a.partial = at<float>(workspace, L.partial);
-  a.arrived = at<int32_t>(workspace, L.arrived);
   a.status = device_status;
   MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, tokens, in_features, a.g, L.tile, nullptr,
-                           0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, a.arrived,
-                           L.counters(), s));
+                           0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
   return run_gemm(false, false, codes, codes, 1, at<uint8_t>(workspace, L.xq), a, L.tile,
                   static_cast<long long>(L.units) * L.ksplit, s);
 }
 
 size_t dsmoe_mxfp4_matmul_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features) {
   if (check_shape("mxfp4_matmul", tokens, in_features, out_features) || tokens == 0) return 0;
-  return plan_matmul(tokens, in_features, out_features).total;
+  return plan_matmul(tokens, in_features).total;
 }
 
 int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens, int32_t in_features,
@@ -297,8 +287,9 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   if ((r = check_weight("mxfp4_matmul", codes, atoms))) return r;
   if (!aligned(x_codes, 16) || !aligned(x_scales, 4) || !aligned(out, 16) || !aligned(device_status, 4))
     return fail(DSMOE_ERR_INVALID, "mxfp4_matmul: pointer NULL or unaligned");
-  const Plan L = plan_matmul(tokens, in_features, out_features);
+  Plan L = plan_matmul(tokens, in_features);
   if ((r = check_ws("mxfp4_matmul", workspace, workspace_bytes, L.total))) return r;
+  L.split_k(true, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   mx::GemmArgs a{};
   a.g.n = 1;
@@ -310,11 +301,9 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
-  a.partial = at<float>(workspace, L.partial);
-  a.arrived = at<int32_t>(workspace, L.arrived);
   a.status = device_status;
   MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(x_scales), 1, tokens, in_features, L.tile,
-                                 mx::tile_atoms(L.tile), at<uint8_t>(workspace, L.sf), a.arrived, L.counters(), s));
+                                 mx::tile_atoms(L.tile), at<uint8_t>(workspace, L.sf), s));
   return run_gemm(true, false, codes, codes, 1, static_cast<const uint8_t*>(x_codes), a, L.tile,
                   static_cast<long long>(L.units) * L.ksplit, s);
 }
@@ -359,7 +348,7 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
                               s));
   MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, rows, in_features, a.g, L.tile, nullptr, 0,
                            0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf),
-                           clear_rest ? a.y : nullptr, out_features, nullptr, 0, s));
+                           clear_rest ? a.y : nullptr, out_features, s));
   return run_gemm(false, false, codes, codes, n_experts, at<uint8_t>(workspace, L.xq), a, L.tile,
                   L.tiles * ceil_div(out_features, 256), s);
 }
@@ -420,8 +409,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, at<int32_t>(workspace, L.counts),
                                 at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), pos, s));
   MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(hidden), row_stride, tokens, H, a.g, L.tile, pos, top_k,
-                           shared, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, nullptr,
-                           0, s));
+                           shared, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
   if ((r = run_gemm(false, true, w->gate_codes, w->up_codes, G, at<uint8_t>(workspace, L.xq), a, L.tile,
                     L.tiles * (F / 128), s)))
     return r;

@@ -53,7 +53,6 @@ struct Unit {
   int32_t both;    // hi and lo side by side (N = 2 n)
   int32_t kb0, kb1;
   int32_t part;    // K part
-  int32_t id;      // tile unit (split-K bookkeeping)
 };
 
 template <bool FP4_, int BN_, int STAGES_>
@@ -87,8 +86,10 @@ struct Cfg {
   static constexpr int NUM_BARS = 2 * STAGES + 5 + 2 * RING;
   static constexpr int MISC_OFF = BAR_OFF + 8 * NUM_BARS;
   static constexpr int PLAN_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
-  static constexpr int SMEM = PLAN_OFF + RING * static_cast<int>(sizeof(Unit)) + 1024;
+  static constexpr int TAB_OFF = PLAN_OFF + RING * static_cast<int>(sizeof(Unit));
+  static constexpr int SMEM = TAB_OFF + (FP4 ? 0 : 4 * (kMaxGroups + 1)) + 1024;  // group table; kind::mxf4 has none
   static_assert(SMEM <= 232448, "shared memory");
+  static_assert(STAGES * OP_BYTES >= BN * 2 * BM * 4, "a K part's sums");
   static_assert(OP_BYTES % 1024 == 0, "operand alignment");
   static_assert(HALF >= BN && (FP4 || 4 * (BN < 96 ? BN : 96) <= 2 * HALF), "accumulator columns");
 };
@@ -129,6 +130,20 @@ __device__ __forceinline__ void mma_scaled(uint32_t d, uint64_t a, uint64_t b, u
         : "memory");
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Two floats at this CTA's shared-memory address `p`, read in CTA `rank` of
+// the cluster.
+__device__ __forceinline__ float2 load_peer(const float* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
 // Instruction descriptor of the block-scaled kinds: D fp32, both operands
 // K-major, e8m0 scales; A e2m1, B e4m3 (mxf8f6f4) or e2m1 (mxf4). sf_id is
 // the byte of the 32-bit scale words an MMA's K starts at.
@@ -152,24 +167,24 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// `tiles` is the tile_start table (in shared memory), unused without groups.
 template <class C, bool SWIGLU>
-__device__ __forceinline__ Unit decode(int u, const GemmArgs& p) {
+__device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tiles) {
   Unit e;
   const int per = SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
   const int id = p.ksplit > 1 ? u / p.ksplit : u;
-  e.id = id;
   e.part = u - id * p.ksplit;
   int g = 0, rows = p.g.rows, row_start = 0, tile0 = 0, ntiles;
   if (p.g.counts) {
     int lo = 0, hi = p.g.n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(p.g.tile_start + mid) * per <= id) lo = mid; else hi = mid;
+      if (tiles[mid] * per <= id) lo = mid; else hi = mid;
     }
     g = lo;
     rows = __ldg(p.g.counts + g);
     row_start = __ldg(p.g.row_start + g);
-    tile0 = __ldg(p.g.tile_start + g);
+    tile0 = tiles[g];
   }
   ntiles = (rows + C::BN - 1) / C::BN;
   const int local = id - tile0 * per;
@@ -272,10 +287,16 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
 
   if (warp == PLAN_WARP) {
     // ------------------------------------------------------------- planner
+    // The search for a unit's group walks a shared-memory copy of the table:
+    // nine dependent global loads would be ~3 us before the first copy.
+    int* tiles = reinterpret_cast<int*>(smem + C::TAB_OFF);
+    if (p.g.counts)
+      for (int t = lane; t <= p.g.n; t += 32) tiles[t] = __ldg(p.g.tile_start + t);
+    __syncwarp();
     if (lane == 0) {
       int i = 0;
       for (int u = blockIdx.x; u < total; u += gridDim.x, ++i) {
-        const Unit e = decode<C, SWIGLU>(u, p);
+        const Unit e = decode<C, SWIGLU>(u, p, tiles);
         const int ri = i % RING;
         if (!mbar_wait(&uempty[ri], ((i / RING) & 1) ^ 1, p.status, kDevTimeoutProducer, s_abort)) break;
         plan[ri] = e;
@@ -511,41 +532,16 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
             }
           }
         } else {
-          // Every part leaves its sums in `partial`; the warp that arrives
-          // last on its (tile, quadrant, column group) adds the parts up in
-          // part order, so the result does not depend on who that is.
-          const size_t part_sz = static_cast<size_t>(C::BN) * 2 * BM;
-          float* all = p.partial + static_cast<size_t>(e.id) * p.ksplit * part_sz + quad * 32 + lane;
-          float* mine = all + e.part * part_sz;
+          // This part's sums, fp32, into the (now unused) operand stages:
+          // [column][256 features].
+          float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
           for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
             float v[CHUNK];
             for (int a = 0; a < (two ? 2 : 1); ++a) {
               load(a ? d1 : d0, c0, v);
 #pragma unroll
               for (int j = 0; j < CHUNK; ++j)
-                if (c0 + j < e.ncols) mine[(c0 + j) * 2 * BM + a * BM] = v[j];
-            }
-          }
-          __threadfence();
-          __syncwarp();
-          int last = 0;
-          if (lane == 0) last = atomicAdd(p.arrived + e.id * kEpiWarps + warp - EPI_WARP0, 1) == p.ksplit - 1;
-          last = __shfl_sync(0xffffffffu, last, 0);
-          if (last) {
-            __threadfence();
-            for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
-              for (int a = 0; a < (two ? 2 : 1); ++a) {
-                float v[CHUNK];
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) v[j] = 0.f;
-                for (int s = 0; s < p.ksplit; ++s)
-#pragma unroll
-                  for (int j = 0; j < CHUNK; ++j)
-                    if (c0 + j < e.ncols) v[j] += __ldcg(all + s * part_sz + (c0 + j) * 2 * BM + a * BM);
-                const int m = a ? e.m1 : e.m0;
-                store_pairs(v, c0, e.ncols, m + ld_feat < p.M, p.y + static_cast<size_t>(e.row0) * p.M + m + ld_feat,
-                            p.M, lane);
-              }
+                if (c0 + j < e.ncols) part[(c0 + j) * 2 * BM + a * BM] = v[j];
             }
           }
         }
@@ -560,32 +556,103 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, 512);
+  if constexpr (!SWIGLU) {
+    if (p.ksplit > 1) {
+      // The cluster's CTAs hold the parts of one tile. Each adds up its share
+      // of the columns over all of them, in part order, from their shared
+      // memory. Every thread of every CTA passes both barriers, also after an
+      // abort (the sums are then meaningless and the status says so).
+      cluster_sync();
+      const Unit e = plan[0];  // the CTA's only unit
+      const int m = 2 * (threadIdx.x & 127);
+      if (e.m0 + m < p.M) {
+        const float* mine = reinterpret_cast<const float*>(smem) + m;
+        for (int c = e.part + p.ksplit * (threadIdx.x >> 7); c < e.ncols; c += p.ksplit * (THREADS / 128)) {
+          float2 v[kMaxSplit];
+#pragma unroll
+          for (int s = 0; s < kMaxSplit; ++s)
+            if (s < p.ksplit) v[s] = load_peer(mine + c * 2 * BM, s);
+          float x = 0.f, y = 0.f;
+#pragma unroll
+          for (int s = 0; s < kMaxSplit; ++s)
+            if (s < p.ksplit) x += v[s].x, y += v[s].y;
+          *reinterpret_cast<__nv_bfloat162*>(p.y + static_cast<size_t>(e.row0 + c) * p.M + e.m0 + m) =
+              __floats2bfloat162_rn(x, y);
+        }
+      }
+      cluster_sync();  // no CTA exits while another reads its shared memory
+    }
+  }
+}
+
+template <class C, bool SWIGLU>
+cudaError_t prepare(int* dev) {
+  static bool attr[64] = {false};
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return e;
+  if (*dev < 0 || *dev >= 64) return cudaErrorInvalidDevice;
+  if (!attr[*dev]) {
+    e = cudaFuncSetAttribute(mx_gemm_kernel<C, SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    attr[*dev] = true;
+  }
+  return cudaSuccess;
+}
+
+template <class C>
+cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int cluster) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = THREADS;
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cfg.attrs = at;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cfg;
 }
 
 template <class C, bool SWIGLU>
 cudaError_t launch(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& x32,
                    const GemmArgs& a, int grid, cudaStream_t s) {
-  static bool attr[64] = {false};
   int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  const cudaError_t e = prepare<C, SWIGLU>(&dev);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!attr[dev]) {
-    e = cudaFuncSetAttribute(mx_gemm_kernel<C, SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
-    attr[dev] = true;
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg = config<C>(grid, s, at, a.ksplit);
+  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<C, SWIGLU>, w0, w1, x, x32, a);
+}
+
+// Clusters of `split` CTAs that run at the same time on the current device.
+template <class C>
+int resident_clusters(int split) {
+  static int cache[64][kMaxSplit + 1] = {};
+  int dev = 0;
+  if (prepare<C, false>(&dev) != cudaSuccess) return 0;
+  int& n = cache[dev][split];
+  if (n == 0) {
+    cudaLaunchAttribute at[2];
+    cudaLaunchConfig_t cfg = config<C>(split, nullptr, at, split);
+    if (cudaOccupancyMaxActiveClusters(&n, mx_gemm_kernel<C, false>, &cfg) != cudaSuccess) n = -1;
   }
-  mx_gemm_kernel<C, SWIGLU><<<grid, THREADS, C::SMEM, s>>>(w0, w1, x, x32, a);
-  return cudaGetLastError();
+  return n;
 }
 
 }  // namespace
 
-int pick_ksplit(int units, int kblocks, int sms) {
-  int s = sms / (units > 0 ? units : 1);
-  if (s > kblocks / 4) s = kblocks / 4;  // at least four K blocks a part
-  if (s > 16) s = 16;
-  return s < 1 ? 1 : s;
+// The widest split that keeps four K blocks per part and runs in one wave.
+int pick_ksplit(bool fp4, int tile, int units, int kblocks) {
+  int best = 1;
+  for (int s = 2; s <= kMaxSplit && s * 4 <= kblocks; ++s) {
+    int n = 0;
+    if (fp4) n = tile == 64 ? resident_clusters<Cfg<true, 64, 4>>(s) : resident_clusters<Cfg<true, 160, 4>>(s);
+    else n = tile == 32 ? resident_clusters<Cfg<false, 32, 5>>(s)
+             : tile == 64 ? resident_clusters<Cfg<false, 64, 4>>(s) : resident_clusters<Cfg<false, 160, 3>>(s);
+    if (n >= units) best = s;
+  }
+  return best;
 }
 
 cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
@@ -593,7 +660,7 @@ cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUte
   if (fp4) {
     switch (tile) {
       case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
-      case 176: return launch<Cfg<true, 176, 3>, false>(w0, w1, x, x32, a, grid, s);
+      case 160: return launch<Cfg<true, 160, 4>, false>(w0, w1, x, x32, a, grid, s);
       default: return cudaErrorInvalidValue;
     }
   }

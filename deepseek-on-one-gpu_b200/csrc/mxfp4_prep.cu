@@ -160,13 +160,11 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
                                                     int K, const Groups g, const int32_t* __restrict__ pos, int top_k,
                                                     int shared, int P, uint8_t* __restrict__ xq,
                                                     uint8_t* __restrict__ sf, __nv_bfloat16* __restrict__ zero_out,
-                                                    int M, int32_t* __restrict__ zero, int n_zero) {
+                                                    int M) {
   constexpr int MAXR = 9;
   const int t = blockIdx.x;
   const int tid = threadIdx.x;
   const int KB = K / 128;
-  if (t == 0 && blockIdx.y == 0)
-    for (int i = tid; i < n_zero; i += 256) zero[i] = 0;
   __shared__ int s_row[MAXR];
   __shared__ SfSpot s_spot[MAXR];
   const int n = pos ? top_k + shared : 1;
@@ -305,10 +303,10 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
                          const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
-                         __nv_bfloat16* zero_out, int M, int32_t* zero, int n_zero, cudaStream_t s) {
+                         __nv_bfloat16* zero_out, int M, cudaStream_t s) {
   const dim3 grid(T, (K + 2047) / 2048);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, s>>>(x, row_stride, T, K, g, pos, top_k, shared, P, xq, sf, zero_out, M, zero, n_zero);
+    kern<<<grid, 256, 0, s>>>(x, row_stride, T, K, g, pos, top_k, shared, P, xq, sf, zero_out, M);
   };
   switch (tile) {
     case 32: go(split_kernel<32>); break;

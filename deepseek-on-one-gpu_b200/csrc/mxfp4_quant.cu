@@ -165,10 +165,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
 // One thread: the four scales of one row and K block (one word of an atom).
 // Words of an atom that belong to no row are zero.
 __global__ void __launch_bounds__(256) tile_scales_kernel(const uint32_t* __restrict__ scales, int mats, int N, int KB,
-                                                          int tile, int atoms, uint32_t* __restrict__ out,
-                                                          int32_t* __restrict__ zero, int n_zero) {
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < n_zero; i += 256) zero[i] = 0;
+                                                          int tile, int atoms, uint32_t* __restrict__ out) {
   const int tiles = (N + tile - 1) / tile;
   const uint64_t words = static_cast<uint64_t>(mats) * tiles * KB * atoms * 128;
   for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < words; i += gridDim.x * 256ull) {
@@ -230,11 +227,11 @@ cudaError_t launch_dequantize(const uint8_t* codes, const uint8_t* scales, long 
 }
 
 cudaError_t launch_tile_scales(const uint8_t* scales, int mats, int N, int K, int tile, int atoms, uint8_t* out,
-                               int32_t* zero, int n_zero, cudaStream_t s) {
+                               cudaStream_t s) {
   const int KB = K / 128;
   const uint64_t words = static_cast<uint64_t>(mats) * ((N + tile - 1) / tile) * KB * atoms * 128;
   tile_scales_kernel<<<grid_for(words, 256), 256, 0, s>>>(reinterpret_cast<const uint32_t*>(scales), mats, N, KB, tile,
-                                                          atoms, reinterpret_cast<uint32_t*>(out), zero, n_zero);
+                                                          atoms, reinterpret_cast<uint32_t*>(out));
   return cudaGetLastError();
 }
 
