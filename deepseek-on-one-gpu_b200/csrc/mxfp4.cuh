@@ -71,6 +71,50 @@ struct GemmArgs {
   int* status;
 };
 
+// The kernels of one call are chained by programmatic dependent launches: the
+// first one is launched normally, so everything enqueued before the call is
+// done when it starts; a later one may start while its predecessor runs and
+// waits (dependency_wait) before it touches anything an earlier one of the
+// chain reads or writes.
+__device__ __forceinline__ void dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("fence.proxy.async.global;" ::: "memory");  // its data may be read by TMA next
+}
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Loads of what an earlier kernel of the chain wrote. Not __ldg, and not
+// through a const __restrict__ pointer: the compiler takes such data as fixed
+// for the whole kernel and may read it before the wait.
+__device__ __forceinline__ int32_t load_dep(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 load_dep(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
+template <class... P, class... A>
+cudaError_t launch_chained(bool chained, void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                           A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
 // -------------------------------------------------------- mxfp4_quant.cu
 cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long long row_stride, const float* scale_inv,
                             long long rows_per_mat, uint8_t* codes, uint8_t* scales, cudaStream_t s);
@@ -91,9 +135,16 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 // bf16 rows [T][K] -> hi/lo rows and scale atoms. pos == NULL: row t is row t
 // of g (zero_out, optional: rows of y outside every segment are cleared);
 // else token t goes to the rows pos names (and to row t of group 0 with shared).
+// Chained to the kernel that made the tables, if g has any.
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
                          const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
                          __nv_bfloat16* zero_out, int M, cudaStream_t s);
+// launch_route_plan and launch_split in one kernel, for a few tokens: tile 32,
+// at most kRouteTokens tokens and 256 pairs.
+constexpr int kRouteTokens = 32;
+cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
+                               int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
+                               int32_t* tile_start, int32_t* pos, uint8_t* xq, uint8_t* sf, cudaStream_t s);
 // out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
                            int shared, float scale, __nv_bfloat16* out, cudaStream_t s);

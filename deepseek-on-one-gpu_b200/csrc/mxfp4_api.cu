@@ -406,11 +406,18 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   a.hq = at<uint8_t>(workspace, L.hq);
   a.hsf = at<uint8_t>(workspace, L.hsf);
   a.status = device_status;
-  MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, at<int32_t>(workspace, L.counts),
-                                at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), pos, s));
-  MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(hidden), row_stride, tokens, H, a.g, L.tile, pos, top_k,
-                           shared, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
-  if ((r = run_gemm(false, true, w->gate_codes, w->up_codes, G, at<uint8_t>(workspace, L.xq), a, L.tile,
+  const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(hidden);
+  int32_t *counts = at<int32_t>(workspace, L.counts), *row_start = at<int32_t>(workspace, L.row_start),
+          *tile_start = at<int32_t>(workspace, L.tile_start);
+  uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
+  if (tokens <= mx::kRouteTokens && L.tile == 32) {
+    MX_CUDA(mx::launch_route_split(x, row_stride, tokens, H, topk_idx, top_k, E, shared, L.P, counts, row_start,
+                                   tile_start, pos, xq, sf, s));
+  } else {
+    MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, counts, row_start, tile_start, pos, s));
+    MX_CUDA(mx::launch_split(x, row_stride, tokens, H, a.g, L.tile, pos, top_k, shared, L.P, xq, sf, nullptr, 0, s));
+  }
+  if ((r = run_gemm(false, true, w->gate_codes, w->up_codes, G, xq, a, L.tile,
                     L.tiles * (F / 128), s)))
     return r;
   a.M = H;

@@ -182,8 +182,8 @@ __device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tile
       if (tiles[mid] * per <= id) lo = mid; else hi = mid;
     }
     g = lo;
-    rows = __ldg(p.g.counts + g);
-    row_start = __ldg(p.g.row_start + g);
+    rows = load_dep(p.g.counts + g);
+    row_start = load_dep(p.g.row_start + g);
     tile0 = tiles[g];
   }
   ntiles = (rows + C::BN - 1) / C::BN;
@@ -212,7 +212,7 @@ __device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tile
 
 __device__ __forceinline__ int unit_count(const GemmArgs& p, int bn, bool swiglu) {
   const int per = swiglu ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
-  const int tiles = p.g.counts ? __ldg(p.g.tile_start + p.g.n) : (p.g.rows + bn - 1) / bn;
+  const int tiles = p.g.counts ? load_dep(p.g.tile_start + p.g.n) : (p.g.rows + bn - 1) / bn;
   return tiles * per * p.ksplit;
 }
 
@@ -280,6 +280,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   __syncthreads();
   tc_fence_after();
 
+  launch_dependents();
+  // With group tables every role needs what earlier kernels of the chain
+  // wrote. Without, only the copies of the rows do: the producer waits, after
+  // it has started on the weights.
+  if (p.g.counts) dependency_wait();
   const uint32_t tmem = *s_tmem;
   const int total = unit_count(p, BN, SWIGLU);
   const int KB = p.K / 128;
@@ -291,7 +296,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     // nine dependent global loads would be ~3 us before the first copy.
     int* tiles = reinterpret_cast<int*>(smem + C::TAB_OFF);
     if (p.g.counts)
-      for (int t = lane; t <= p.g.n; t += 32) tiles[t] = __ldg(p.g.tile_start + t);
+      for (int t = lane; t <= p.g.n; t += 32) tiles[t] = load_dep(p.g.tile_start + t);
     __syncwarp();
     if (lane == 0) {
       int i = 0;
@@ -321,28 +326,50 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         const uint8_t* fa1 = p.sfa1 + (static_cast<size_t>(e.group) * MT + (two ? e.m1 : 0) / BM) * KB * 512;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
         const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
-        for (int kb = e.kb0; kb < e.kb1; kb += C::KB_STAGE) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, p.status, kDevTimeoutProducer, s_abort)) { ok = false; break; }
+        auto load_w = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES;
           uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);  // an odd last K block: only its scales exist
-          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * (C::A_TX + nkb * 512) + xbytes + nkb * C::ATOMS * 512);
           const int kx = FP4 ? kb * 64 : kb * 128;  // coordinate: bytes of packed codes, or numbers
+          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * (C::A_TX + nkb * 512) + xbytes + nkb * C::ATOMS * 512);
           tma_load_2d(st, &tm_w0, &full[stage], kx, wrow + e.m0, pol_w);
           if (two) tma_load_2d(st + C::A_BYTES, &tm_w1, &full[stage], kx, wrow + e.m1, pol_w);
-          if (!FP4 && e.both) {
-            for (int s = 0; s < e.n; s += 32) {
-              tma_load_2d(st + C::B_OFF + s * 128, &tm_x32, &full[stage], kx, e.row0 + s, pol_x);
-              tma_load_2d(st + C::B_OFF + (e.n + s) * 128, &tm_x32, &full[stage], kx, p.P + e.row0 + s, pol_x);
-            }
-          } else {
-            tma_load_2d(st + C::B_OFF, &tm_x, &full[stage], kx, e.row0, pol_x);
-            if (!FP4) tma_load_2d(st + C::B_OFF + BN * 128, &tm_x, &full[stage], kx, p.P + e.row0, pol_x);
-          }
           bulk_load(sf, fa0 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
           if (two) bulk_load(sf + C::SFA_BYTES, fa1 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
-          bulk_load(sf + 2 * C::SFA_BYTES, fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512,
-                    &full[stage]);
+        };
+        auto load_x = [&](int kb, int stage) {
+          uint8_t* st = smem + stage * C::OP_BYTES + C::B_OFF;
+          const int nkb = min(C::KB_STAGE, e.kb1 - kb);
+          const int kx = FP4 ? kb * 64 : kb * 128;
+          if (!FP4 && e.both) {
+            for (int s = 0; s < e.n; s += 32) {
+              tma_load_2d(st + s * 128, &tm_x32, &full[stage], kx, e.row0 + s, pol_x);
+              tma_load_2d(st + (e.n + s) * 128, &tm_x32, &full[stage], kx, p.P + e.row0 + s, pol_x);
+            }
+          } else {
+            tma_load_2d(st, &tm_x, &full[stage], kx, e.row0, pol_x);
+            if (!FP4) tma_load_2d(st + BN * 128, &tm_x, &full[stage], kx, p.P + e.row0, pol_x);
+          }
+          bulk_load(smem + C::SF0 + stage * C::SF_BYTES + 2 * C::SFA_BYTES,
+                    fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512, &full[stage]);
+        };
+        int kb = e.kb0;
+        if (i == 0 && !p.g.counts) {
+          // The first stages' weights are on their way while the kernel before
+          // this one still prepares the rows.
+          const int n = min(STAGES, (e.kb1 - kb + C::KB_STAGE - 1) / C::KB_STAGE);
+          for (int s = 0; s < n; ++s) load_w(kb + s * C::KB_STAGE, s);
+          dependency_wait();
+          for (int s = 0; s < n; ++s) load_x(kb + s * C::KB_STAGE, s);
+          issued = n;
+          kb += n * C::KB_STAGE;
+          stage = n % STAGES;
+          phase = n == STAGES;
+        }
+        for (; kb < e.kb1; kb += C::KB_STAGE) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, p.status, kDevTimeoutProducer, s_abort)) { ok = false; break; }
+          load_w(kb, stage);
+          load_x(kb, stage);
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -607,10 +634,12 @@ cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = at;
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cfg;
 }
 

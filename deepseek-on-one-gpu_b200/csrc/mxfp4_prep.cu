@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(kMaxGroups) segments_kernel(const int32_t* __r
                                                               int32_t* __restrict__ tile_start,
                                                               int* __restrict__ status) {
   __shared__ int buf[kMaxGroups];
+  launch_dependents();
   const int i = threadIdx.x;
   const int lo = i < n ? offsets[i] : 0, hi = i < n ? offsets[i + 1] : 0;
   if (i < n && (lo < 0 || hi < lo || hi > rows)) atomicCAS(status, 0, kDevBadCount);
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(1024) route_plan_kernel(const int64_t* __restr
                                                           int32_t* __restrict__ tile_start, int32_t* __restrict__ pos) {
   extern __shared__ int hist[];  // [kPlanWarps][n_routed]
   __shared__ int buf[kMaxGroups];
+  launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pairs = T * top_k;
   const int per = ((pairs + kPlanWarps - 1) / kPlanWarps + 31) & ~31;
@@ -75,9 +77,22 @@ __global__ void __launch_bounds__(1024) route_plan_kernel(const int64_t* __restr
   for (int i = threadIdx.x; i < kPlanWarps * n_routed; i += 1024) hist[i] = 0;
   __syncthreads();
   int* mine = hist + warp * n_routed;
-  for (int p = p0 + lane; p < p1; p += 32) {
-    const int64_t e = idx[p];
-    if (e >= 0 && e < n_routed) atomicAdd(&mine[e], 1);
+  // expert of pair p, -1 past the warp's pairs or for an id outside; batches of
+  // 8 x 32 pairs are loaded together (one dependent load per 32 pairs was 2/3
+  // of this kernel's time)
+  constexpr int B = 8;
+  auto expert = [&](int p) {
+    if (p >= p1) return -1;
+    const int64_t e = __ldg(idx + p);
+    return e >= 0 && e < n_routed ? static_cast<int>(e) : -1;
+  };
+  for (int p = p0; p < p1; p += 32 * B) {
+    int e[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) e[j] = expert(p + 32 * j + lane);
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (e[j] >= 0) atomicAdd(&mine[e[j]], 1);
   }
   __syncthreads();
   // group totals and, per warp, the rows of earlier warps
@@ -122,20 +137,21 @@ __global__ void __launch_bounds__(1024) route_plan_kernel(const int64_t* __restr
       for (int w = 0; w < kPlanWarps; ++w) hist[w * n_routed + g - shared] += start;
   }
   __syncthreads();
-  for (int b = p0; b < p1; b += 32) {  // warp-uniform
-    const int p = b + lane;
-    int e = -1;
-    if (p < p1) {
-      const int64_t v = idx[p];
-      if (v >= 0 && v < n_routed) e = static_cast<int>(v);
+  for (int p = p0; p < p1; p += 32 * B) {  // warp-uniform
+    int e[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j) e[j] = expert(p + 32 * j + lane);
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      const int q = p + 32 * j + lane;
+      const unsigned same = __match_any_sync(0xffffffffu, e[j]);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int base = e[j] >= 0 ? mine[e[j]] : 0;
+      __syncwarp();
+      if (e[j] >= 0 && rank == 0) mine[e[j]] = base + __popc(same);
+      __syncwarp();
+      if (q < p1) pos[q] = e[j] >= 0 ? base + rank : -1;
     }
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    const int base = e >= 0 ? mine[e] : 0;
-    __syncwarp();
-    if (e >= 0 && rank == 0) mine[e] = base + __popc(same);
-    __syncwarp();
-    if (p < p1) pos[p] = e >= 0 ? base + rank : -1;
   }
 }
 
@@ -153,54 +169,20 @@ __device__ __forceinline__ SfSpot sf_spot(int tile0, int count, int local, int K
   return {base + word(c), n32 ? base + word(c + n32) : -1};
 }
 
-// One block: 2048 columns of one row. 4 threads share a 32-number block, 16 a
-// K block's scale word.
-template <int TILE>
-__global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
-                                                    int K, const Groups g, const int32_t* __restrict__ pos, int top_k,
-                                                    int shared, int P, uint8_t* __restrict__ xq,
-                                                    uint8_t* __restrict__ sf, __nv_bfloat16* __restrict__ zero_out,
-                                                    int M) {
-  constexpr int MAXR = 9;
-  const int t = blockIdx.x;
+// This thread's 8 columns of a row (zero past its end): block y of the grid
+// has columns 2048 y and up.
+__device__ __forceinline__ uint4 load_cols(const __nv_bfloat16* row, int K) {
+  const int col = blockIdx.y * 2048 + threadIdx.x * 8;
+  return col < K ? __ldg(reinterpret_cast<const uint4*>(row + col)) : make_uint4(0, 0, 0, 0);
+}
+
+// Splits the row and stores it, with its scale words, at n rows. 4 threads
+// share a 32-number block, 16 a K block's scale word.
+__device__ __forceinline__ void split_row(const uint4& q, int K, int P, int n, const int* s_row, const SfSpot* s_spot,
+                                          int atoms, uint8_t* __restrict__ xq, uint8_t* __restrict__ sf) {
   const int tid = threadIdx.x;
-  const int KB = K / 128;
-  __shared__ int s_row[MAXR];
-  __shared__ SfSpot s_spot[MAXR];
-  const int n = pos ? top_k + shared : 1;
-  if (tid < n) {
-    int row, grp = 0, count, local, tile0 = 0;
-    if (pos) row = tid < shared ? t : pos[static_cast<size_t>(t) * top_k + tid - shared];
-    else row = t;
-    if (row >= 0 && g.counts) {
-      int lo = 0, hi = g.n;  // last group that starts at or before the row
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (g.row_start[mid] <= row) lo = mid; else hi = mid;
-      }
-      grp = lo;
-      count = g.counts[grp];
-      local = row - g.row_start[grp];
-      tile0 = g.tile_start[grp];
-      if (local < 0 || local >= count) row = -1;
-    } else {
-      count = g.rows;
-      local = row;
-    }
-    s_row[tid] = row;
-    if (row >= 0) s_spot[tid] = sf_spot<TILE>(tile0, count, local, KB);
-  }
-  __syncthreads();
-  if (!pos && s_row[0] < 0) {  // a row outside every segment
-    if (zero_out && blockIdx.y == 0)
-      for (int c = tid; c < M / 8; c += 256)
-        reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t) * M)[c] = make_uint4(0, 0, 0, 0);
-    return;
-  }
   const int col = blockIdx.y * 2048 + tid * 8;
   const bool in = col < K;  // K is a multiple of 128: 16 threads of a K block are in or out together
-  uint4 q = make_uint4(0, 0, 0, 0);
-  if (in) q = __ldg(reinterpret_cast<const uint4*>(x + t * row_stride + col));
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   uint32_t amax = 0;  // |bf16| bit patterns order like the numbers
 #pragma unroll
@@ -224,7 +206,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
   word |= __shfl_xor_sync(0xffffffffu, word, 8);
   if (!in) return;
-  const long long step = static_cast<long long>(col >> 7) * tile_atoms(TILE) * 128;
+  const long long step = static_cast<long long>(col >> 7) * atoms * 128;
   for (int r = 0; r < n; ++r) {
     const int row = s_row[r];
     if (row < 0) continue;
@@ -239,25 +221,148 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
   }
 }
 
-__global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* __restrict__ y, int T, int H,
-                                                      const int32_t* __restrict__ pos, const float* __restrict__ w,
+constexpr int MAXR = 9;  // rows of a token: the shared expert's and top_k <= 8
+
+// One block: 2048 columns of one row.
+template <int TILE>
+__global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
+                                                    int K, const Groups g, const int32_t* pos, int top_k,
+                                                    int shared, int P, uint8_t* __restrict__ xq,
+                                                    uint8_t* __restrict__ sf, __nv_bfloat16* __restrict__ zero_out,
+                                                    int M) {
+  const int t = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int KB = K / 128;
+  launch_dependents();
+  dependency_wait();
+  __shared__ int s_row[MAXR];
+  __shared__ SfSpot s_spot[MAXR];
+  const int n = pos ? top_k + shared : 1;
+  if (tid < n) {
+    int row, grp = 0, count, local, tile0 = 0;
+    if (pos) row = tid < shared ? t : load_dep(pos + static_cast<size_t>(t) * top_k + tid - shared);
+    else row = t;
+    if (row >= 0 && g.counts) {
+      int lo = 0, hi = g.n;  // last group that starts at or before the row
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (load_dep(g.row_start + mid) <= row) lo = mid; else hi = mid;
+      }
+      grp = lo;
+      count = load_dep(g.counts + grp);
+      local = row - load_dep(g.row_start + grp);
+      tile0 = load_dep(g.tile_start + grp);
+      if (local < 0 || local >= count) row = -1;
+    } else {
+      count = g.rows;
+      local = row;
+    }
+    s_row[tid] = row;
+    if (row >= 0) s_spot[tid] = sf_spot<TILE>(tile0, count, local, KB);
+  }
+  __syncthreads();
+  if (!pos && s_row[0] < 0) {  // a row outside every segment
+    if (zero_out && blockIdx.y == 0)
+      for (int c = tid; c < M / 8; c += 256)
+        reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t) * M)[c] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  split_row(load_cols(x + t * row_stride, K), K, P, n, s_row, s_spot, tile_atoms(TILE), xq, sf);
+}
+
+// Plan and split for a few tokens. Every block builds the group tables for
+// itself (a 512-entry histogram and scan in shared memory, ~1 us) instead of
+// waiting for a kernel that does; block 0 also writes them out. A group has at
+// most 32 rows, one token tile.
+__global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride,
+                                                          int T, int K, const int64_t* __restrict__ idx, int top_k,
+                                                          int n_routed, int shared, int P,
+                                                          int32_t* __restrict__ counts, int32_t* __restrict__ row_start,
+                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ pos,
+                                                          uint8_t* __restrict__ xq, uint8_t* __restrict__ sf) {
+  constexpr int TILE = 32;
+  static_assert(kRouteTokens <= TILE, "one tile per group");
+  __shared__ int s_e[256], s_cnt[kMaxGroups], s_start[kMaxGroups], s_tile[kMaxGroups];
+  __shared__ int s_sum[2][8];
+  __shared__ int s_row[MAXR];
+  __shared__ SfSpot s_spot[MAXR];
+  launch_dependents();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pairs = T * top_k, G = n_routed + shared;
+  const uint4 q = load_cols(x + t * row_stride, K);
+  int e = -1;
+  if (tid < pairs) {
+    const int64_t v = __ldg(idx + tid);
+    if (v >= 0 && v < n_routed) e = static_cast<int>(v) + shared;
+  }
+  s_e[tid] = e;
+  s_cnt[tid] = s_cnt[tid + 256] = 0;
+  __syncthreads();
+  if (e >= 0) atomicAdd(&s_cnt[e], 1);
+  if (shared && tid == 0) s_cnt[0] = T;
+  __syncthreads();
+  // Exclusive scans of rows and tiles; thread tid has groups 2 tid, 2 tid + 1.
+  const int c0 = s_cnt[2 * tid], c1 = s_cnt[2 * tid + 1];
+  int rows = c0 + c1, tiles = (c0 > 0) + (c1 > 0);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, rows, o), b = __shfl_up_sync(0xffffffffu, tiles, o);
+    if (lane >= o) rows += a, tiles += b;
+  }
+  if (lane == 31) s_sum[0][warp] = rows, s_sum[1][warp] = tiles;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) rows += s_sum[0][w], tiles += s_sum[1][w];
+  s_start[2 * tid + 1] = rows - c1;
+  s_start[2 * tid] = rows - c1 - c0;
+  s_tile[2 * tid + 1] = tiles - (c1 > 0);
+  s_tile[2 * tid] = tiles - (c1 > 0) - (c0 > 0);
+  __syncthreads();
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int g = tid; g <= G; g += 256) {
+      if (g < G) counts[g] = s_cnt[g], row_start[g] = s_start[g], tile_start[g] = s_tile[g];
+      else tile_start[g] = s_tile[G - 1] + (s_cnt[G - 1] > 0);
+    }
+  // Warp w places pair w of the token: earlier pairs of the same expert first.
+  const int n = top_k + shared;
+  if (warp < top_k) {
+    const int p = t * top_k + warp, mine = s_e[p];
+    int rank = 0;
+    for (int b = 0; b < p; b += 32) rank += __popc(__ballot_sync(0xffffffffu, b + lane < p && s_e[b + lane] == mine));
+    if (lane == 0) {
+      const int row = mine >= 0 ? s_start[mine] + rank : -1;
+      s_row[shared + warp] = row;
+      if (mine >= 0) s_spot[shared + warp] = sf_spot<TILE>(s_tile[mine], s_cnt[mine], rank, K / 128);
+      if (blockIdx.y == 0) pos[p] = row;
+    }
+  }
+  if (shared && tid == 0) {
+    s_row[0] = t;
+    s_spot[0] = sf_spot<TILE>(0, T, t, K / 128);
+  }
+  __syncthreads();
+  split_row(q, K, P, n, s_row, s_spot, tile_atoms(TILE), xq, sf);
+}
+
+__global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, int T, int H,
+                                                      const int32_t* pos, const float* __restrict__ w,
                                                       int top_k, int shared, float scale,
                                                       __nv_bfloat16* __restrict__ out) {
   constexpr int MAXK = 8;
   const int t = blockIdx.x;
   __shared__ int s_row[MAXK];
   __shared__ float s_w[MAXK];
+  dependency_wait();
   if (threadIdx.x < top_k) {
-    s_row[threadIdx.x] = pos[static_cast<size_t>(t) * top_k + threadIdx.x];
+    s_row[threadIdx.x] = load_dep(pos + static_cast<size_t>(t) * top_k + threadIdx.x);
     s_w[threadIdx.x] = scale * w[static_cast<size_t>(t) * top_k + threadIdx.x];
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < H / 8; c += 256) {
+  for (int c = blockIdx.y * 256 + threadIdx.x; c < H / 8; c += gridDim.y * 256) {
     uint4 v[MAXK + 1];
 #pragma unroll
     for (int k = 0; k < MAXK; ++k)
-      if (k < top_k && s_row[k] >= 0) v[k] = __ldg(reinterpret_cast<const uint4*>(y + static_cast<size_t>(s_row[k]) * H) + c);
-    if (shared) v[MAXK] = __ldg(reinterpret_cast<const uint4*>(y + static_cast<size_t>(t) * H) + c);
+      if (k < top_k && s_row[k] >= 0) v[k] = load_dep(reinterpret_cast<const uint4*>(y + static_cast<size_t>(s_row[k]) * H) + c);
+    if (shared) v[MAXK] = load_dep(reinterpret_cast<const uint4*>(y + static_cast<size_t>(t) * H) + c);
     float acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -306,21 +411,31 @@ cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, in
                          __nv_bfloat16* zero_out, int M, cudaStream_t s) {
   const dim3 grid(T, (K + 2047) / 2048);
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, s>>>(x, row_stride, T, K, g, pos, top_k, shared, P, xq, sf, zero_out, M);
+    return launch_chained(g.counts != nullptr, kern, grid, 256, 0, s, x, row_stride, T, K, g, pos, top_k, shared, P, xq,
+                          sf, zero_out, M);
   };
   switch (tile) {
-    case 32: go(split_kernel<32>); break;
-    case 64: go(split_kernel<64>); break;
-    case 160: go(split_kernel<160>); break;
+    case 32: return go(split_kernel<32>);
+    case 64: return go(split_kernel<64>);
+    case 160: return go(split_kernel<160>);
     default: return cudaErrorInvalidValue;
   }
+}
+
+cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
+                               int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
+                               int32_t* tile_start, int32_t* pos, uint8_t* xq, uint8_t* sf, cudaStream_t s) {
+  if (T > kRouteTokens || T * top_k > 256 || n_routed + shared > kMaxGroups) return cudaErrorInvalidValue;
+  route_split_kernel<<<dim3(T, (K + 2047) / 2048), 256, 0, s>>>(x, row_stride, T, K, idx, top_k, n_routed, shared, P,
+                                                                 counts, row_start, tile_start, pos, xq, sf);
   return cudaGetLastError();
 }
 
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
                            int shared, float scale, __nv_bfloat16* out, cudaStream_t s) {
-  combine_kernel<<<T, 256, 0, s>>>(y, T, H, pos, w, top_k, shared, scale, out);
-  return cudaGetLastError();
+  // Few tokens: a block per 2048 columns; many: one per token.
+  const dim3 grid(T, T < 512 ? (H + 2047) / 2048 : 1);
+  return launch_chained(true, combine_kernel, grid, 256, 0, s, y, T, H, pos, w, top_k, shared, scale, out);
 }
 
 }  // namespace mx

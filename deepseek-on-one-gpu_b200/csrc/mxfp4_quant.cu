@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
 // Words of an atom that belong to no row are zero.
 __global__ void __launch_bounds__(256) tile_scales_kernel(const uint32_t* __restrict__ scales, int mats, int N, int KB,
                                                           int tile, int atoms, uint32_t* __restrict__ out) {
+  launch_dependents();
   const int tiles = (N + tile - 1) / tile;
   const uint64_t words = static_cast<uint64_t>(mats) * tiles * KB * atoms * 128;
   for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < words; i += gridDim.x * 256ull) {

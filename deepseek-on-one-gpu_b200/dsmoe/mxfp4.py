@@ -22,6 +22,7 @@ is no CPU path and no backward: tensors that require a gradient are rejected.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 
@@ -67,8 +68,16 @@ def _index(device: torch.device) -> torch.device:
     return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch; free when it already is."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _require(what: str, *tensors: torch.Tensor) -> None:
-    dev = None
+    dev, grad = None, torch.is_grad_enabled()
     for t in tensors:
         if t is None:
             continue
@@ -79,7 +88,7 @@ def _require(what: str, *tensors: torch.Tensor) -> None:
         if dev is not None and t.device != dev:
             raise RuntimeError(f"{what}: tensors on different devices ({dev}, {t.device})")
         dev = t.device
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise RuntimeError(f"{what} has no backward: detach the inputs or call it under torch.no_grad()")
 
 
@@ -109,7 +118,7 @@ def _quantize_into(x: torch.Tensor, scale_inv: torch.Tensor | None, codes: torch
     fp8 = x.dtype == torch.float8_e4m3fn
     x2 = _rows(x, 8 if fp8 else 16)
     per = x.shape[-2] if fp8 else 1
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         check(lib().dsmoe_mxfp4_quantize(ptr(x2), _DTYPES[x.dtype], x2.shape[0], K, x2.stride(0), ptr(scale_inv),
                                          max(per, 1), ptr(codes), ptr(scales), stream_handle(x.device)),
               "dsmoe_mxfp4_quantize")
@@ -169,7 +178,7 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
     codes, scales = _dense(codes, 4), scales.contiguous()
     out = torch.empty(*codes.shape[:-1], K, dtype=out_dtype, device=codes.device)
     if out.numel():
-        with torch.cuda.device(codes.device):
+        with _on(codes.device):
             check(lib().dsmoe_mxfp4_dequantize(ptr(codes), ptr(scales), scales.numel(), _DTYPES[out_dtype], ptr(out),
                                                stream_handle(codes.device)), "dsmoe_mxfp4_dequantize")
     return out
@@ -200,7 +209,7 @@ class MXFP4Weight:
 
     def _pack(self, scales: torch.Tensor, first: int, mats: int) -> None:
         per = self.atoms.numel() // (1 if self.experts is None else self.experts)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             check(lib().dsmoe_mxfp4_scale_atoms(ptr(scales), mats, self.out_features, self.in_features,
                                                 ptr(self.atoms) + first * per, stream_handle(self.device)),
                   "dsmoe_mxfp4_scale_atoms")
@@ -257,7 +266,7 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
     T, K, N = x2.shape[0], weight.in_features, weight.out_features
     out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
     if T:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             ws = _scratch(lib().dsmoe_mxfp4_linear_workspace_size(T, K, N), x.device)
             check(lib().dsmoe_mxfp4_linear(ptr(x2), x2.stride(0), T, K, N, ptr(weight.codes), ptr(weight.atoms),
                                            ptr(out), ptr(ws), ws.numel(), ptr(weight.status),
@@ -278,7 +287,7 @@ def mxfp4_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: MXFP4Weight)
     T = c2.shape[0]
     out = torch.empty(*shape, N, dtype=torch.bfloat16, device=codes.device)
     if T:
-        with torch.cuda.device(codes.device):
+        with _on(codes.device):
             ws = _scratch(lib().dsmoe_mxfp4_matmul_workspace_size(T, K, N), codes.device)
             check(lib().dsmoe_mxfp4_matmul(ptr(c2), ptr(s2), T, K, N, ptr(weight.codes), ptr(weight.atoms), ptr(out),
                                            ptr(ws), ws.numel(), ptr(weight.status), stream_handle(codes.device)),
@@ -307,7 +316,7 @@ def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Te
         raise ValueError(f"out must be a dense, 16-byte aligned bf16 tensor ({R}, {N})")
     if R:
         x2, off = _rows(x, 16), offsets.contiguous()
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             need = lib().dsmoe_mxfp4_grouped_linear_workspace_size(R, K, N, weight.experts)
             ws = _scratch(need, x.device)
             check(lib().dsmoe_mxfp4_grouped_linear(ptr(x2), x2.stride(0), R, K, N, weight.experts, ptr(off),
@@ -369,7 +378,7 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     out = torch.empty(*lead, H, dtype=torch.bfloat16, device=hidden.device)
     if T:
         idx, w = topk_idx.contiguous(), topk_w.contiguous()
-        with torch.cuda.device(hidden.device):
+        with _on(hidden.device):
             ws = _scratch(lib().dsmoe_mxfp4_moe_workspace_size(T, H, experts.inter, experts.n_routed,
                                                                int(experts.shared), K), hidden.device)
             check(lib().dsmoe_mxfp4_moe(ptr(x2), x2.stride(0), T, ctypes.byref(experts.desc), ptr(idx), ptr(w), K,
