@@ -187,12 +187,10 @@ int dsmoe_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t col
   if (rows == 0) return DSMOE_OK;
   if (rows > (0xffffffe0ll * 8) / cols) return fail(DSMOE_ERR_UNSUPPORTED, "mxfp4_quantize: more than 2^35 numbers");
   const int size = dtype == DSMOE_F32 ? 4 : dtype == DSMOE_E4M3 ? 1 : 2;
-  // A thread loads 8 numbers: 16 bytes (twice for fp32), or 8 for e4m3.
-  const int load = size == 1 ? 8 : 16;
-  if (!aligned(x, load) || !aligned(codes, 4) || !scales)
-    return fail(DSMOE_ERR_INVALID, "mxfp4_quantize: pointer NULL or x not %d-byte aligned", load);
-  if (rows > 1 && (row_stride < cols || row_stride * size % load))
-    return fail(DSMOE_ERR_INVALID, "mxfp4_quantize: rows must not overlap and must start on %d bytes", load);
+  if (!aligned(x, 16) || !aligned(codes, 8) || !scales)
+    return fail(DSMOE_ERR_INVALID, "mxfp4_quantize: pointer NULL, x not 16-byte or codes not 8-byte aligned");
+  if (rows > 1 && (row_stride < cols || row_stride * size % 16))
+    return fail(DSMOE_ERR_INVALID, "mxfp4_quantize: rows must not overlap and must start on 16 bytes");
   if (dtype == DSMOE_E4M3) {
     if (!aligned(scale_inv, 4)) return fail(DSMOE_ERR_INVALID, "mxfp4_quantize: e4m3 needs its block scales");
     if (rows_per_matrix < 1 || rows % rows_per_matrix)

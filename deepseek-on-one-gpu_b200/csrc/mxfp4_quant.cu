@@ -12,54 +12,100 @@
 // exponent and every later rounding to 2 bits equal to that of the exact
 // product.
 //
-// Bound by memory: 4 threads share a block, each holding 8 numbers from one
-// or two 16-byte loads; codes leave as 4 bytes per thread (128 contiguous
-// bytes per warp).
+// Bound by memory. A thread holds N numbers: 8 of fp32 (two 16-byte loads), 16
+// of the narrower types, so that index arithmetic, shuffles and scale bytes
+// are shared by as many numbers as the registers allow; codes leave in 4- or
+// 8-byte words, contiguous over the warp. Row and matrix indexes come from
+// multiplications (FastDiv): two integer divisions per thread cost more than
+// the quantisation.
 #include "common.cuh"
 #include "mxfp4.cuh"
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace dsmoe {
 namespace mx {
 namespace {
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* v) {
-  const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+// n / d for 32-bit n by one multiplication with 2^64 / d rounded up.
+struct FastDiv {
+  uint32_t d, lo, hi;
+  explicit FastDiv(uint32_t div) : d(div) {
+    const uint64_t m = div > 1 ? ~0ull / div + 1 : 0;
+    lo = static_cast<uint32_t>(m);
+    hi = static_cast<uint32_t>(m >> 32);
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    if (d == 1) return n;
+    return static_cast<uint32_t>((static_cast<uint64_t>(n) * hi + __umulhi(n, lo)) >> 32);
+  }
+};
+
+template <class T> struct Form { static constexpr int N = 16; };  // numbers per thread
+template <> struct Form<float> { static constexpr int N = 8; };
+
+__device__ __forceinline__ void load(const __nv_bfloat16* p, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+  for (int j = 0; j < 2; ++j) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + j);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[8 * j + 2 * i] = __uint_as_float(w[i] << 16);
+      v[8 * j + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
-__device__ __forceinline__ void load8(const __half* p, float* v) {
-  const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-  const __half2* h = reinterpret_cast<const __half2*>(&q);
+__device__ __forceinline__ void load(const __half* p, float* v) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+  for (int j = 0; j < 2; ++j) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + j);
+    const __half2* h = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[8 * j + 2 * i] = f.x;
+      v[8 * j + 2 * i + 1] = f.y;
+    }
   }
 }
-__device__ __forceinline__ void load8(const float* p, float* v) {
+__device__ __forceinline__ void load(const float* p, float* v) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
   v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
-__device__ __forceinline__ void load8(const __nv_fp8_e4m3* p, float* v) {
-  const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+// 16 e4m3 numbers as f16 pairs (exact).
+__device__ __forceinline__ void load(const __nv_fp8_e4m3* p, __half2* v) {
+  const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = e4m3_to_f32(((i < 4 ? q.x : q.y) >> (8 * (i & 3))) & 0xff);
+  for (int i = 0; i < 8; ++i) {
+    uint32_t h;
+    const uint16_t two = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(two));
+    v[i] = *reinterpret_cast<__half2*>(&h);
+  }
 }
 
-// w * s rounded to odd.
-__device__ __forceinline__ float mul_odd(float w, float s) {
-  const float p = __fmul_rz(w, s);
-  const float r = __fmaf_rn(w, s, -p);
-  return r != 0.f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+// Of the two fp32 neighbours of an inexact product the one whose last bit is
+// set (rounding to odd).
+__device__ __forceinline__ float odd(float a, float b) { return __float_as_uint(a) & 1 ? a : b; }
+__device__ __forceinline__ float mul_odd(float w, float s) { return odd(__fmul_rd(w, s), __fmul_ru(w, s)); }
+// Both products of a pair by s, two packed multiplications.
+__device__ __forceinline__ float2 mul_odd(float2 w, float s) {
+  float2 a, b;
+  asm("{\n\t.reg .b64 pw, ps, pa, pb;\n\t"
+      "mov.b64 pw, {%4, %5};\n\t"
+      "mov.b64 ps, {%6, %6};\n\t"
+      "mul.rm.f32x2 pa, pw, ps;\n\t"
+      "mul.rp.f32x2 pb, pw, ps;\n\t"
+      "mov.b64 {%0, %1}, pa;\n\t"
+      "mov.b64 {%2, %3}, pb;\n\t}"
+      : "=f"(a.x), "=f"(a.y), "=f"(b.x), "=f"(b.y)
+      : "f"(w.x), "f"(w.y), "f"(s));
+  return make_float2(odd(a.x, b.x), odd(a.y, b.y));
 }
 
 __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
@@ -68,48 +114,97 @@ __device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
   return r;
 }
 
-// One thread: 8 numbers. `units` = rows * K / 8, fewer than 2^32.
-template <class T>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t units, uint32_t per_row,
-                                                       long long row_stride, const float* __restrict__ scale_inv,
-                                                       uint32_t rows_per_mat, uint32_t sc_rows, uint32_t sc_cols,
-                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  // per_row is a multiple of 4, so the 4 threads of a block are in or out
-  // together; the loop bound is warp-aligned for the shuffles.
-  const uint32_t bound = (units + 31) & ~31u;
+// Scale byte of a block whose largest magnitude has the bit pattern `amax`.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  const uint32_t ef = amax >> 23;
+  return ef == 255 ? 255u : (ef > 2 ? ef - 2 : 0u);
+}
+
+// `units` = rows * K / N, fewer than 2^32 - 32. ROWS: rows are not back to back.
+template <class T, bool ROWS>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, uint32_t units, FastDiv per_row,
+                                                       long long row_stride, uint8_t* __restrict__ codes,
+                                                       uint8_t* __restrict__ scales) {
+  constexpr int N = Form<T>::N;
+  // A block's 32 / N threads are in or out together; the loop bound is
+  // warp-aligned for the shuffles.
+  const uint64_t bound = (static_cast<uint64_t>(units) + 31) & ~31ull;
   for (uint64_t u64 = blockIdx.x * 256u + threadIdx.x; u64 < bound; u64 += gridDim.x * 256u) {
     const uint32_t u = static_cast<uint32_t>(u64);
-    const bool in = u < units;
-    float v[8];
+    const bool in = u64 < units;
+    float v[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
     if (in) {
-      const uint32_t row = u / per_row, c = u - row * per_row;
-      load8(x + row * row_stride + c * 8, v);
-      if constexpr (sizeof(T) == 1) {
-        const uint32_t mat = row / rows_per_mat, r = row - mat * rows_per_mat;
-        const float s = __ldg(scale_inv + (static_cast<size_t>(mat) * sc_rows + r / 128) * sc_cols + c / 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = mul_odd(v[i], s);
+      if constexpr (ROWS) {
+        const uint32_t row = per_row(u), c = u - row * per_row.d;
+        load(x + row * row_stride + c * N, v);
+      } else {
+        load(x + static_cast<size_t>(u) * N, v);
       }
     }
     uint32_t amax = 0;  // bit patterns of |v| order like the numbers, NaN above infinity
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t ef = amax >> 23;
-    const bool bad = ef == 255;
-    const uint32_t byte = bad ? 255u : (ef > 2 ? ef - 2 : 0u);
-    const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
-    uint32_t w = 0;
-    if (!bad) {
+    for (int i = 0; i < N; ++i) amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w |= e2m1x2(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
+    for (int o = 1; o < 32 / N; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const uint32_t byte = scale_byte(amax);
+    const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
+    uint32_t w[N / 8];
+#pragma unroll
+    for (int j = 0; j < N / 8; ++j) {
+      w[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[j] |= e2m1x2(v[8 * j + 2 * i] * inv, v[8 * j + 2 * i + 1] * inv) << (8 * i);
+      if (byte == 255) w[j] = 0;
     }
     if (in) {
-      reinterpret_cast<uint32_t*>(codes)[u] = w;
-      if ((u & 3) == 0) scales[u >> 2] = static_cast<uint8_t>(byte);
+      if constexpr (N == 16) reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
+      else reinterpret_cast<uint32_t*>(codes)[u] = w[0];
+      if (u % (32 / N) == 0) scales[u / (32 / N)] = static_cast<uint8_t>(byte);
+    }
+  }
+}
+
+// The checkpoint's e4m3 with block scales. A block of 32 has one scale_inv s
+// (128 is a multiple of 32), so its largest product is that of its largest
+// number, and s 2^-e is exact: one rounded product per number.
+__global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* __restrict__ x, uint32_t units,
+                                                           FastDiv per_row, long long row_stride,
+                                                           const float* __restrict__ scale_inv, FastDiv rows_per_mat,
+                                                           uint32_t sc_rows, uint32_t sc_cols,
+                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const uint64_t bound = (static_cast<uint64_t>(units) + 31) & ~31ull;
+  for (uint64_t u64 = blockIdx.x * 256u + threadIdx.x; u64 < bound; u64 += gridDim.x * 256u) {
+    const uint32_t u = static_cast<uint32_t>(u64);
+    const bool in = u64 < units;
+    __half2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __half2half2(__ushort_as_half(0));
+    float s = 1.f;
+    if (in) {
+      const uint32_t row = per_row(u), c = u - row * per_row.d;
+      load(x + row * row_stride + c * 16, v);
+      const uint32_t mat = rows_per_mat(row), r = row - mat * rows_per_mat.d;
+      s = __ldg(scale_inv + (static_cast<size_t>(mat) * sc_rows + r / 128) * sc_cols + c / 8);
+    }
+    __half2 m = __habs2(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(v[i]));
+    m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    const float wmax = __half2float(__hmax_nan(__low2half(m), __high2half(m)));
+    const uint32_t byte = scale_byte(__float_as_uint(mul_odd(wmax, s)) & 0x7fffffffu);
+    const float sc = s * __uint_as_float((254u - byte) << 23);
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 p = mul_odd(__half22float2(v[i]), sc);
+      w[i >> 2] |= e2m1x2(p.x, p.y) << (8 * (i & 3));
+    }
+    if (byte == 255) w[0] = w[1] = 0;
+    if (in) {
+      reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
+      if ((u & 1) == 0) scales[u >> 1] = static_cast<uint8_t>(byte);
     }
   }
 }
@@ -143,22 +238,35 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
-// One thread: 8 codes. code * 2^(b - 127) is exact in fp32 and bf16.
+// A thread takes 8 codes at a time, 4 such groups a block's width apart with
+// their loads together. code * 2^(b - 127) is exact in fp32 and bf16.
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, uint64_t units,
                                                          T* __restrict__ out) {
-  for (uint64_t u = blockIdx.x * 256ull + threadIdx.x; u < units; u += gridDim.x * 256ull) {
-    const uint32_t w = __ldg(codes + u);
-    const float s = e8m0(__ldg(scales + (u >> 2)));
-    float v[8];
+  constexpr int G = 4;
+  for (uint64_t u0 = blockIdx.x * (256ull * G) + threadIdx.x; u0 < units; u0 += gridDim.x * (256ull * G)) {
+    uint32_t w[G], b[G];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = e2m1_pair((w >> (8 * i)) & 0xff);
-      v[2 * i] = f.x * s;
-      v[2 * i + 1] = f.y * s;
+    for (int g = 0; g < G; ++g) {
+      const uint64_t u = u0 + 256 * g;
+      w[g] = u < units ? __ldg(codes + u) : 0;
+      b[g] = u < units ? __ldg(scales + (u >> 2)) : 0;
     }
-    store8(out + u * 8, v);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint64_t u = u0 + 256 * g;
+      if (u >= units) break;
+      const float s = e8m0(b[g]);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = e2m1_pair((w[g] >> (8 * i)) & 0xff);
+        v[2 * i] = f.x * s;
+        v[2 * i + 1] = f.y * s;
+      }
+      store8(out + u * 8, v);
+    }
   }
 }
 
@@ -194,20 +302,30 @@ int grid_for(uint64_t units, int per_block) {
 cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long long row_stride,
                             const float* scale_inv, long long rows_per_mat, uint8_t* codes, uint8_t* scales,
                             cudaStream_t s) {
-  const uint32_t per_row = K / 8;
-  const uint64_t units = static_cast<uint64_t>(rows) * per_row;
-  const int grid = grid_for(units, 256);
-  const uint32_t scr = static_cast<uint32_t>((rows_per_mat + 127) / 128), scc = (K + 127) / 128;
-  const uint32_t rpm = static_cast<uint32_t>(rows_per_mat);
-  auto go = [&](auto* p) {
-    quantize_kernel<<<grid, 256, 0, s>>>(p, static_cast<uint32_t>(units), per_row, row_stride, scale_inv, rpm, scr, scc,
-                                         codes, scales);
+  if (type == kTypeE4m3) {
+    const FastDiv per_row(K / 16), rpm(static_cast<uint32_t>(rows_per_mat));
+    const uint64_t units = static_cast<uint64_t>(rows) * per_row.d;
+    quantize_fp8_kernel<<<grid_for(units, 256), 256, 0, s>>>(
+        static_cast<const __nv_fp8_e4m3*>(x), static_cast<uint32_t>(units), per_row, row_stride, scale_inv, rpm,
+        static_cast<uint32_t>((rows_per_mat + 127) / 128), (K + 127) / 128, codes, scales);
+    return cudaGetLastError();
+  }
+  auto go = [&](auto* p, auto with_rows) {
+    using T = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    constexpr bool ROWS = decltype(with_rows)::value;
+    const FastDiv per_row(K / Form<T>::N);
+    const uint64_t units = static_cast<uint64_t>(rows) * per_row.d;
+    quantize_kernel<T, ROWS><<<grid_for(units, 256), 256, 0, s>>>(p, static_cast<uint32_t>(units), per_row, row_stride,
+                                                                  codes, scales);
+  };
+  auto either = [&](auto* p) {
+    if (rows == 1 || row_stride == K) go(p, std::false_type{});
+    else go(p, std::true_type{});
   };
   switch (type) {
-    case kTypeBf16: go(static_cast<const __nv_bfloat16*>(x)); break;
-    case kTypeF16: go(static_cast<const __half*>(x)); break;
-    case kTypeF32: go(static_cast<const float*>(x)); break;
-    case kTypeE4m3: go(static_cast<const __nv_fp8_e4m3*>(x)); break;
+    case kTypeBf16: either(static_cast<const __nv_bfloat16*>(x)); break;
+    case kTypeF16: either(static_cast<const __half*>(x)); break;
+    case kTypeF32: either(static_cast<const float*>(x)); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -216,7 +334,7 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
 cudaError_t launch_dequantize(const uint8_t* codes, const uint8_t* scales, long long blocks, int type, void* out,
                               cudaStream_t s) {
   const uint64_t units = static_cast<uint64_t>(blocks) * 4;
-  const int grid = grid_for(units, 256);
+  const int grid = grid_for(units, 1024);
   const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
   switch (type) {
     case kTypeBf16: dequantize_kernel<<<grid, 256, 0, s>>>(c, scales, units, static_cast<__nv_bfloat16*>(out)); break;

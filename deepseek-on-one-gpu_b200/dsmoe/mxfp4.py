@@ -29,7 +29,7 @@ import threading
 import torch
 
 from . import _lib
-from ._lib import check, lib, ptr, stream_handle
+from ._lib import check, lib, ptr
 
 BLOCK = 32
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
@@ -68,6 +68,11 @@ def _index(device: torch.device) -> torch.device:
     return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
+def stream_handle(device: torch.device) -> int:
+    """The device's current stream, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 _HERE = contextlib.nullcontext()
 
 
@@ -92,16 +97,16 @@ def _require(what: str, *tensors: torch.Tensor) -> None:
             raise RuntimeError(f"{what} has no backward: detach the inputs or call it under torch.no_grad()")
 
 
-def _rows(x: torch.Tensor, align: int) -> torch.Tensor:
+def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as (rows, K) with unit column stride, rows that do not overlap
-    and start on ``align`` bytes; a copy only where the strides need one."""
-    K = x.shape[-1]
-    x2 = x.reshape(-1, K)
-    if x2.stride(1) != 1 and K > 1:
-        return x2.contiguous()
-    if x2.data_ptr() % align or (x2.shape[0] > 1 and (x2.stride(0) < K or x2.stride(0) * x2.element_size() % align)):
-        return x2.clone(memory_format=torch.contiguous_format)
-    return x2
+    and start on 16 bytes; a copy only where the strides need one."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    rows, K = x.shape
+    step, unit = x.stride()
+    if (unit != 1 and K > 1) or x.data_ptr() % 16 or (rows > 1 and (step < K or step * x.element_size() % 16)):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
 
 
 def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
@@ -116,7 +121,7 @@ def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
 def _quantize_into(x: torch.Tensor, scale_inv: torch.Tensor | None, codes: torch.Tensor, scales: torch.Tensor) -> None:
     K = x.shape[-1]
     fp8 = x.dtype == torch.float8_e4m3fn
-    x2 = _rows(x, 8 if fp8 else 16)
+    x2 = _rows(x)
     per = x.shape[-2] if fp8 else 1
     with _on(x.device):
         check(lib().dsmoe_mxfp4_quantize(ptr(x2), _DTYPES[x.dtype], x2.shape[0], K, x2.stride(0), ptr(scale_inv),
@@ -262,7 +267,7 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
     infinity or a NaN comes out as NaN."""
     _check_weight("mxfp4_linear", weight, False)
     _check_x("mxfp4_linear", x, weight.in_features, weight.codes)
-    x2 = _rows(x, 16)
+    x2 = _rows(x)
     T, K, N = x2.shape[0], weight.in_features, weight.out_features
     out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
     if T:
@@ -315,7 +320,7 @@ def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Te
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (R, N) or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a dense, 16-byte aligned bf16 tensor ({R}, {N})")
     if R:
-        x2, off = _rows(x, 16), offsets.contiguous()
+        x2, off = _rows(x), offsets.contiguous()
         with _on(x.device):
             need = lib().dsmoe_mxfp4_grouped_linear_workspace_size(R, K, N, weight.experts)
             ws = _scratch(need, x.device)
@@ -373,7 +378,7 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     if topk_idx.dim() < 1 or topk_idx.shape != topk_w.shape or tuple(topk_idx.shape[:-1]) != lead:
         raise ValueError(f"mxfp4_moe: indices {tuple(topk_idx.shape)} and weights {tuple(topk_w.shape)} do not go with "
                          f"hidden {tuple(hidden.shape)}")
-    x2 = _rows(hidden, 16)
+    x2 = _rows(hidden)
     T, H, K = x2.shape[0], experts.hidden, topk_idx.shape[-1]
     out = torch.empty(*lead, H, dtype=torch.bfloat16, device=hidden.device)
     if T:

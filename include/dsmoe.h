@@ -443,7 +443,8 @@ enum { DSMOE_BF16 = 0, DSMOE_F16 = 1, DSMOE_F32 = 2, DSMOE_E4M3 = 3 };
  * codes 0, a zero block scale byte 0. DSMOE_E4M3 takes the checkpoint's form:
  * scale_inv fp32 [rows / rows_per_matrix][ceil(rows_per_matrix/128)][ceil(cols/128)]
  * multiplies 128x128 blocks, and the exact products are rounded (a product
- * beyond fp32's largest number saturates there). Rows start on 16 bytes (e4m3: 8).
+ * beyond fp32's largest number saturates there). Rows start on 16 bytes; codes
+ * are 8-byte aligned.
  */
 DSMOE_API int dsmoe_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t row_stride,
                                    const float* scale_inv, int64_t rows_per_matrix, void* codes, void* scales,
