@@ -108,9 +108,17 @@ __device__ __forceinline__ float2 mul_odd(float2 w, float s) {
   return make_float2(odd(a.x, b.x), odd(a.y, b.y));
 }
 
-__device__ __forceinline__ uint32_t e2m1x2(float lo, float hi) {
+// 8 numbers to e2m1 codes, the first in the lowest nibble.
+__device__ __forceinline__ uint32_t e2m1x8(const float* v) {
   uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
 
@@ -153,10 +161,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
     uint32_t w[N / 8];
 #pragma unroll
     for (int j = 0; j < N / 8; ++j) {
-      w[j] = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[j] |= e2m1x2(v[8 * j + 2 * i] * inv, v[8 * j + 2 * i + 1] * inv) << (8 * i);
-      if (byte == 255) w[j] = 0;
+      for (int i = 0; i < 8; ++i) v[8 * j + i] *= inv;
+      w[j] = byte == 255 ? 0 : e2m1x8(v + 8 * j);
     }
     if (in) {
       if constexpr (N == 16) reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
@@ -195,13 +202,18 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* 
     const float wmax = __half2float(__hmax_nan(__low2half(m), __high2half(m)));
     const uint32_t byte = scale_byte(__float_as_uint(mul_odd(wmax, s)) & 0x7fffffffu);
     const float sc = s * __uint_as_float((254u - byte) << 23);
-    uint32_t w[2] = {0, 0};
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 p = mul_odd(__half22float2(v[i]), sc);
-      w[i >> 2] |= e2m1x2(p.x, p.y) << (8 * (i & 3));
+    for (int j = 0; j < 2; ++j) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 o = mul_odd(__half22float2(v[4 * j + i]), sc);
+        p[2 * i] = o.x;
+        p[2 * i + 1] = o.y;
+      }
+      w[j] = byte == 255 ? 0 : e2m1x8(p);
     }
-    if (byte == 255) w[0] = w[1] = 0;
     if (in) {
       reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
       if ((u & 1) == 0) scales[u >> 1] = static_cast<uint8_t>(byte);
@@ -209,10 +221,17 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* 
   }
 }
 
-__device__ __forceinline__ float2 e2m1_pair(uint32_t byte) {
-  uint32_t h;
-  asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(byte));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
+// 8 codes as four f16 pairs (exact).
+__device__ __forceinline__ void e2m1_read(uint32_t w, __half2* h) {
+  uint32_t* o = reinterpret_cast<uint32_t*>(h);
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "mov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
 }
 
 __device__ __forceinline__ float e8m0(uint32_t b) {
@@ -258,10 +277,12 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
       const uint64_t u = u0 + 256 * g;
       if (u >= units) break;
       const float s = e8m0(b[g]);
+      __half2 h[4];
+      e2m1_read(w[g], h);
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 f = e2m1_pair((w[g] >> (8 * i)) & 0xff);
+        const float2 f = __half22float2(h[i]);
         v[2 * i] = f.x * s;
         v[2 * i + 1] = f.y * s;
       }
