@@ -198,12 +198,20 @@ int check_cfg(const dsmoe_moe_config_t* c) {
   return DSMOE_OK;
 }
 
-int do_route(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, const float* bias, int T,
-             int64_t* idx64, float* w_out, const Ws& L, void* ws, cudaStream_t s) {
+// Scratch of one router call.
+struct RouteBufs {
+  float* partial;  // [ksplit][T][E]
+  int32_t* idx;    // [T][top_k]
+  float* w;        // [T][top_k]
+  int* status;
+  int ksplit;
+};
+
+int run_route(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, const float* bias, int T,
+              int64_t* idx64, float* w_out, const RouteBufs& b, cudaStream_t s) {
   if (!hidden || !gate) return fail(DSMOE_ERR_INVALID, "hidden / gate_weight is NULL");
   if (!aligned16(hidden) || !aligned16(gate)) return fail(DSMOE_ERR_INVALID, "hidden / gate_weight not 16-byte aligned");
   if (c->router_mode == DSMOE_ROUTER_V3 && !bias) return fail(DSMOE_ERR_INVALID, "router v3 needs score_bias");
-  float* partial = at<float>(ws, L.partial);
   CUtensorMap m_x, m_g;
   int r;
   if ((r = make_map(&m_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, hidden, c->hidden, T, 64, 128,
@@ -213,15 +221,21 @@ int do_route(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, 
                     CU_TENSOR_MAP_SWIZZLE_128B)))
     return r;
   prof(0, s);
-  DSMOE_CUDA(launch_router_logits_tc(m_x, m_g, partial, T, c->hidden, c->n_routed, L.ksplit, at<int>(ws, L.status),
-                                     s));
-  DSMOE_CUDA(launch_router_select(partial, L.ksplit, bias, T, c->n_routed, c->n_group, c->topk_group, c->top_k,
-                                  c->router_mode, c->norm_topk_prob, c->routed_scaling_factor, at<int32_t>(ws, L.idx),
-                                  idx64, at<float>(ws, L.w), s));
-  if (w_out) DSMOE_CUDA(cudaMemcpyAsync(w_out, at<float>(ws, L.w), sizeof(float) * T * c->top_k,
+  DSMOE_CUDA(launch_router_logits_tc(m_x, m_g, b.partial, T, c->hidden, c->n_routed, b.ksplit, b.status, s));
+  DSMOE_CUDA(launch_router_select(b.partial, b.ksplit, bias, T, c->n_routed, c->n_group, c->topk_group, c->top_k,
+                                  c->router_mode, c->norm_topk_prob, c->routed_scaling_factor, b.idx, idx64, b.w,
+                                  s));
+  if (w_out) DSMOE_CUDA(cudaMemcpyAsync(w_out, b.w, sizeof(float) * T * c->top_k,
                                         cudaMemcpyDeviceToDevice, s));
   prof(1, s);
   return DSMOE_OK;
+}
+
+int do_route(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, const float* bias, int T,
+             int64_t* idx64, float* w_out, const Ws& L, void* ws, cudaStream_t s) {
+  return run_route(c, hidden, gate, bias, T, idx64, w_out,
+                   {at<float>(ws, L.partial), at<int32_t>(ws, L.idx), at<float>(ws, L.w), at<int>(ws, L.status), L.ksplit},
+                   s);
 }
 
 int check_weights(const dsmoe_moe_config_t* c, const dsmoe_layer_weights_t* w) {
@@ -371,6 +385,26 @@ int make_tma_map(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, con
                  uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
   return make_map_strided(m, dt, row_bytes, base, cols, rows, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
+size_t route_scratch_bytes(const dsmoe_moe_config_t* c, int T) {
+  if (check_cfg(c) != DSMOE_OK) return 0;
+  const size_t pairs = 4 * static_cast<size_t>(T) * c->top_k;
+  return align_up(sizeof(float) * static_cast<size_t>(router_tc_ksplit(T, c->hidden, 148)) * T * c->n_routed) +
+         2 * align_up(pairs);
+}
+
+int route_private(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, const float* bias, int T,
+                  int64_t* idx64, float* w, void* scratch, int* status, cudaStream_t s) {
+  RouteBufs b;
+  b.ksplit = router_tc_ksplit(T, c->hidden, 148);
+  b.partial = static_cast<float*>(scratch);
+  size_t o = align_up(sizeof(float) * static_cast<size_t>(b.ksplit) * T * c->n_routed);
+  b.idx = at<int32_t>(scratch, o);
+  o += align_up(4 * static_cast<size_t>(T) * c->top_k);
+  b.w = at<float>(scratch, o);
+  b.status = status;
+  return run_route(c, hidden, gate, bias, T, idx64, w, b, s);
+}
+
 int sm_count() { return num_sms(); }
 int gemm_grid() { return g_gemm_ctas > 0 && g_gemm_ctas < num_sms() ? g_gemm_ctas : num_sms(); }
 

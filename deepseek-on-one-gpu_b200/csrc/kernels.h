@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/dsmoe.h"
+
 namespace dsmoe {
 
 // Records `msg` as the calling thread's dsmoe_last_error() and returns `code`.
@@ -13,6 +15,11 @@ int set_last_error(int code, const char* msg);
 // 2-D row-major TMA map with a 128-byte swizzle; returns a DSMOE_* code.
 int make_tma_map(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
                  uint64_t rows, uint32_t box_cols, uint32_t box_rows);
+// The router with scratch of its own (route_scratch_bytes, 256-byte aligned,
+// uninitialised) and errors in *status; 0 bytes: a config it does not take.
+size_t route_scratch_bytes(const dsmoe_moe_config_t* c, int T);
+int route_private(const dsmoe_moe_config_t* c, const void* hidden, const void* gate, const float* bias, int T,
+                  int64_t* idx64, float* w, void* scratch, int* status, cudaStream_t s);
 int sm_count();   // SMs of the current device
 int gemm_grid();  // CTAs of a persistent GEMM launch (dsmoe_set_gemm_sm_limit)
 // Device address of the current device's allocation-free scratch status word

@@ -430,4 +430,36 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   return DSMOE_OK;
 }
 
+size_t dsmoe_mxfp4_moe_forward_workspace_size(const dsmoe_moe_config_t* cfg, int32_t tokens) {
+  if (!cfg || tokens <= 0 || check_moe(tokens, cfg->hidden, cfg->inter, cfg->n_routed, 1, cfg->top_k)) return 0;
+  const size_t route = route_scratch_bytes(cfg, tokens);
+  return route ? route + dsmoe_mxfp4_moe_workspace_size(tokens, cfg->hidden, cfg->inter, cfg->n_routed, 1, cfg->top_k) : 0;
+}
+
+int dsmoe_mxfp4_moe_forward(const dsmoe_moe_config_t* cfg, const void* gate_weight, const float* score_bias,
+                            const dsmoe_mxfp4_experts_t* w, const void* hidden, int32_t tokens, void* out,
+                            int64_t* topk_idx, float* topk_w, void* workspace, size_t workspace_bytes,
+                            int32_t* device_status, dsmoe_stream_t stream) {
+  if (!cfg || !w) return fail(DSMOE_ERR_INVALID, "mxfp4_moe_forward: config or weights is NULL");
+  if (tokens < 0) return fail(DSMOE_ERR_INVALID, "mxfp4_moe_forward: negative token count");
+  if (w->hidden != cfg->hidden || w->inter != cfg->inter || w->n_routed != cfg->n_routed || w->shared != 1)
+    return fail(DSMOE_ERR_INVALID, "mxfp4_moe_forward: weights do not go with the config (shared expert included)");
+  int r = check_moe(tokens, cfg->hidden, cfg->inter, cfg->n_routed, 1, cfg->top_k);
+  if (r) return r;
+  if (tokens == 0) return DSMOE_OK;
+  const size_t route = route_scratch_bytes(cfg, tokens);
+  if (route == 0) return DSMOE_ERR_UNSUPPORTED;  // the router's check left its message
+  if (!aligned(topk_idx, 8) || !aligned(topk_w, 4) || !aligned(device_status, 4))
+    return fail(DSMOE_ERR_INVALID, "mxfp4_moe_forward: pointer NULL or unaligned");
+  if ((r = check_ws("mxfp4_moe_forward", workspace, workspace_bytes,
+                    dsmoe_mxfp4_moe_forward_workspace_size(cfg, tokens))))
+    return r;
+  if ((r = route_private(cfg, hidden, gate_weight, score_bias, tokens, topk_idx, topk_w, workspace, device_status,
+                         reinterpret_cast<cudaStream_t>(stream))))
+    return r;
+  const float scale = cfg->router_mode == DSMOE_ROUTER_V3 ? 1.0f : cfg->routed_scaling_factor;
+  return dsmoe_mxfp4_moe(hidden, cfg->hidden, tokens, w, topk_idx, topk_w, cfg->top_k, scale, out,
+                         at<uint8_t>(workspace, route), workspace_bytes - route, device_status, stream);
+}
+
 }  // extern "C"

@@ -31,6 +31,7 @@ EXPORTED = (
     "dsmoe_mxfp4_scale_atoms", "dsmoe_mxfp4_linear_workspace_size", "dsmoe_mxfp4_linear",
     "dsmoe_mxfp4_matmul_workspace_size", "dsmoe_mxfp4_matmul", "dsmoe_mxfp4_grouped_linear_workspace_size",
     "dsmoe_mxfp4_grouped_linear", "dsmoe_mxfp4_moe_workspace_size", "dsmoe_mxfp4_moe",
+    "dsmoe_mxfp4_moe_forward_workspace_size", "dsmoe_mxfp4_moe_forward",
 )
 
 
@@ -155,6 +156,10 @@ def lib() -> ctypes.CDLL:
                 L.dsmoe_mxfp4_moe_workspace_size.restype = sz
                 L.dsmoe_mxfp4_moe.argtypes = [vp, i64, i32, ctypes.POINTER(MXFP4ExpertsDesc), vp, vp, i32, f32, vp, vp,
                                               sz, vp, vp]
+                L.dsmoe_mxfp4_moe_forward_workspace_size.argtypes = [cfgp, i32]
+                L.dsmoe_mxfp4_moe_forward_workspace_size.restype = sz
+                L.dsmoe_mxfp4_moe_forward.argtypes = [cfgp, vp, vp, ctypes.POINTER(MXFP4ExpertsDesc), vp, i32, vp, vp,
+                                                      vp, vp, sz, vp, vp]
                 for name in EXPORTED:
                     getattr(L, name).restype = getattr(L, name).restype or ctypes.c_int
                 _lib = L

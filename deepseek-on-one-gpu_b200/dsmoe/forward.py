@@ -14,7 +14,9 @@ device weight bank. In streaming mode (fewer slots than experts) with a
 device-managed slot table (``device_slots``) the missing experts are placed
 and copied by ``dsmoe_slotcache_step`` on the device; otherwise the routing is
 read back once per block (the reference reads it back once per token, via
-``.tolist()``) to bring missing experts in before the expert GEMMs.
+``.tolist()``) to bring missing experts in before the expert GEMMs. With
+``expert_format="mxfp4"`` the experts are 4-bit and run through
+``mxfp4.moe_forward`` (fp32 combine, one rounding of the result).
 """
 from __future__ import annotations
 
@@ -22,6 +24,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib, ptr, require_cuda, stream_handle
+from .mxfp4 import MXFP4LayerBank, moe_forward
 
 
 def _layer_weights(bank, gate_weight, bias) -> _lib.LayerWeights:
@@ -51,12 +54,15 @@ def moe_block(hidden: torch.Tensor, layer_idx: int, weight_store, gpu_transfer, 
     require_cuda(x, gate_weight, bias)
     cfg = _lib.moe_config(config)
     K = cfg.top_k
+    bank = gpu_transfer.bank(layer_idx)
+    if isinstance(bank, MXFP4LayerBank):
+        out, idx, w = moe_forward(x, gate_weight, bias, config, bank.experts)
+        return _result(hidden, out, idx, w, return_routing)
     out = torch.empty_like(x)
     idx = torch.empty(T, K, dtype=torch.int64, device=x.device)
     w = torch.empty(T, K, dtype=torch.float32, device=x.device)
     ws = _lib.Workspace.get(x.device).ensure(lib().dsmoe_workspace_size(cfg, T))
     stream = stream_handle(x.device)
-    bank = gpu_transfer.bank(layer_idx)
     if bank.fully_resident:
         lw = _layer_weights(bank, gate_weight, bias)
         check(lib().dsmoe_moe_forward(cfg, lw, ptr(x), T, ptr(out), ptr(idx), ptr(w), ptr(ws), ws.numel(), stream),
@@ -76,9 +82,13 @@ def moe_block(hidden: torch.Tensor, layer_idx: int, weight_store, gpu_transfer, 
         check(lib().dsmoe_moe_experts(cfg, lw, ptr(x), T, ptr(out), ptr(ws), ws.numel(), stream),
               "dsmoe_moe_experts")
     gpu_transfer.mark_used(layer_idx)
+    return _result(hidden, out, idx, w, return_routing)
+
+
+def _result(hidden, out, idx, w, return_routing: bool):
     out = out.view(hidden.shape)
     if return_routing:
-        shape = tuple(hidden.shape[:-1]) + (K,)
+        shape = tuple(hidden.shape[:-1]) + (idx.shape[-1],)
         return out, idx.view(shape), w.view(shape)
     return out
 
@@ -98,7 +108,7 @@ def moe_layer_ffn(hidden: torch.Tensor, layer_idx: int, weight_store, gpu_transf
     _, post_ln = weight_store.get_layer_norm_weights(layer_idx)
     eps = float(getattr(config, "rms_norm_eps", 1e-6))
     bank = gpu_transfer.bank(layer_idx)
-    if not bank.fully_resident:
+    if not bank.fully_resident or isinstance(bank, MXFP4LayerBank):
         from .ops import rms_norm
         normed = rms_norm(x, post_ln, eps)
         return (x + moe_block(normed, layer_idx, weight_store, gpu_transfer, config, verbose=verbose)).view(

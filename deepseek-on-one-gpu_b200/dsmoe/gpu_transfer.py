@@ -23,6 +23,10 @@ on the GPU by ``dsmoe_slotcache_step`` (``DeviceSlotCache``), which places the
 step's missing experts in least-recently-used slots and copies them from host
 memory with the SMs, all on the compute stream: the routing is never read
 back and the host never waits.
+
+4-bit experts (``expert_format="mxfp4"``, resident mode): each layer's experts
+are quantised to MXFP4 as they come in (``mxfp4.MXFP4LayerBank``, 17/32 of the
+FP8 bytes) and ``moe_block`` / ``moe_layer_ffn`` run on them.
 """
 from __future__ import annotations
 
@@ -173,7 +177,13 @@ class GPUTransfer:
     ``transfer_experts`` signature (``inference/gpu_transfer.py:15-16,50-52``)."""
 
     def __init__(self, config, weight_store, device, verbose: bool = False, slots_per_layer: int | None = None,
-                 device_slots: bool = False):
+                 device_slots: bool = False, expert_format: str = "fp8"):
+        if expert_format not in ("fp8", "mxfp4"):
+            raise ValueError(f"expert_format is \"fp8\" or \"mxfp4\", not {expert_format!r}")
+        if expert_format == "mxfp4" and (device_slots or (slots_per_layer or config.n_routed_experts + 1)
+                                         < config.n_routed_experts + 1):
+            raise ValueError("mxfp4 experts are resident: slots_per_layer and device_slots go with fp8")
+        self.expert_format = expert_format
         self.config = config
         self.weight_store = weight_store
         self.device = torch.device(device)
@@ -197,7 +207,11 @@ class GPUTransfer:
     def bank(self, layer: int) -> LayerBank:
         b = self.banks.get(layer)
         if b is None:
-            b = LayerBank(self.config, self.slots, self.device)
+            if self.expert_format == "mxfp4":
+                from .mxfp4 import MXFP4LayerBank
+                b = MXFP4LayerBank(self.config, self.device)
+            else:
+                b = LayerBank(self.config, self.slots, self.device)
             self.banks[layer] = b
             if self.resident and hasattr(self.weight_store, "fill_bank"):
                 self.weight_store.fill_bank(layer, b)
@@ -230,7 +244,7 @@ class GPUTransfer:
         experts whose copy was started."""
         b = self.bank(layer)
         missing = [g for g in dict.fromkeys(int(e) + 1 for e in experts) if b.slot_of_host[g] < 0]
-        if not missing:
+        if not missing:  # always so with mxfp4 experts
             return 0
         ts = self.transfer_stream
         if b.last_use is not None:
@@ -282,6 +296,8 @@ class GPUTransfer:
         self.banks[layer].last_use = ev
 
     def transfer_experts(self, layer: int, expert_indices: torch.Tensor, verbose: bool = False):
+        if self.expert_format == "mxfp4":
+            raise TypeError("transfer_experts hands out FP8 (weight, scale) pairs; mxfp4 experts have none")
         indices = [int(i) for i in expert_indices.reshape(-1).tolist()]
         b = self.ensure_resident(layer, indices)
         if verbose or self.verbose:

@@ -12,7 +12,8 @@ users who halve the expert memory and the bytes a decode step reads:
   * ``mxfp4_linear``           bf16 activations times an MXFP4 weight;
   * ``mxfp4_matmul``           MXFP4 activations times an MXFP4 weight;
   * ``mxfp4_grouped_linear``   rows sorted by expert times each expert's weight;
-  * ``MXFP4Experts`` / ``mxfp4_moe``  the routed FFN after ``route``.
+  * ``MXFP4Experts`` / ``mxfp4_moe``  the routed FFN after ``route``;
+  * ``MXFP4LayerBank``         a layer's experts, filled from FP8 weights.
 
 ``GPUTransfer(..., expert_format="mxfp4")`` makes ``moe_block`` and
 ``moe_layer_ffn`` run on 4-bit experts. Every call goes through
@@ -238,6 +239,11 @@ class MXFP4Weight:
         return self
 
     def _set(self, slot: int, weight: torch.Tensor, scale_inv: torch.Tensor | None) -> None:
+        if tuple(weight.shape) != (self.out_features, self.in_features):
+            raise ValueError(f"expert weight is {tuple(weight.shape)}, the stack holds "
+                             f"{(self.out_features, self.in_features)}")
+        if scale_inv is not None and tuple(scale_inv.shape) != (-(-self.out_features // 128), self.in_features // 128):
+            raise ValueError("scale_inv does not go with the weight")
         scales = torch.empty(self.out_features, self.in_features // BLOCK, dtype=torch.uint8, device=self.device)
         _quantize_into(weight, scale_inv, self.codes[slot], scales)
         self._pack(scales, slot, 1)
@@ -390,3 +396,70 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
                                         float(scale), ptr(out), ptr(ws) or None, ws.numel(), ptr(experts.gate.status),
                                         stream_handle(hidden.device)), "dsmoe_mxfp4_moe")
     return out
+
+
+def moe_forward(x: torch.Tensor, gate_weight: torch.Tensor, bias: torch.Tensor | None, config,
+                experts: MXFP4Experts) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``moe_block``'s work on MXFP4 experts: dense bf16 ``x`` [T, hidden] ->
+    output, routing indices and weights. Scratch is private to the call."""
+    _check_x("moe_forward", x, experts.hidden, gate_weight, bias, experts.gate.codes)
+    cfg = _lib.moe_config(config)
+    T, K = x.shape[0], cfg.top_k
+    out = torch.empty_like(x)
+    idx = torch.empty(T, K, dtype=torch.int64, device=x.device)
+    w = torch.empty(T, K, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        ws = _scratch(lib().dsmoe_mxfp4_moe_forward_workspace_size(cfg, T), x.device)
+        check(lib().dsmoe_mxfp4_moe_forward(cfg, ptr(gate_weight), ptr(bias), ctypes.byref(experts.desc), ptr(x), T,
+                                            ptr(out), ptr(idx), ptr(w), ptr(ws) or None, ws.numel(),
+                                            ptr(experts.gate.status), stream_handle(x.device)),
+              "dsmoe_mxfp4_moe_forward")
+    return out, idx, w
+
+
+class MXFP4LayerBank:
+    """Every expert of one MoE layer in MXFP4 on the device (6.0 GB per
+    DeepSeek-R1 layer, against 11.3 GB in FP8), written expert by expert from
+    the checkpoint's FP8 weights. Stands where ``GPUTransfer`` keeps a
+    ``LayerBank``; every expert is resident, group 0 is the shared expert."""
+
+    def __init__(self, config, device: torch.device):
+        E, H, F = config.n_routed_experts, config.hidden_size, config.moe_intermediate_size
+        self.n_slots = self.n_groups = E + 1
+        self.device = _index(torch.device(device))
+        self.w = {"gate_proj": MXFP4Weight._empty(E + 1, F, H, self.device),
+                  "up_proj": MXFP4Weight._empty(E + 1, F, H, self.device),
+                  "down_proj": MXFP4Weight._empty(E + 1, H, F, self.device)}
+        self.experts = MXFP4Experts(self.w["gate_proj"], self.w["up_proj"], self.w["down_proj"], shared=True)
+        self.slot_of_host = [-1] * (E + 1)
+        self.last_use: torch.cuda.Event | None = None
+        self.pending: torch.cuda.Event | None = None
+
+    @property
+    def fully_resident(self) -> bool:
+        return all(s >= 0 for s in self.slot_of_host)
+
+    @property
+    def nbytes(self) -> int:
+        return self.experts.nbytes
+
+    def assign(self, group: int, pinned=None) -> int:
+        self.slot_of_host[group] = group
+        return group
+
+    def write_slot(self, slot: int, expert: dict, non_blocking: bool = False) -> int:
+        """Quantise one FP8 expert ``{proj: (weight, scale_inv)}``, on the host
+        or the device, into ``slot``; returns the FP8 bytes read."""
+        n = 0
+        for p, stack in self.w.items():
+            w, s = expert[p]
+            if isinstance(w, dict):  # ExpertCache entry form
+                w, s = w["weight"], w["weight_scale_inv"]
+            n += w.nbytes + s.nbytes
+            w = w.to(self.device, non_blocking=non_blocking)
+            s = s.to(self.device, torch.float32, non_blocking=non_blocking).contiguous()
+            stack._set(slot, w, s)
+        return n
+
+    def sync_table(self, non_blocking: bool = True) -> None:
+        """Nothing to bring up to date: slot g is group g."""

@@ -521,6 +521,19 @@ DSMOE_API int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t to
                               int32_t top_k, float scale, void* out, void* workspace, size_t workspace_bytes,
                               int32_t* device_status, dsmoe_stream_t stream);
 
+/*
+ * The whole MoE block on MXFP4 experts (shared expert included): dsmoe_route's
+ * routing, then dsmoe_mxfp4_moe, scaled as dsmoe_moe_forward does. hidden
+ * [tokens][hidden] dense; topk_idx [tokens][top_k] and topk_w receive the
+ * routing (not NULL). `workspace` as for the entry points above: it shares
+ * nothing with dsmoe_route's.
+ */
+DSMOE_API size_t dsmoe_mxfp4_moe_forward_workspace_size(const dsmoe_moe_config_t* cfg, int32_t tokens);
+DSMOE_API int dsmoe_mxfp4_moe_forward(const dsmoe_moe_config_t* cfg, const void* gate_weight, const float* score_bias,
+                                      const dsmoe_mxfp4_experts_t* weights, const void* hidden, int32_t tokens,
+                                      void* out, int64_t* topk_idx, float* topk_w, void* workspace,
+                                      size_t workspace_bytes, int32_t* device_status, dsmoe_stream_t stream);
+
 /* Reads (synchronously) and clears the device error word kept in `workspace`.
  * workspace == NULL reads the error word of dsmoe_expert_ffn_noalloc's
  * library-owned scratch on the current device: that entry point has no

@@ -145,6 +145,26 @@ def test_moe_rejects(kw, code):
     assert L.dsmoe_mxfp4_moe(256, 512, 4, None, 256, 256, 2, 1.0, 256, 256, BIG, 256, None) == -1
 
 
+def test_moe_forward_rejects():
+    L = _lib.lib()
+
+    def call(cfg=None, d=None, gate=256, bias=None, x=256, t=4, out=256, idx=256, w=256, ws=256, nbytes=BIG, st=256):
+        c = _lib.MoeConfig(**{**dict(hidden=512, inter=256, n_routed=64, n_group=2, topk_group=1, top_k=4, router_mode=0,
+                                     norm_topk_prob=1, routed_scaling_factor=2.5), **(cfg or {})})
+        e = _lib.MXFP4ExpertsDesc(**{**dict(hidden=512, inter=256, n_routed=64, shared=1, gate_codes=256, gate_atoms=256,
+                                            up_codes=256, up_atoms=256, down_codes=256, down_atoms=256), **(d or {})})
+        return L.dsmoe_mxfp4_moe_forward(c, gate, bias, ctypes.byref(e), x, t, out, idx, w, ws, nbytes, st, None)
+
+    assert call(t=-1) == -1 and call(t=0) == 0
+    assert call(d=dict(shared=0)) == -1 and call(d=dict(n_routed=32)) == -1 and call(d=dict(hidden=256)) == -1
+    assert call(cfg=dict(topk_group=3)) == -4
+    assert call(idx=None) == -1 and call(w=None) == -1 and call(st=None) == -1
+    assert call(ws=272) == -1 and call(nbytes=1000) == -3
+    assert call(gate=None) == -1 and call(x=264) == -1
+    assert call(cfg=dict(router_mode=1)) == -1  # the bias-corrected router needs the bias
+    assert L.dsmoe_mxfp4_moe_forward(None, 256, None, None, 256, 4, 256, 256, 256, 256, BIG, 256, None) == -1
+
+
 def test_workspace_sizes():
     L = _lib.lib()
     assert L.dsmoe_mxfp4_linear_workspace_size(4096, 7168, 2048) >= 2 * 4096 * 7168
