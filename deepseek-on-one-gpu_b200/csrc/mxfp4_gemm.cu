@@ -23,7 +23,7 @@
 //              for each A tile: per stage the thread copies the scale atoms to
 //              its TMEM columns (tcgen05.cp) and issues the MMAs behind them
 //   warp 3     unit planner, a shared-memory ring of decoded units
-//   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 16-column chunks
+//   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 8-column chunks
 // TMEM: two halves of accumulator columns, then one set of scale columns per
 // stage (a stage's scales are overwritten only after its MMAs released it). A
 // unit that fits a half alternates between them, so its epilogue overlaps the
@@ -40,7 +40,7 @@ constexpr int RING = 4;
 constexpr int PLAN_WARP = 3;
 constexpr int EPI_WARP0 = 4;
 constexpr int NUM_CG = kEpiWarps / 4;
-constexpr int CHUNK = 16;
+constexpr int CHUNK = 8;
 constexpr int THREADS = (EPI_WARP0 + kEpiWarps) * 32;
 
 struct Unit {
@@ -81,6 +81,7 @@ struct Cfg {
   static constexpr int SF_TOTAL = STAGES * 2 * SF_COLS;
   static constexpr int HALF = (512 - SF_TOTAL) / 2 / 16 * 16;
   static constexpr int SF_BASE = 2 * HALF;
+  static constexpr int CHUNKS = (BN + NUM_CG * CHUNK - 1) / (NUM_CG * CHUNK);  // of an epilogue warp
   static constexpr int BAR_OFF = STAGES * (OP_BYTES + SF_BYTES);
   // full[S], empty[S], tfull[2], tempty[2], done, ufull[RING], uempty[RING]
   static constexpr int NUM_BARS = 2 * STAGES + 5 + 2 * RING;
@@ -216,21 +217,20 @@ __device__ __forceinline__ int unit_count(const GemmArgs& p, int bn, bool swiglu
   return tiles * per * p.ksplit;
 }
 
-// bf16 pairs of features: an even lane stores features (lane, lane + 1) of
-// token c, its odd neighbour those of token c + 1.
-__device__ __forceinline__ void store_pairs(const float* v, int c0, int ncols, int feat_ok, __nv_bfloat16* y,
-                                            size_t ld, int lane) {
-  const int odd = lane & 1;
-#pragma unroll
-  for (int c = 0; c < CHUNK; c += 2) {
-    const unsigned short a = __bfloat16_as_ushort(__float2bfloat16_rn(v[c]));
-    const unsigned short b = __bfloat16_as_ushort(__float2bfloat16_rn(v[c + 1]));
-    const uint32_t mine = odd ? b : a;
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(odd ? a : b), 1);
-    const uint32_t pair = odd ? (other | (mine << 16)) : (mine | (other << 16));
-    const int tok = c0 + c + odd;
-    if (tok < ncols && feat_ok) *reinterpret_cast<uint32_t*>(y + tok * ld) = pair;
-  }
+// Four tokens' bf16 values of 32 features, packed by token pairs (p01: tokens 0
+// and 1 of this lane's feature), transposed over groups of 4 lanes: lane l
+// gets features (l & ~3) .. + 3 of token l & 3.
+__device__ __forceinline__ uint2 transpose4(uint32_t p01, uint32_t p23, int lane) {
+  const uint32_t sel = lane & 1 ? 0x3276 : 0x5410;
+  const uint32_t a = __byte_perm(p01, __shfl_xor_sync(0xffffffffu, p01, 1), sel);
+  const uint32_t b = __byte_perm(p23, __shfl_xor_sync(0xffffffffu, p23, 1), sel);
+  const uint32_t o = __shfl_xor_sync(0xffffffffu, lane & 2 ? a : b, 2);
+  return lane & 2 ? make_uint2(o, b) : make_uint2(a, o);
+}
+// The same for four tokens' bytes.
+__device__ __forceinline__ uint32_t transpose4(uint32_t v, int lane) {
+  v = __byte_perm(v, __shfl_xor_sync(0xffffffffu, v, 1), lane & 1 ? 0x3715 : 0x6240);
+  return __byte_perm(v, __shfl_xor_sync(0xffffffffu, v, 2), lane & 2 ? 0x3276 : 0x5410);
 }
 
 template <class C, bool SWIGLU>
@@ -478,12 +478,13 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
       if (!big) nb ^= 1;
       tc_fence_after();
       const uint32_t d0 = tmem + lanes + b0 * C::HALF, d1 = d0 + nn;
-      // 16 columns from column c on of one accumulator, hi + lo
+      const bool two = e.m1 >= 0;
+      // 8 columns from column c on of one accumulator, hi + lo
       auto load = [&](uint32_t d, int c, float* v) {
-        tmem_ld16(d + c, v);
+        tmem_ld8(d + c, v);
         if (!FP4 && e.both) {
           float l[CHUNK];
-          tmem_ld16(d + e.n + c, l);
+          tmem_ld8(d + e.n + c, l);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < CHUNK; ++j) v[j] += l[j];
@@ -491,92 +492,120 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           tmem_ld_wait();
         }
       };
+      auto column = [&](int j) { return (j * NUM_CG + cg) * CHUNK; };  // of this warp's j-th chunk
+      // The accumulators are read into registers and given back before the
+      // results are rounded and stored: a large unit's MMAs start behind
+      // nothing but that read.
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0)
+          for (int b = b0; b <= b1; ++b) mbar_arrive(&tempty[b]);
+      };
       if constexpr (SWIGLU) {
-        const int f0 = e.m0 + quad * 32;  // this warp's 32 features: one scale block
-        const int KB2 = p.M / 128;
-        for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
-          float h[CHUNK];
-          {
-            float up[CHUNK];
-            load(d0, c0, h);
-            load(d1, c0, up);
+        float h[C::CHUNKS * CHUNK];
 #pragma unroll
-            for (int j = 0; j < CHUNK; ++j) h[j] = __fdividef(h[j], 1.0f + __expf(-h[j])) * up[j];
+        for (int j = 0; j < C::CHUNKS; ++j) {
+          if (column(j) < e.ncols) {  // warp-uniform
+            float g[CHUNK], up[CHUNK];
+            load(d0, column(j), g);
+            load(d1, column(j), up);
+            // silu in fp32 with the fast exp and divide (a few fp32 ulp)
+#pragma unroll
+            for (int t = 0; t < CHUNK; ++t) h[j * CHUNK + t] = __fdividef(g[t], 1.0f + __expf(-g[t])) * up[t];
           }
+        }
+        release();
+        const int f0 = e.m0 + quad * 32;  // this warp's 32 features: one scale block
+        uint8_t* sf = p.hsf + (static_cast<size_t>(e.tile) * (p.M / 128) + e.m0 / 128) * (C::ATOMS * 512) + quad;
+        auto spot = [](int c) { return (c >> 7) * 512 + (c & 31) * 16 + ((c >> 5) & 3) * 4; };
 #pragma unroll
-          for (int j = 0; j < CHUNK; j += 4) {
+        for (int j = 0; j < C::CHUNKS * CHUNK; j += 4) {
+          const int c0 = column(j / CHUNK) + j % CHUNK;
+          if (c0 < e.ncols) {
             uint32_t hi4 = 0, lo4 = 0, bytes = 0;
+            float q[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              const float v = h[j + t];
-              const uint32_t ef = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7fffffffu) >> 23;
+              const uint32_t ef = __reduce_max_sync(0xffffffffu, __float_as_uint(h[j + t]) & 0x7fffffffu) >> 23;
               const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
-              const float inv = ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23);
-              const float q = v * inv;
-              const uint32_t hb = f32x2_to_e4m3x2(q, 0.f) & 0xff;
-              const uint32_t lb = f32x2_to_e4m3x2(q - e4m3_to_f32(static_cast<uint8_t>(hb)), 0.f) & 0xff;
-              hi4 |= hb << (8 * t);
-              lo4 |= lb << (8 * t);
+              q[t] = h[j + t] * (ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23));
               bytes |= byte << (8 * t);
             }
-            // 4x4 byte transpose over groups of 4 lanes: lane l then holds 4
-            // features of token j + l % 4
-            auto transpose = [&](uint32_t v) {
-              uint32_t o = __shfl_xor_sync(0xffffffffu, v, 1);
-              v = __byte_perm(v, o, lane & 1 ? 0x3715 : 0x6240);
-              o = __shfl_xor_sync(0xffffffffu, v, 2);
-              return __byte_perm(v, o, lane & 2 ? 0x3276 : 0x5410);
-            };
-            hi4 = transpose(hi4);
-            lo4 = transpose(lo4);
-            const int col = c0 + j + (lane & 3);
+#pragma unroll
+            for (int t = 0; t < 4; t += 2) {
+              const uint32_t h2 = f32x2_to_e4m3x2(q[t], q[t + 1]);
+              const uint32_t l2 = f32x2_to_e4m3x2(q[t] - e4m3_to_f32(h2 & 0xff), q[t + 1] - e4m3_to_f32(h2 >> 8));
+              hi4 |= h2 << (8 * t);
+              lo4 |= l2 << (8 * t);
+            }
+            hi4 = transpose4(hi4, lane);
+            lo4 = transpose4(lo4, lane);
+            const int col = c0 + (lane & 3);
             if (col < e.ncols) {
               const size_t off = static_cast<size_t>(e.row0 + col) * p.M + f0 + (lane & ~3);
               *reinterpret_cast<uint32_t*>(p.hq + off) = hi4;
               *reinterpret_cast<uint32_t*>(p.hq + static_cast<size_t>(p.P) * p.M + off) = lo4;
               if (lane < 4) {
-                uint8_t* sf = p.hsf + (static_cast<size_t>(e.tile) * KB2 + e.m0 / 128) * (C::ATOMS * 512) + quad;
                 const uint8_t byte = static_cast<uint8_t>(bytes >> (8 * lane));
-                auto spot = [](int c) { return (c >> 7) * 512 + (c & 31) * 16 + ((c >> 5) & 3) * 4; };
                 sf[spot(col)] = byte;
                 if (e.both) sf[spot(col + e.n)] = byte;
               }
             }
           }
         }
-      } else {
-        const bool two = e.m1 >= 0;
-        const int ld_feat = quad * 32 + (lane & ~1);
-        if (p.ksplit == 1) {
-          for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
-            float v[CHUNK];
-            __nv_bfloat16* y = p.y + static_cast<size_t>(e.row0) * p.M + ld_feat;
-            load(d0, c0, v);
-            store_pairs(v, c0, e.ncols, e.m0 + ld_feat < p.M, y + e.m0, p.M, lane);
-            if (two) {
-              load(d1, c0, v);
-              store_pairs(v, c0, e.ncols, e.m1 + ld_feat < p.M, y + e.m1, p.M, lane);
-            }
-          }
-        } else {
-          // This part's sums, fp32, into the (now unused) operand stages:
-          // [column][256 features].
-          float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
-          for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
-            float v[CHUNK];
-            for (int a = 0; a < (two ? 2 : 1); ++a) {
-              load(a ? d1 : d0, c0, v);
+      } else if (p.ksplit == 1) {
+        uint32_t y2[2][C::CHUNKS * CHUNK / 2];  // bf16 pairs of tokens
 #pragma unroll
-              for (int j = 0; j < CHUNK; ++j)
-                if (c0 + j < e.ncols) part[(c0 + j) * 2 * BM + a * BM] = v[j];
+        for (int j = 0; j < C::CHUNKS; ++j) {
+          if (column(j) < e.ncols) {
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              if (a == 0 || two) {
+                float v[CHUNK];
+                load(a ? d1 : d0, column(j), v);
+#pragma unroll
+                for (int t = 0; t < CHUNK; t += 2) {
+                  const __nv_bfloat162 w = __floats2bfloat162_rn(v[t], v[t + 1]);
+                  y2[a][(j * CHUNK + t) / 2] = *reinterpret_cast<const uint32_t*>(&w);
+                }
+              }
             }
           }
         }
+        release();
+        const int f = quad * 32 + (lane & ~3);  // M is a multiple of 8: four features are in or out together
+#pragma unroll
+        for (int j = 0; j < C::CHUNKS * CHUNK; j += 4) {
+          const int c0 = column(j / CHUNK) + j % CHUNK;
+          if (c0 < e.ncols) {
+            const int col = c0 + (lane & 3);
+            __nv_bfloat16* y = p.y + static_cast<size_t>(e.row0 + col) * p.M + f;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              if (a == 0 || two) {
+                const int m = a ? e.m1 : e.m0;
+                const uint2 v = transpose4(y2[a][j / 2], y2[a][j / 2 + 1], lane);
+                if (col < e.ncols && m + f < p.M) *reinterpret_cast<uint2*>(y + m) = v;
+              }
+            }
+          }
+        }
+      } else {
+        // This part's sums, fp32, into the (now unused) operand stages:
+        // [column][256 features].
+        float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
+        for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+          float v[CHUNK];
+          for (int a = 0; a < (two ? 2 : 1); ++a) {
+            load(a ? d1 : d0, c0, v);
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j)
+              if (c0 + j < e.ncols) part[(c0 + j) * 2 * BM + a * BM] = v[j];
+          }
+        }
+        release();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0)
-        for (int b = b0; b <= b1; ++b) mbar_arrive(&tempty[b]);
     }
   }
   tc_fence_before();
