@@ -134,10 +134,11 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
                               int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* pos, cudaStream_t s);
 // bf16 rows [T][K] -> hi/lo rows and scale atoms. pos == NULL: row t is row t
 // of g (zero_out, optional: rows of y outside every segment are cleared);
-// else token t goes to the rows pos names (and to row t of group 0 with shared).
+// else token t goes to the rows pos names for its ids idx (and to row t of group
+// 0 with shared).
 // Chained to the kernel that made the tables, if g has any.
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
-                         const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
+                         const int64_t* idx, const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
                          __nv_bfloat16* zero_out, int M, cudaStream_t s);
 // launch_route_plan and launch_split in one kernel, for a few tokens: tile 32,
 // at most kRouteTokens tokens and 256 pairs.

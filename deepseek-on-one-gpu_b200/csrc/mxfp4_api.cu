@@ -266,7 +266,7 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
   a.y = static_cast<__nv_bfloat16*>(out);
   a.status = device_status;
   MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, tokens, in_features, a.g, L.tile, nullptr,
-                           0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
+                           nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
   return run_gemm(false, false, codes, codes, 1, at<uint8_t>(workspace, L.xq), a, L.tile,
                   static_cast<long long>(L.units) * L.ksplit, s);
 }
@@ -344,8 +344,8 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
   MX_CUDA(mx::launch_segments(offsets, n_experts, rows, L.tile, at<int32_t>(workspace, L.counts),
                               at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), device_status,
                               s));
-  MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, rows, in_features, a.g, L.tile, nullptr, 0,
-                           0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf),
+  MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, rows, in_features, a.g, L.tile, nullptr,
+                           nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf),
                            clear_rest ? a.y : nullptr, out_features, s));
   return run_gemm(false, false, codes, codes, n_experts, at<uint8_t>(workspace, L.xq), a, L.tile,
                   L.tiles * ceil_div(out_features, 256), s);
@@ -413,7 +413,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
                                    tile_start, pos, xq, sf, s));
   } else {
     MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, counts, row_start, tile_start, pos, s));
-    MX_CUDA(mx::launch_split(x, row_stride, tokens, H, a.g, L.tile, pos, top_k, shared, L.P, xq, sf, nullptr, 0, s));
+    MX_CUDA(mx::launch_split(x, row_stride, tokens, H, a.g, L.tile, topk_idx, pos, top_k, shared, L.P, xq, sf, nullptr, 0, s));
   }
   if ((r = run_gemm(false, true, w->gate_codes, w->up_codes, G, xq, a, L.tile,
                     L.tiles * (F / 128), s)))

@@ -223,51 +223,67 @@ __device__ __forceinline__ void split_row(const uint4& q, int K, int P, int n, c
 
 constexpr int MAXR = 9;  // rows of a token: the shared expert's and top_k <= 8
 
-// One block: 2048 columns of one row.
-template <int TILE>
+// One block: 2048 columns of R rows (tokens), their loads in flight together.
+// The place of a row is found by one thread each: for a routing the group is
+// known from idx, for segments it is searched (nine dependent loads: with one
+// row per block they took twice as long as the split itself, 322 us for 32768
+// rows of 7168 against 110 with eight).
+template <int TILE, int R>
 __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
-                                                    int K, const Groups g, const int32_t* pos, int top_k,
-                                                    int shared, int P, uint8_t* __restrict__ xq,
-                                                    uint8_t* __restrict__ sf, __nv_bfloat16* __restrict__ zero_out,
-                                                    int M) {
-  const int t = blockIdx.x;
+                                                    int K, const Groups g, const int64_t* __restrict__ idx,
+                                                    const int32_t* pos, int top_k, int shared, int P,
+                                                    uint8_t* __restrict__ xq, uint8_t* __restrict__ sf,
+                                                    __nv_bfloat16* __restrict__ zero_out, int M) {
+  const int t0 = blockIdx.x * R;
   const int tid = threadIdx.x;
   const int KB = K / 128;
   launch_dependents();
+  uint4 q[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) q[r] = t0 + r < T ? load_cols(x + (t0 + r) * row_stride, K) : make_uint4(0, 0, 0, 0);
   dependency_wait();
-  __shared__ int s_row[MAXR];
-  __shared__ SfSpot s_spot[MAXR];
+  __shared__ int s_row[R * MAXR];
+  __shared__ SfSpot s_spot[R * MAXR];
   const int n = pos ? top_k + shared : 1;
-  if (tid < n) {
-    int row, grp = 0, count, local, tile0 = 0;
-    if (pos) row = tid < shared ? t : load_dep(pos + static_cast<size_t>(t) * top_k + tid - shared);
-    else row = t;
-    if (row >= 0 && g.counts) {
-      int lo = 0, hi = g.n;  // last group that starts at or before the row
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (load_dep(g.row_start + mid) <= row) lo = mid; else hi = mid;
+  if (tid < R * n) {
+    const int r = tid / n, j = tid - r * n, t = t0 + r;
+    int row = -1, grp = 0, count = g.rows, local = t, tile0 = 0;
+    if (t < T) {
+      row = t;
+      if (pos && j >= shared) {
+        const size_t pair = static_cast<size_t>(t) * top_k + j - shared;
+        row = load_dep(pos + pair);
+        if (row >= 0) grp = static_cast<int>(__ldg(idx + pair)) + shared;  // row < 0: an id outside
+      } else if (g.counts && !pos) {
+        int lo = 0, hi = g.n;  // last group that starts at or before the row
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (load_dep(g.row_start + mid) <= row) lo = mid; else hi = mid;
+        }
+        grp = lo;
       }
-      grp = lo;
-      count = load_dep(g.counts + grp);
-      local = row - load_dep(g.row_start + grp);
-      tile0 = load_dep(g.tile_start + grp);
-      if (local < 0 || local >= count) row = -1;
-    } else {
-      count = g.rows;
-      local = row;
+      if (g.counts && row >= 0) {
+        count = load_dep(g.counts + grp);
+        local = row - load_dep(g.row_start + grp);
+        tile0 = load_dep(g.tile_start + grp);
+        if (local < 0 || local >= count) row = -1;  // a row outside every segment
+      }
     }
     s_row[tid] = row;
     if (row >= 0) s_spot[tid] = sf_spot<TILE>(tile0, count, local, KB);
   }
   __syncthreads();
-  if (!pos && s_row[0] < 0) {  // a row outside every segment
-    if (zero_out && blockIdx.y == 0)
-      for (int c = tid; c < M / 8; c += 256)
-        reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t) * M)[c] = make_uint4(0, 0, 0, 0);
-    return;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (t0 + r >= T) break;
+    if (!pos && s_row[r] < 0) {
+      if (zero_out && blockIdx.y == 0)
+        for (int c = tid; c < M / 8; c += 256)
+          reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t0 + r) * M)[c] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    split_row(q[r], K, P, n, s_row + r * n, s_spot + r * n, tile_atoms(TILE), xq, sf);
   }
-  split_row(load_cols(x + t * row_stride, K), K, P, n, s_row, s_spot, tile_atoms(TILE), xq, sf);
 }
 
 // Plan and split for a few tokens. Every block builds the group tables for
@@ -407,17 +423,19 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 }
 
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
-                         const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
+                         const int64_t* idx, const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
                          __nv_bfloat16* zero_out, int M, cudaStream_t s) {
-  const dim3 grid(T, (K + 2047) / 2048);
-  auto go = [&](auto kern) {
-    return launch_chained(g.counts != nullptr, kern, grid, 256, 0, s, x, row_stride, T, K, g, pos, top_k, shared, P, xq,
-                          sf, zero_out, M);
+  constexpr int R = 8;
+  const bool many = T >= 1024;  // fewer rows: one per block, to reach every SM
+  const dim3 grid(many ? (T + R - 1) / R : T, (K + 2047) / 2048);
+  auto go = [&](auto one, auto several) {
+    return launch_chained(g.counts != nullptr, many ? several : one, grid, 256, 0, s, x, row_stride, T, K, g, idx, pos,
+                          top_k, shared, P, xq, sf, zero_out, M);
   };
   switch (tile) {
-    case 32: return go(split_kernel<32>);
-    case 64: return go(split_kernel<64>);
-    case 160: return go(split_kernel<160>);
+    case 32: return go(split_kernel<32, 1>, split_kernel<32, R>);
+    case 64: return go(split_kernel<64, 1>, split_kernel<64, R>);
+    case 160: return go(split_kernel<160, 1>, split_kernel<160, R>);
     default: return cudaErrorInvalidValue;
   }
 }
