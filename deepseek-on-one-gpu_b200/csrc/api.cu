@@ -76,7 +76,8 @@ EncodeTiledFn encode_fn() {
 // 2-D row-major map: `rows` x `cols` elements in rows of `row_bytes` bytes, box
 // `box_rows` x `box_cols`.
 int make_map_strided(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
-                     uint64_t rows, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw) {
+                     uint64_t rows, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle sw,
+                     CUtensorMapL2promotion promote = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(DSMOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {cols, rows};
@@ -84,7 +85,7 @@ int make_map_strided(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes,
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  promote, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(DSMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): rows=%llu cols=%llu box=%ux%u", int(r),
                 (unsigned long long)rows, (unsigned long long)cols, box_rows, box_cols);
@@ -383,7 +384,8 @@ int set_last_error(int code, const char* msg) { return fail(code, "%s", msg); }
 
 int make_tma_map(CUtensorMap* m, CUtensorMapDataType dt, uint64_t row_bytes, const void* base, uint64_t cols,
                  uint64_t rows, uint32_t box_cols, uint32_t box_rows) {
-  return make_map_strided(m, dt, row_bytes, base, cols, rows, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  return make_map_strided(m, dt, row_bytes, base, cols, rows, box_cols, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }
 size_t route_scratch_bytes(const dsmoe_moe_config_t* c, int T) {
   if (check_cfg(c) != DSMOE_OK) return 0;

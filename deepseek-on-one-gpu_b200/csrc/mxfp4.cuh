@@ -66,6 +66,7 @@ struct GemmArgs {
   const uint8_t* sfa1;   // up projection (SwiGLU), else == sfa0
   const uint8_t* sfb;    // scale atoms of the rows [tile][K/128][tile_atoms][512]
   __nv_bfloat16* y;      // [row][M]
+  int32_t* next;         // counter of handed-out units, 0 before the launch; NULL: units in fixed turns
   uint8_t* hq;           // SwiGLU: split rows [2][P][M] and their atoms
   uint8_t* hsf;
   int* status;
@@ -126,12 +127,14 @@ cudaError_t launch_tile_scales(const uint8_t* scales, int mats, int N, int K, in
 
 // --------------------------------------------------------- mxfp4_prep.cu
 // Segments of rows sorted by expert from offsets[n + 1].
+// The kernels that make group tables also clear next[2].
 cudaError_t launch_segments(const int32_t* offsets, int n, int rows, int tile, int32_t* counts, int32_t* row_start,
-                            int32_t* tile_start, int* status, cudaStream_t s);
+                            int32_t* tile_start, int32_t* next, int* status, cudaStream_t s);
 // Segments from a routing: pos[T][top_k] is the row of each (token, k), in
 // token order inside an expert, -1 for an id outside [0, n_routed).
 cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed, int shared, int tile,
-                              int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* pos, cudaStream_t s);
+                              int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* next, int32_t* pos,
+                              cudaStream_t s);
 // bf16 rows [T][K] -> hi/lo rows and scale atoms. pos == NULL: row t is row t
 // of g (zero_out, optional: rows of y outside every segment are cleared);
 // else token t goes to the rows pos names for its ids idx (and to row t of group
@@ -145,7 +148,8 @@ cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, in
 constexpr int kRouteTokens = 32;
 cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
                                int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
-                               int32_t* tile_start, int32_t* pos, uint8_t* xq, uint8_t* sf, cudaStream_t s);
+                               int32_t* tile_start, int32_t* next, int32_t* pos, uint8_t* xq, uint8_t* sf,
+                               cudaStream_t s);
 // out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
                            int shared, float scale, __nv_bfloat16* out, cudaStream_t s);

@@ -48,7 +48,7 @@ int grouped_tile(long long rows, int groups) {
 }
 
 struct Plan {
-  size_t counts = 0, row_start = 0, tile_start = 0, pos = 0, xq = 0, sf = 0, hq = 0, hsf = 0, y = 0, total = 0;
+  size_t counts = 0, row_start = 0, tile_start = 0, next = 0, pos = 0, xq = 0, sf = 0, hq = 0, hsf = 0, y = 0, total = 0;
   int tile = 32, P = 0, ksplit = 1, units = 0;
   long long tiles = 0;
   size_t take(size_t bytes) {
@@ -60,6 +60,7 @@ struct Plan {
     counts = take(4 * static_cast<size_t>(groups));
     row_start = take(4 * static_cast<size_t>(groups));
     tile_start = take(4 * (static_cast<size_t>(groups) + 1));
+    next = take(8);
   }
   size_t atoms(int K) const { return static_cast<size_t>(tiles) * (K / 128) * mx::tile_atoms(tile) * 512; }
   void split_k(bool fp4, int N, int K) {
@@ -340,10 +341,11 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
   a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
+  a.next = at<int32_t>(workspace, L.next);
   a.status = device_status;
   MX_CUDA(mx::launch_segments(offsets, n_experts, rows, L.tile, at<int32_t>(workspace, L.counts),
-                              at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), device_status,
-                              s));
+                              at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), a.next,
+                              device_status, s));
   MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, rows, in_features, a.g, L.tile, nullptr,
                            nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf),
                            clear_rest ? a.y : nullptr, out_features, s));
@@ -403,6 +405,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.hq = at<uint8_t>(workspace, L.hq);
   a.hsf = at<uint8_t>(workspace, L.hsf);
+  a.next = at<int32_t>(workspace, L.next);
   a.status = device_status;
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(hidden);
   int32_t *counts = at<int32_t>(workspace, L.counts), *row_start = at<int32_t>(workspace, L.row_start),
@@ -410,9 +413,10 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
   if (tokens <= mx::kRouteTokens && L.tile == 32) {
     MX_CUDA(mx::launch_route_split(x, row_stride, tokens, H, topk_idx, top_k, E, shared, L.P, counts, row_start,
-                                   tile_start, pos, xq, sf, s));
+                                   tile_start, a.next, pos, xq, sf, s));
   } else {
-    MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, counts, row_start, tile_start, pos, s));
+    MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, counts, row_start, tile_start, a.next, pos,
+                                  s));
     MX_CUDA(mx::launch_split(x, row_stride, tokens, H, a.g, L.tile, topk_idx, pos, top_k, shared, L.P, xq, sf, nullptr, 0, s));
   }
   if ((r = run_gemm(false, true, w->gate_codes, w->up_codes, G, xq, a, L.tile,
@@ -422,6 +426,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   a.K = F;
   a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(w->down_atoms);
   a.sfb = at<uint8_t>(workspace, L.hsf);
+  ++a.next;
   a.y = at<__nv_bfloat16>(workspace, L.y);
   if ((r = run_gemm(false, false, w->down_codes, w->down_codes, G, at<uint8_t>(workspace, L.hq), a, L.tile,
                     L.tiles * ceil_div(H, 256), s)))

@@ -44,7 +44,7 @@ constexpr int CHUNK = 8;
 constexpr int THREADS = (EPI_WARP0 + kEpiWarps) * 32;
 
 struct Unit {
-  int32_t ncols;   // valid rows of the token tile
+  int32_t ncols;   // valid rows of the token tile; 0: no more units
   int32_t row0;    // first row
   int32_t tile;    // token tile index (scale atoms)
   int32_t group;
@@ -292,7 +292,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   // it has started on the weights.
   if (p.g.counts) dependency_wait();
   const uint32_t tmem = *s_tmem;
-  const int total = unit_count(p, BN, SWIGLU);
   const int KB = p.K / 128;
   const int MT = (p.M + BM - 1) / BM;
 
@@ -301,17 +300,25 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     // The search for a unit's group walks a shared-memory copy of the table:
     // nine dependent global loads would be ~3 us before the first copy.
     int* tiles = reinterpret_cast<int*>(smem + C::TAB_OFF);
+    const int total = unit_count(p, BN, SWIGLU);
     if (p.g.counts)
       for (int t = lane; t <= p.g.n; t += 32) tiles[t] = load_dep(p.g.tile_start + t);
     __syncwarp();
     if (lane == 0) {
-      int i = 0;
-      for (int u = blockIdx.x; u < total; u += gridDim.x, ++i) {
-        const Unit e = decode<C, SWIGLU>(u, p, tiles);
+      int u = blockIdx.x;
+      for (int i = 0;; ++i) {
+        Unit e;
+        e.ncols = 0;  // the end
+        if (u < total) e = decode<C, SWIGLU>(u, p, tiles);
         const int ri = i % RING;
         if (!mbar_wait(&uempty[ri], ((i / RING) & 1) ^ 1, p.status, kDevTimeoutProducer, s_abort)) break;
         plan[ri] = e;
         mbar_arrive(&ufull[ri]);
+        if (u >= total) break;
+        // Units of ragged groups cost between 64 and 160 columns: handed out
+        // as CTAs become free. (In fixed turns the slowest of 148 CTAs got
+        // ~20% more than the mean.)
+        u = p.next ? static_cast<int>(gridDim.x) + atomicAdd(p.next, 1) : u + static_cast<int>(gridDim.x);
       }
     }
   } else if (warp == 0) {
@@ -319,16 +326,17 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     if (elect_one()) {
       // Rows are read by every feature tile: kept. Weights: where experts have
       // few rows a weight tile is read once or twice and makes room first;
-      // with large token tiles the 256-byte lines its 64-byte reads promote
-      // must outlive four K blocks of other CTAs' rows (evict-first: 1.5-4% slower).
+      // with large token tiles the lines its 64-byte reads promote must outlive
+      // the other CTAs' rows (evict-first: 1.5-4% slower).
       const uint64_t pol_w = BN > 64 ? policy_evict_normal() : policy_evict_first(), pol_x = policy_evict_last();
       int stage = 0, issued = 0, i = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+      for (; ok; ++i) {
         const int ri = i % RING;
         if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutProducer, s_abort)) break;
         const Unit e = plan[ri];
+        if (e.ncols == 0) break;
         mbar_arrive(&uempty[ri]);
         const int wrow = e.group * p.M;
         const bool two = e.m1 >= 0;
@@ -401,9 +409,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
       int stage = 0, nb = 0, i = 0;
       uint32_t phase = 0, tphase = 0;  // tphase: one bit per half
       bool ok = true;
-      for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+      for (; ok; ++i) {
         const int ri = i % RING;
         if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutMma, s_abort)) break;
+        if (plan[ri].ncols == 0) break;
         const int m1 = plan[ri].m1, n = plan[ri].n, both = plan[ri].both, kb0 = plan[ri].kb0, kb1 = plan[ri].kb1;
         mbar_arrive(&uempty[ri]);
         const int nn = both ? 2 * n : n;  // columns of one accumulator
@@ -471,10 +480,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     int nb = 0, i = 0;
     uint32_t tphase = 0;  // one bit per half
     bool ok = true;
-    for (int u = blockIdx.x; u < total && ok; u += gridDim.x, ++i) {
+    for (; ok; ++i) {
       const int ri = i % RING;
       if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutEpilogue, s_abort)) break;
       const Unit e = plan[ri];
+      if (e.ncols == 0) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&uempty[ri]);
       const int nn = e.both ? 2 * e.n : e.n;

@@ -33,10 +33,11 @@ __global__ void __launch_bounds__(kMaxGroups) segments_kernel(const int32_t* __r
                                                               int tile, int32_t* __restrict__ counts,
                                                               int32_t* __restrict__ row_start,
                                                               int32_t* __restrict__ tile_start,
-                                                              int* __restrict__ status) {
+                                                              int32_t* __restrict__ next, int* __restrict__ status) {
   __shared__ int buf[kMaxGroups];
   launch_dependents();
   const int i = threadIdx.x;
+  if (i < 2) next[i] = 0;
   const int lo = i < n ? offsets[i] : 0, hi = i < n ? offsets[i + 1] : 0;
   if (i < n && (lo < 0 || hi < lo || hi > rows)) atomicCAS(status, 0, kDevBadCount);
   const int first = min(max(offsets[0], 0), rows);
@@ -57,29 +58,45 @@ __global__ void __launch_bounds__(kMaxGroups) segments_kernel(const int32_t* __r
   }
 }
 
-// Stable counting sort of the (token, k) pairs by expert, by one block: warp w
-// owns a contiguous range of pairs, counts it, and after the scans walks it
-// again in order; lanes of one step that hold the same expert are ranked by
-// lane. The row of a pair therefore depends on the routing only.
+// Stable counting sort of the (token, k) pairs by expert, by one cluster of
+// CTAs: each warp owns a contiguous range of pairs, counts it, and after the
+// scans over warps, CTAs (through shared memory) and groups walks it again in
+// order; lanes of one step that hold the same expert are ranked by lane. The
+// row of a pair therefore depends on the routing only. One CTA took 63 us for
+// 32768 pairs.
 constexpr int kPlanWarps = 32;
+constexpr int kPlanCtas = 8;
+
+__device__ __forceinline__ int load_peer(const int* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 __global__ void __launch_bounds__(1024) route_plan_kernel(const int64_t* __restrict__ idx, int T, int top_k,
                                                           int n_routed, int shared, int tile,
                                                           int32_t* __restrict__ counts, int32_t* __restrict__ row_start,
-                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ pos) {
+                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ next,
+                                                          int32_t* __restrict__ pos) {
   extern __shared__ int hist[];  // [kPlanWarps][n_routed]
-  __shared__ int buf[kMaxGroups];
+  __shared__ int s_total[kMaxGroups];  // this CTA's pairs per expert
+  __shared__ int s_sum[2][kMaxGroups / 32];
   launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = gridDim.x, me = blockIdx.x;  // the grid is one cluster
   const int pairs = T * top_k;
-  const int per = ((pairs + kPlanWarps - 1) / kPlanWarps + 31) & ~31;
-  const int p0 = min(pairs, warp * per), p1 = min(pairs, p0 + per);
+  const int per = ((pairs + kPlanWarps * ctas - 1) / (kPlanWarps * ctas) + 31) & ~31;
+  const int p0 = min(pairs, (me * kPlanWarps + warp) * per), p1 = min(pairs, p0 + per);
   for (int i = threadIdx.x; i < kPlanWarps * n_routed; i += 1024) hist[i] = 0;
   __syncthreads();
   int* mine = hist + warp * n_routed;
   // expert of pair p, -1 past the warp's pairs or for an id outside; batches of
-  // 8 x 32 pairs are loaded together (one dependent load per 32 pairs was 2/3
-  // of this kernel's time)
+  // 8 x 32 pairs are loaded together
   constexpr int B = 8;
   auto expert = [&](int p) {
     if (p >= p1) return -1;
@@ -95,47 +112,57 @@ __global__ void __launch_bounds__(1024) route_plan_kernel(const int64_t* __restr
       if (e[j] >= 0) atomicAdd(&mine[e[j]], 1);
   }
   __syncthreads();
-  // group totals and, per warp, the rows of earlier warps
-  const int groups = n_routed + shared;
-  const int g = threadIdx.x;
-  int c = 0;
-  if (g < groups) {
-    if (g < shared) {
-      c = T;
-    } else {
-      for (int w = 0; w < kPlanWarps; ++w) {
-        int* h = &hist[w * n_routed + g - shared];
-        const int n = *h;
-        *h = c;
+  // per expert: the pairs of earlier warps, then of earlier CTAs
+  const int g = threadIdx.x;  // group
+  const int ex = g - shared;  // its expert
+  const bool routed = ex >= 0 && ex < n_routed;
+  int own = 0;
+  if (routed) {
+    for (int w = 0; w < kPlanWarps; ++w) {
+      int* h = &hist[w * n_routed + ex];
+      const int n = *h;
+      *h = own;
+      own += n;
+    }
+    s_total[ex] = own;
+  }
+  int c = g < shared ? T : own, before = 0;
+  if (ctas > 1) {
+    cluster_sync();
+    if (routed) {
+      c = 0;
+      for (int r = 0; r < ctas; ++r) {
+        const int n = r == me ? own : load_peer(&s_total[ex], r);
+        if (r < me) before += n;
         c += n;
       }
     }
+    cluster_sync();  // no CTA leaves, or reuses s_total, while it is read
   }
-  // Scans over the first kMaxGroups threads; the others keep the barriers.
+  // scans of rows and token tiles over the groups (the first kMaxGroups threads)
   const int nt = (c + tile - 1) / tile;
   int rows = c, tiles = nt;
-  for (int pass = 0; pass < 2; ++pass) {
-    int& v = pass ? tiles : rows;
-    if (g < kMaxGroups) buf[g] = v;
-    __syncthreads();
-    for (int o = 1; o < kMaxGroups; o <<= 1) {
-      const int a = g < kMaxGroups && g >= o ? buf[g - o] : 0;
-      __syncthreads();
-      if (g < kMaxGroups) buf[g] += a;
-      __syncthreads();
-    }
-    if (g < kMaxGroups) v = buf[g];
-    __syncthreads();
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, rows, o), b = __shfl_up_sync(0xffffffffu, tiles, o);
+    if (lane >= o) rows += a, tiles += b;
   }
+  if (lane == 31 && warp < kMaxGroups / 32) s_sum[0][warp] = rows, s_sum[1][warp] = tiles;
+  __syncthreads();
+  for (int w = 0; w < min(warp, kMaxGroups / 32); ++w) rows += s_sum[0][w], tiles += s_sum[1][w];
+  const int groups = n_routed + shared;
   if (g < groups) {
     const int start = rows - c;
-    counts[g] = c;
-    row_start[g] = start;
-    tile_start[g] = tiles - nt;
-    if (g == groups - 1) tile_start[groups] = tiles;
-    if (g >= shared)
-      for (int w = 0; w < kPlanWarps; ++w) hist[w * n_routed + g - shared] += start;
+    if (me == 0) {
+      counts[g] = c;
+      row_start[g] = start;
+      tile_start[g] = tiles - nt;
+      if (g == groups - 1) tile_start[groups] = tiles;
+    }
+    if (routed)
+      for (int w = 0; w < kPlanWarps; ++w) hist[w * n_routed + ex] += start + before;
   }
+  if (me == 0 && threadIdx.x < 2) next[threadIdx.x] = 0;
   __syncthreads();
   for (int p = p0; p < p1; p += 32 * B) {  // warp-uniform
     int e[B];
@@ -225,9 +252,9 @@ constexpr int MAXR = 9;  // rows of a token: the shared expert's and top_k <= 8
 
 // One block: 2048 columns of R rows (tokens), their loads in flight together.
 // The place of a row is found by one thread each: for a routing the group is
-// known from idx, for segments it is searched (nine dependent loads: with one
-// row per block they took twice as long as the split itself, 322 us for 32768
-// rows of 7168 against 110 with eight).
+// known from idx, for segments it is searched in a shared-memory copy of their
+// starts (nine dependent global loads took twice as long as the split itself:
+// 322 us for 32768 rows of 7168).
 template <int TILE, int R>
 __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
                                                     int K, const Groups g, const int64_t* __restrict__ idx,
@@ -244,6 +271,11 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
   dependency_wait();
   __shared__ int s_row[R * MAXR];
   __shared__ SfSpot s_spot[R * MAXR];
+  __shared__ int s_start[kMaxGroups];
+  if (!pos && g.counts) {
+    for (int i = tid; i < g.n; i += 256) s_start[i] = load_dep(g.row_start + i);
+    __syncthreads();
+  }
   const int n = pos ? top_k + shared : 1;
   if (tid < R * n) {
     const int r = tid / n, j = tid - r * n, t = t0 + r;
@@ -258,7 +290,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
         int lo = 0, hi = g.n;  // last group that starts at or before the row
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
-          if (load_dep(g.row_start + mid) <= row) lo = mid; else hi = mid;
+          if (s_start[mid] <= row) lo = mid; else hi = mid;
         }
         grp = lo;
       }
@@ -294,8 +326,9 @@ __global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* _
                                                           int T, int K, const int64_t* __restrict__ idx, int top_k,
                                                           int n_routed, int shared, int P,
                                                           int32_t* __restrict__ counts, int32_t* __restrict__ row_start,
-                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ pos,
-                                                          uint8_t* __restrict__ xq, uint8_t* __restrict__ sf) {
+                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ next,
+                                                          int32_t* __restrict__ pos, uint8_t* __restrict__ xq,
+                                                          uint8_t* __restrict__ sf) {
   constexpr int TILE = 32;
   static_assert(kRouteTokens <= TILE, "one tile per group");
   __shared__ int s_e[256], s_cnt[kMaxGroups], s_start[kMaxGroups], s_tile[kMaxGroups];
@@ -333,11 +366,13 @@ __global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* _
   s_tile[2 * tid + 1] = tiles - (c1 > 0);
   s_tile[2 * tid] = tiles - (c1 > 0) - (c0 > 0);
   __syncthreads();
-  if (blockIdx.x == 0 && blockIdx.y == 0)
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    if (tid < 2) next[tid] = 0;
     for (int g = tid; g <= G; g += 256) {
       if (g < G) counts[g] = s_cnt[g], row_start[g] = s_start[g], tile_start[g] = s_tile[g];
       else tile_start[g] = s_tile[G - 1] + (s_cnt[G - 1] > 0);
     }
+  }
   // Warp w places pair w of the token: earlier pairs of the same expert first.
   const int n = top_k + shared;
   if (warp < top_k) {
@@ -406,20 +441,34 @@ __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, in
 }  // namespace
 
 cudaError_t launch_segments(const int32_t* offsets, int n, int rows, int tile, int32_t* counts, int32_t* row_start,
-                            int32_t* tile_start, int* status, cudaStream_t s) {
-  segments_kernel<<<1, kMaxGroups, 0, s>>>(offsets, n, rows, tile, counts, row_start, tile_start, status);
+                            int32_t* tile_start, int32_t* next, int* status, cudaStream_t s) {
+  segments_kernel<<<1, kMaxGroups, 0, s>>>(offsets, n, rows, tile, counts, row_start, tile_start, next, status);
   return cudaGetLastError();
 }
 
 cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed, int shared, int tile,
-                              int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* pos, cudaStream_t s) {
+                              int32_t* counts, int32_t* row_start, int32_t* tile_start, int32_t* next, int32_t* pos,
+                              cudaStream_t s) {
   const int smem = kPlanWarps * n_routed * 4;
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // static shared memory counts against the default limit too
     const cudaError_t e = cudaFuncSetAttribute(route_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  route_plan_kernel<<<1, 1024, smem, s>>>(idx, T, top_k, n_routed, shared, tile, counts, row_start, tile_start, pos);
-  return cudaGetLastError();
+  // A CTA's warps take 32 pairs a step: a few steps each before more CTAs help.
+  const int ctas = T * top_k >= 4096 ? kPlanCtas : 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = ctas;
+  cfg.blockDim = 1024;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, route_plan_kernel, idx, T, top_k, n_routed, shared, tile, counts, row_start, tile_start,
+                            next, pos);
 }
 
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
@@ -442,10 +491,11 @@ cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, in
 
 cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
                                int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
-                               int32_t* tile_start, int32_t* pos, uint8_t* xq, uint8_t* sf, cudaStream_t s) {
+                               int32_t* tile_start, int32_t* next, int32_t* pos, uint8_t* xq, uint8_t* sf,
+                               cudaStream_t s) {
   if (T > kRouteTokens || T * top_k > 256 || n_routed + shared > kMaxGroups) return cudaErrorInvalidValue;
   route_split_kernel<<<dim3(T, (K + 2047) / 2048), 256, 0, s>>>(x, row_stride, T, K, idx, top_k, n_routed, shared, P,
-                                                                 counts, row_start, tile_start, pos, xq, sf);
+                                                                 counts, row_start, tile_start, next, pos, xq, sf);
   return cudaGetLastError();
 }
 
