@@ -20,6 +20,7 @@
 
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -71,6 +72,29 @@ struct GemmArgs {
   uint8_t* hsf;
   int* status;
 };
+
+// Four scaled numbers -> their hi and lo e4m3 terms, the first in the lowest
+// byte. Conversions work on pairs: one number at a time, they made the split
+// of activations issue-bound at 28 instructions per number.
+__device__ __forceinline__ void split4(const float* q, uint32_t& hi, uint32_t& lo) {
+  uint32_t f0, f1;  // the hi terms back as f16 pairs (exact)
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 a, %4, %3;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 b, %6, %5;\n\t"
+      "mov.b32 %0, {a, b};\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %2, b;\n\t}"
+      : "=r"(hi), "=r"(f0), "=r"(f1)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f0));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f1));
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+      "mov.b32 %0, {a, b};\n\t}"
+      : "=r"(lo)
+      : "f"(q[0] - a.x), "f"(q[1] - a.y), "f"(q[2] - b.x), "f"(q[3] - b.y));
+}
 
 // The kernels of one call are chained by programmatic dependent launches: the
 // first one is launched normally, so everything enqueued before the call is

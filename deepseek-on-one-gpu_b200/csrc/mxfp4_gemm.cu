@@ -543,7 +543,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         for (int j = 0; j < C::CHUNKS * CHUNK; j += 4) {
           const int c0 = column(j / CHUNK) + j % CHUNK;
           if (c0 < e.ncols) {
-            uint32_t hi4 = 0, lo4 = 0, bytes = 0;
+            uint32_t hi4, lo4, bytes = 0;
             float q[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -552,13 +552,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
               q[t] = h[j + t] * (ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23));
               bytes |= byte << (8 * t);
             }
-#pragma unroll
-            for (int t = 0; t < 4; t += 2) {
-              const uint32_t h2 = f32x2_to_e4m3x2(q[t], q[t + 1]);
-              const uint32_t l2 = f32x2_to_e4m3x2(q[t] - e4m3_to_f32(h2 & 0xff), q[t + 1] - e4m3_to_f32(h2 >> 8));
-              hi4 |= h2 << (8 * t);
-              lo4 |= l2 << (8 * t);
-            }
+            split4(q, hi4, lo4);
             hi4 = transpose4(hi4, lane);
             lo4 = transpose4(lo4, lane);
             const int col = c0 + (lane & 3);

@@ -211,39 +211,43 @@ __device__ __forceinline__ void split_row(const uint4& q, int K, int P, int n, c
   const int col = blockIdx.y * 2048 + tid * 8;
   const bool in = col < K;  // K is a multiple of 128: 16 threads of a K block are in or out together
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  uint32_t amax = 0;  // |bf16| bit patterns order like the numbers
+  // |bf16| bit patterns order like the numbers; two at a time
+  uint32_t m2 = w[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  for (int i = 1; i < 4; ++i) m2 = __vmaxu2(m2, w[i] & 0x7fff7fffu);
+  m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+  m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 2));
+  const uint32_t amax = max(m2 & 0xffffu, m2 >> 16);
   const uint32_t ef = amax >> 7;
   const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
   const float inv = ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23);
-  uint32_t hw[2] = {0, 0}, lw[2] = {0, 0};
+  float v[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float a = __uint_as_float(w[i] << 16) * inv, b = __uint_as_float(w[i] & 0xffff0000u) * inv;
-    const uint32_t h2 = f32x2_to_e4m3x2(a, b);
-    const uint32_t l2 = f32x2_to_e4m3x2(a - e4m3_to_f32(h2 & 0xff), b - e4m3_to_f32(h2 >> 8));
-    hw[i >> 1] |= h2 << (16 * (i & 1));
-    lw[i >> 1] |= l2 << (16 * (i & 1));
+    v[2 * i] = __uint_as_float(w[i] << 16) * inv;
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * inv;
   }
+  uint32_t hw[2], lw[2];
+  split4(v, hw[0], lw[0]);
+  split4(v + 4, hw[1], lw[1]);
   // scale word of the K block: bytes from threads 0, 4, 8, 12 of its 16
   uint32_t word = byte << (8 * ((tid >> 2) & 3));
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
   word |= __shfl_xor_sync(0xffffffffu, word, 8);
   if (!in) return;
   const long long step = static_cast<long long>(col >> 7) * atoms * 128;
+  const size_t lo_rows = static_cast<size_t>(P) * K;
   for (int r = 0; r < n; ++r) {
     const int row = s_row[r];
     if (row < 0) continue;
-    const size_t off = static_cast<size_t>(row) * K + col;
-    *reinterpret_cast<uint2*>(xq + off) = make_uint2(hw[0], hw[1]);
-    *reinterpret_cast<uint2*>(xq + static_cast<size_t>(P) * K + off) = make_uint2(lw[0], lw[1]);
+    uint8_t* dst = xq + static_cast<size_t>(row) * K + col;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(hw[0], hw[1]);
+    *reinterpret_cast<uint2*>(dst + lo_rows) = make_uint2(lw[0], lw[1]);
     if ((tid & 15) == 0) {
-      uint32_t* s32 = reinterpret_cast<uint32_t*>(sf);
-      s32[s_spot[r].hi + step] = word;
-      if (s_spot[r].lo >= 0) s32[s_spot[r].lo + step] = word;
+      uint32_t* s32 = reinterpret_cast<uint32_t*>(sf) + step;
+      const SfSpot at = s_spot[r];
+      s32[at.hi] = word;
+      if (at.lo >= 0) s32[at.lo] = word;
     }
   }
 }
