@@ -73,27 +73,29 @@ struct GemmArgs {
   int* status;
 };
 
-// Four scaled numbers -> their hi and lo e4m3 terms, the first in the lowest
-// byte. Conversions work on pairs: one number at a time, they made the split
-// of activations issue-bound at 28 instructions per number.
-__device__ __forceinline__ void split4(const float* q, uint32_t& hi, uint32_t& lo) {
-  uint32_t f0, f1;  // the hi terms back as f16 pairs (exact)
-  asm("{\n\t.reg .b16 a, b;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f32 a, %4, %3;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f32 b, %6, %5;\n\t"
+// Four scaled numbers (f16 pairs) -> their hi and lo e4m3 terms, the first in
+// the lowest byte. f16 holds what the two terms can (8 significant bits down
+// to 2^-9, |x| <= 256), and its pairs take half the instructions of fp32: one
+// number at a time, the split of activations was issue-bound at 28
+// instructions per number.
+__device__ __forceinline__ void split4(uint32_t x01, uint32_t x23, uint32_t& hi, uint32_t& lo) {
+  asm("{\n\t.reg .b16 a, b;\n\t.reg .b32 f, g;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 a, %2;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 b, %3;\n\t"
       "mov.b32 %0, {a, b};\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, a;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %2, b;\n\t}"
-      : "=r"(hi), "=r"(f0), "=r"(f1)
-      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]));
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f0));
-  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f1));
-  asm("{\n\t.reg .b16 a, b;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
-      "mov.b32 %0, {a, b};\n\t}"
-      : "=r"(lo)
-      : "f"(q[0] - a.x), "f"(q[1] - a.y), "f"(q[2] - b.x), "f"(q[3] - b.y));
+      "cvt.rn.f16x2.e4m3x2 f, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 g, b;\n\t"
+      "sub.rn.f16x2 f, %2, f;\n\t"
+      "sub.rn.f16x2 g, %3, g;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 a, f;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 b, g;\n\t"
+      "mov.b32 %1, {a, b};\n\t}"
+      : "=&r"(hi), "=r"(lo)
+      : "r"(x01), "r"(x23));
+}
+__device__ __forceinline__ uint32_t f16_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // The kernels of one call are chained by programmatic dependent launches: the

@@ -552,7 +552,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
               q[t] = h[j + t] * (ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23));
               bytes |= byte << (8 * t);
             }
-            split4(q, hi4, lo4);
+            // f16's 11 bits on the way to the two terms' 8 or 9
+            split4(f16_pair(q[0], q[1]), f16_pair(q[2], q[3]), hi4, lo4);
             hi4 = transpose4(hi4, lane);
             lo4 = transpose4(lo4, lane);
             const int col = c0 + (lane & 3);

@@ -196,55 +196,67 @@ __device__ __forceinline__ SfSpot sf_spot(int tile0, int count, int local, int K
   return {base + word(c), n32 ? base + word(c + n32) : -1};
 }
 
-// This thread's 8 columns of a row (zero past its end): block y of the grid
-// has columns 2048 y and up.
-__device__ __forceinline__ uint4 load_cols(const __nv_bfloat16* row, int K) {
-  const int col = blockIdx.y * 2048 + threadIdx.x * 8;
-  return col < K ? __ldg(reinterpret_cast<const uint4*>(row + col)) : make_uint4(0, 0, 0, 0);
+// Split kernels: blocks of kSplitThreads, 16 columns of a row per thread.
+constexpr int kSplitThreads = 128;
+constexpr int kSplitCols = kSplitThreads * 16;
+
+struct Cols {
+  uint4 a, b;
+};
+
+// This thread's 16 columns of a row (zero past its end): block y of the grid
+// has columns kSplitCols * y and up.
+__device__ __forceinline__ Cols load_cols(const __nv_bfloat16* row, int K) {
+  const int col = blockIdx.y * kSplitCols + threadIdx.x * 16;
+  Cols c{};
+  if (col < K) {
+    const uint4* p = reinterpret_cast<const uint4*>(row + col);
+    c.a = __ldg(p);
+    c.b = __ldg(p + 1);
+  }
+  return c;
 }
 
-// Splits the row and stores it, with its scale words, at n rows. 4 threads
-// share a 32-number block, 16 a K block's scale word.
-__device__ __forceinline__ void split_row(const uint4& q, int K, int P, int n, const int* s_row, const SfSpot* s_spot,
+// Splits the row and stores it, with its scale words, at n rows. 2 threads
+// share a 32-number block, 8 a K block's scale word.
+__device__ __forceinline__ void split_row(const Cols& q, int K, int P, int n, const int* s_row, const SfSpot* s_spot,
                                           int atoms, uint8_t* __restrict__ xq, uint8_t* __restrict__ sf) {
   const int tid = threadIdx.x;
-  const int col = blockIdx.y * 2048 + tid * 8;
-  const bool in = col < K;  // K is a multiple of 128: 16 threads of a K block are in or out together
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  const int col = blockIdx.y * kSplitCols + tid * 16;
+  const bool in = col < K;  // K is a multiple of 128: 8 threads of a K block are in or out together
+  const uint32_t w[8] = {q.a.x, q.a.y, q.a.z, q.a.w, q.b.x, q.b.y, q.b.z, q.b.w};
   // |bf16| bit patterns order like the numbers; two at a time
   uint32_t m2 = w[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int i = 1; i < 4; ++i) m2 = __vmaxu2(m2, w[i] & 0x7fff7fffu);
+  for (int i = 1; i < 8; ++i) m2 = __vmaxu2(m2, w[i] & 0x7fff7fffu);
   m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
-  m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 2));
   const uint32_t amax = max(m2 & 0xffffu, m2 >> 16);
   const uint32_t ef = amax >> 7;
   const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
-  const float inv = ef == 255 ? 0.f : __uint_as_float((254u - byte) << 23);
-  float v[8];
+  // 2^(127 - byte); the product is exact (or below all that the terms hold)
+  const __nv_bfloat162 inv = __bfloat162bfloat162(__ushort_as_bfloat16(ef == 255 ? 0 : (254u - byte) << 7));
+  uint32_t x[8], hw[4], lw[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16) * inv;
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * inv;
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __bfloat1622float2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), inv));
+    x[i] = f16_pair(f.x, f.y);
   }
-  uint32_t hw[2], lw[2];
-  split4(v, hw[0], lw[0]);
-  split4(v + 4, hw[1], lw[1]);
-  // scale word of the K block: bytes from threads 0, 4, 8, 12 of its 16
-  uint32_t word = byte << (8 * ((tid >> 2) & 3));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split4(x[2 * i], x[2 * i + 1], hw[i], lw[i]);
+  // scale word of the K block: bytes from threads 0, 2, 4, 6 of its 8
+  uint32_t word = byte << (8 * ((tid >> 1) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
   word |= __shfl_xor_sync(0xffffffffu, word, 4);
-  word |= __shfl_xor_sync(0xffffffffu, word, 8);
   if (!in) return;
-  const long long step = static_cast<long long>(col >> 7) * atoms * 128;
+  uint32_t* s32 = reinterpret_cast<uint32_t*>(sf) + static_cast<long long>(col >> 7) * atoms * 128;
   const size_t lo_rows = static_cast<size_t>(P) * K;
   for (int r = 0; r < n; ++r) {
     const int row = s_row[r];
     if (row < 0) continue;
     uint8_t* dst = xq + static_cast<size_t>(row) * K + col;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(hw[0], hw[1]);
-    *reinterpret_cast<uint2*>(dst + lo_rows) = make_uint2(lw[0], lw[1]);
-    if ((tid & 15) == 0) {
-      uint32_t* s32 = reinterpret_cast<uint32_t*>(sf) + step;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+    *reinterpret_cast<uint4*>(dst + lo_rows) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+    if ((tid & 7) == 0) {
       const SfSpot at = s_spot[r];
       s32[at.hi] = word;
       if (at.lo >= 0) s32[at.lo] = word;
@@ -254,13 +266,13 @@ __device__ __forceinline__ void split_row(const uint4& q, int K, int P, int n, c
 
 constexpr int MAXR = 9;  // rows of a token: the shared expert's and top_k <= 8
 
-// One block: 2048 columns of R rows (tokens), their loads in flight together.
+// One block: kSplitCols columns of R rows (tokens), their loads in flight together.
 // The place of a row is found by one thread each: for a routing the group is
 // known from idx, for segments it is searched in a shared-memory copy of their
 // starts (nine dependent global loads took twice as long as the split itself:
 // 322 us for 32768 rows of 7168).
 template <int TILE, int R>
-__global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
+__global__ void __launch_bounds__(kSplitThreads) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
                                                     int K, const Groups g, const int64_t* __restrict__ idx,
                                                     const int32_t* pos, int top_k, int shared, int P,
                                                     uint8_t* __restrict__ xq, uint8_t* __restrict__ sf,
@@ -269,15 +281,15 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
   const int tid = threadIdx.x;
   const int KB = K / 128;
   launch_dependents();
-  uint4 q[R];
+  Cols q[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) q[r] = t0 + r < T ? load_cols(x + (t0 + r) * row_stride, K) : make_uint4(0, 0, 0, 0);
+  for (int r = 0; r < R; ++r) q[r] = t0 + r < T ? load_cols(x + (t0 + r) * row_stride, K) : Cols{};
   dependency_wait();
   __shared__ int s_row[R * MAXR];
   __shared__ SfSpot s_spot[R * MAXR];
   __shared__ int s_start[kMaxGroups];
   if (!pos && g.counts) {
-    for (int i = tid; i < g.n; i += 256) s_start[i] = load_dep(g.row_start + i);
+    for (int i = tid; i < g.n; i += kSplitThreads) s_start[i] = load_dep(g.row_start + i);
     __syncthreads();
   }
   const int n = pos ? top_k + shared : 1;
@@ -314,7 +326,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
     if (t0 + r >= T) break;
     if (!pos && s_row[r] < 0) {
       if (zero_out && blockIdx.y == 0)
-        for (int c = tid; c < M / 8; c += 256)
+        for (int c = tid; c < M / 8; c += kSplitThreads)
           reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t0 + r) * M)[c] = make_uint4(0, 0, 0, 0);
       continue;
     }
@@ -326,7 +338,7 @@ __global__ void __launch_bounds__(256) split_kernel(const __nv_bfloat16* __restr
 // itself (a 512-entry histogram and scan in shared memory, ~1 us) instead of
 // waiting for a kernel that does; block 0 also writes them out. A group has at
 // most 32 rows, one token tile.
-__global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride,
+__global__ void __launch_bounds__(kSplitThreads) route_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride,
                                                           int T, int K, const int64_t* __restrict__ idx, int top_k,
                                                           int n_routed, int shared, int P,
                                                           int32_t* __restrict__ counts, int32_t* __restrict__ row_start,
@@ -336,27 +348,36 @@ __global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* _
   constexpr int TILE = 32;
   static_assert(kRouteTokens <= TILE, "one tile per group");
   __shared__ int s_e[256], s_cnt[kMaxGroups], s_start[kMaxGroups], s_tile[kMaxGroups];
-  __shared__ int s_sum[2][8];
+  constexpr int NT = kSplitThreads, GT = kMaxGroups / NT;  // groups per thread
+  __shared__ int s_sum[2][NT / 32];
   __shared__ int s_row[MAXR];
   __shared__ SfSpot s_spot[MAXR];
   launch_dependents();
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pairs = T * top_k, G = n_routed + shared;
-  const uint4 q = load_cols(x + t * row_stride, K);
-  int e = -1;
-  if (tid < pairs) {
-    const int64_t v = __ldg(idx + tid);
-    if (v >= 0 && v < n_routed) e = static_cast<int>(v) + shared;
+  const Cols q = load_cols(x + t * row_stride, K);
+  for (int p = tid; p < 256; p += NT) {
+    int e = -1;
+    if (p < pairs) {
+      const int64_t v = __ldg(idx + p);
+      if (v >= 0 && v < n_routed) e = static_cast<int>(v) + shared;
+    }
+    s_e[p] = e;
   }
-  s_e[tid] = e;
-  s_cnt[tid] = s_cnt[tid + 256] = 0;
+  for (int g = tid; g < kMaxGroups; g += NT) s_cnt[g] = 0;
   __syncthreads();
-  if (e >= 0) atomicAdd(&s_cnt[e], 1);
+  for (int p = tid; p < pairs; p += NT)
+    if (s_e[p] >= 0) atomicAdd(&s_cnt[s_e[p]], 1);
   if (shared && tid == 0) s_cnt[0] = T;
   __syncthreads();
-  // Exclusive scans of rows and tiles; thread tid has groups 2 tid, 2 tid + 1.
-  const int c0 = s_cnt[2 * tid], c1 = s_cnt[2 * tid + 1];
-  int rows = c0 + c1, tiles = (c0 > 0) + (c1 > 0);
+  // Exclusive scans of rows and tiles; thread tid has groups GT * tid and up.
+  int c[GT], rows = 0, tiles = 0;
+#pragma unroll
+  for (int j = 0; j < GT; ++j) {
+    c[j] = s_cnt[GT * tid + j];
+    rows += c[j];
+    tiles += c[j] > 0;
+  }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, rows, o), b = __shfl_up_sync(0xffffffffu, tiles, o);
@@ -365,28 +386,31 @@ __global__ void __launch_bounds__(256) route_split_kernel(const __nv_bfloat16* _
   if (lane == 31) s_sum[0][warp] = rows, s_sum[1][warp] = tiles;
   __syncthreads();
   for (int w = 0; w < warp; ++w) rows += s_sum[0][w], tiles += s_sum[1][w];
-  s_start[2 * tid + 1] = rows - c1;
-  s_start[2 * tid] = rows - c1 - c0;
-  s_tile[2 * tid + 1] = tiles - (c1 > 0);
-  s_tile[2 * tid] = tiles - (c1 > 0) - (c0 > 0);
+#pragma unroll
+  for (int j = GT - 1; j >= 0; --j) {
+    rows -= c[j];
+    tiles -= c[j] > 0;
+    s_start[GT * tid + j] = rows;
+    s_tile[GT * tid + j] = tiles;
+  }
   __syncthreads();
   if (blockIdx.x == 0 && blockIdx.y == 0) {
     if (tid < 2) next[tid] = 0;
-    for (int g = tid; g <= G; g += 256) {
+    for (int g = tid; g <= G; g += NT) {
       if (g < G) counts[g] = s_cnt[g], row_start[g] = s_start[g], tile_start[g] = s_tile[g];
       else tile_start[g] = s_tile[G - 1] + (s_cnt[G - 1] > 0);
     }
   }
-  // Warp w places pair w of the token: earlier pairs of the same expert first.
+  // A warp places a pair of the token: earlier pairs of the same expert first.
   const int n = top_k + shared;
-  if (warp < top_k) {
-    const int p = t * top_k + warp, mine = s_e[p];
+  for (int k = warp; k < top_k; k += NT / 32) {
+    const int p = t * top_k + k, mine = s_e[p];
     int rank = 0;
     for (int b = 0; b < p; b += 32) rank += __popc(__ballot_sync(0xffffffffu, b + lane < p && s_e[b + lane] == mine));
     if (lane == 0) {
       const int row = mine >= 0 ? s_start[mine] + rank : -1;
-      s_row[shared + warp] = row;
-      if (mine >= 0) s_spot[shared + warp] = sf_spot<TILE>(s_tile[mine], s_cnt[mine], rank, K / 128);
+      s_row[shared + k] = row;
+      if (mine >= 0) s_spot[shared + k] = sf_spot<TILE>(s_tile[mine], s_cnt[mine], rank, K / 128);
       if (blockIdx.y == 0) pos[p] = row;
     }
   }
@@ -478,11 +502,11 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
                          const int64_t* idx, const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
                          __nv_bfloat16* zero_out, int M, cudaStream_t s) {
-  constexpr int R = 8;
+  constexpr int R = 4;
   const bool many = T >= 1024;  // fewer rows: one per block, to reach every SM
-  const dim3 grid(many ? (T + R - 1) / R : T, (K + 2047) / 2048);
+  const dim3 grid(many ? (T + R - 1) / R : T, (K + kSplitCols - 1) / kSplitCols);
   auto go = [&](auto one, auto several) {
-    return launch_chained(g.counts != nullptr, many ? several : one, grid, 256, 0, s, x, row_stride, T, K, g, idx, pos,
+    return launch_chained(g.counts != nullptr, many ? several : one, grid, kSplitThreads, 0, s, x, row_stride, T, K, g, idx, pos,
                           top_k, shared, P, xq, sf, zero_out, M);
   };
   switch (tile) {
@@ -498,7 +522,7 @@ cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int
                                int32_t* tile_start, int32_t* next, int32_t* pos, uint8_t* xq, uint8_t* sf,
                                cudaStream_t s) {
   if (T > kRouteTokens || T * top_k > 256 || n_routed + shared > kMaxGroups) return cudaErrorInvalidValue;
-  route_split_kernel<<<dim3(T, (K + 2047) / 2048), 256, 0, s>>>(x, row_stride, T, K, idx, top_k, n_routed, shared, P,
+  route_split_kernel<<<dim3(T, (K + kSplitCols - 1) / kSplitCols), kSplitThreads, 0, s>>>(x, row_stride, T, K, idx, top_k, n_routed, shared, P,
                                                                  counts, row_start, tile_start, next, pos, xq, sf);
   return cudaGetLastError();
 }
