@@ -184,6 +184,8 @@ cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* 
 // K split of a single-group product of `units` (feature tile pair, token tile)
 // pairs on the current device.
 int pick_ksplit(bool fp4, int tile, int units, int kblocks);
+// x: rows in boxes of the token tile (bf16 activations in tiles up to 64: of 8),
+// x32: of 32.
 cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
                         const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s);
 

@@ -162,7 +162,8 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
     m_w1 = m_w0;
     if (w1 != w0 && (r = make_tma_map(&m_w1, u4, a.K / 2, w1, a.K, wrows, 128, 128))) return r;
     const uint64_t rows = 2 * static_cast<uint64_t>(a.P);
-    if ((r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
+    // Tiles up to 64 rows never load as one box: their first map has 8-row boxes.
+    if ((r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile <= 64 ? 8 : tile))) return r;
     if ((r = make_tma_map(&m_x32, u8, a.K, x, a.K, rows, 128, 32))) return r;
   }
   // A split tile is a cluster, one unit per CTA; otherwise persistent CTAs.

@@ -343,7 +343,13 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         const uint8_t* fa0 = p.sfa0 + (static_cast<size_t>(e.group) * MT + e.m0 / BM) * KB * 512;
         const uint8_t* fa1 = p.sfa1 + (static_cast<size_t>(e.group) * MT + (two ? e.m1 : 0) / BM) * KB * 512;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
-        const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
+        // Rows side by side come in 32-row boxes; where a small tile has at most
+        // 16, in 8-row boxes (the columns behind them keep what an earlier stage
+        // left, and are not stored): 64 rows instead of 16 per stage took a
+        // tenth of a one-token FFN.
+        const bool few = BN <= 64 && e.ncols <= 16;
+        const int step = few ? 8 : 32, xrows = few ? (e.ncols + 7) & ~7 : e.n;
+        const uint32_t xbytes = e.both ? 2 * xrows * 128 : C::B_BYTES;
         auto load_w = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES;
           uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
@@ -360,9 +366,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);
           const int kx = FP4 ? kb * 64 : kb * 128;
           if (!FP4 && e.both) {
-            for (int s = 0; s < e.n; s += 32) {
-              tma_load_2d(st + s * 128, &tm_x32, &full[stage], kx, e.row0 + s, pol_x);
-              tma_load_2d(st + (e.n + s) * 128, &tm_x32, &full[stage], kx, p.P + e.row0 + s, pol_x);
+            const CUtensorMap* tm = few ? &tm_x : &tm_x32;
+            for (int s = 0; s < xrows; s += step) {
+              tma_load_2d(st + s * 128, tm, &full[stage], kx, e.row0 + s, pol_x);
+              tma_load_2d(st + (e.n + s) * 128, tm, &full[stage], kx, p.P + e.row0 + s, pol_x);
             }
           } else {
             tma_load_2d(st, &tm_x, &full[stage], kx, e.row0, pol_x);
