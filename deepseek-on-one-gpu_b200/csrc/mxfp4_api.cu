@@ -38,9 +38,26 @@ bool aligned(const void* p, size_t a) { return p && reinterpret_cast<uintptr_t>(
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Token tile of a product over `rows` rows of one group.
-int linear_tile(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 160; }
-int fp4_tile(int rows) { return rows <= 64 ? 64 : 160; }
+// Token tile of a single-group product: the smallest that holds all rows, up
+// to the largest; smaller again while the tiles, each split eight ways along
+// K, leave SMs idle.
+int single_tile(const int* sizes, int n, int rows, int N) {
+  int i = 0;
+  while (i + 1 < n && rows > sizes[i]) ++i;
+  const auto ctas = [&](int tile) {
+    return static_cast<long long>(ceil_div(rows, tile)) * ceil_div(N, 256) * mx::kMaxSplit;
+  };
+  while (i > 0 && ctas(sizes[i]) < sm_count()) --i;
+  return sizes[i];
+}
+int linear_tile(int rows, int N) {
+  static const int sizes[3] = {32, 64, 160};
+  return single_tile(sizes, 3, rows, N);
+}
+int fp4_tile(int rows, int N) {
+  static const int sizes[2] = {64, 160};
+  return single_tile(sizes, 2, rows, N);
+}
 // Token tile where `rows` rows spread over `groups` experts.
 int grouped_tile(long long rows, int groups) {
   const long long mean = (rows + groups - 1) / groups;
@@ -69,9 +86,9 @@ struct Plan {
   }
 };
 
-Plan plan_linear(int T, int K) {
+Plan plan_linear(int T, int K, int N) {
   Plan w;
-  w.tile = linear_tile(T);
+  w.tile = linear_tile(T, N);
   w.P = T;
   w.tiles = ceil_div(T, w.tile);
   w.xq = w.take(2 * static_cast<size_t>(T) * K);
@@ -79,9 +96,9 @@ Plan plan_linear(int T, int K) {
   return w;
 }
 
-Plan plan_matmul(int T, int K) {
+Plan plan_matmul(int T, int K, int N) {
   Plan w;
-  w.tile = fp4_tile(T);
+  w.tile = fp4_tile(T, N);
   w.P = T;
   w.tiles = ceil_div(T, w.tile);
   w.sf = w.take(w.atoms(K));
@@ -238,7 +255,7 @@ int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_fe
 
 size_t dsmoe_mxfp4_linear_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features) {
   if (check_shape("mxfp4_linear", tokens, in_features, out_features) || tokens == 0) return 0;
-  return plan_linear(tokens, in_features).total;
+  return plan_linear(tokens, in_features, out_features).total;
 }
 
 int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_t in_features, int32_t out_features,
@@ -252,7 +269,7 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: pointer NULL or not 16-byte aligned");
   if (tokens > 1 && (row_stride < in_features || row_stride % 8))
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: rows must not overlap and must start on 16 bytes");
-  Plan L = plan_linear(tokens, in_features);
+  Plan L = plan_linear(tokens, in_features, out_features);
   if ((r = check_ws("mxfp4_linear", workspace, workspace_bytes, L.total))) return r;
   L.split_k(false, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -275,7 +292,7 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
 
 size_t dsmoe_mxfp4_matmul_workspace_size(int32_t tokens, int32_t in_features, int32_t out_features) {
   if (check_shape("mxfp4_matmul", tokens, in_features, out_features) || tokens == 0) return 0;
-  return plan_matmul(tokens, in_features).total;
+  return plan_matmul(tokens, in_features, out_features).total;
 }
 
 int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens, int32_t in_features,
@@ -287,7 +304,7 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   if ((r = check_weight("mxfp4_matmul", codes, atoms))) return r;
   if (!aligned(x_codes, 16) || !aligned(x_scales, 4) || !aligned(out, 16) || !aligned(device_status, 4))
     return fail(DSMOE_ERR_INVALID, "mxfp4_matmul: pointer NULL or unaligned");
-  Plan L = plan_matmul(tokens, in_features);
+  Plan L = plan_matmul(tokens, in_features, out_features);
   if ((r = check_ws("mxfp4_matmul", workspace, workspace_bytes, L.total))) return r;
   L.split_k(true, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
