@@ -38,30 +38,51 @@ bool aligned(const void* p, size_t a) { return p && reinterpret_cast<uintptr_t>(
 size_t up(size_t v) { return (v + 255) / 256 * 256; }
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Token tile of a single-group product: the smallest that holds all rows, up
-// to the largest; smaller again while the tiles, each split eight ways along
-// K, leave SMs idle.
-int single_tile(const int* sizes, int n, int rows, int N) {
-  int i = 0;
-  while (i + 1 < n && rows > sizes[i]) ++i;
-  const auto ctas = [&](int tile) {
-    return static_cast<long long>(ceil_div(rows, tile)) * ceil_div(N, 256) * mx::kMaxSplit;
-  };
-  while (i > 0 && ctas(sizes[i]) < sm_count()) --i;
-  return sizes[i];
+// Token tile and K split of a single-group product: the pair with the least
+// estimated time in SM cycles. Per K block a tile of n columns takes 8 n cycles
+// of MMA (16 of N = n, or 8 of N = 2 n with hi and lo side by side), 4-bit rows
+// 2 n, with a floor of 64 cycles an MMA, and small tiles pay `drag` for moving
+// more operand bytes per MMA. Around the K loop a tile costs ~1500 cycles plus
+// its epilogue, a split as much again for the sums. Against every choice
+// measured (T x N x K, us for tiles 32 / 64 / 128 / 160, the estimate's choice
+// starred): 128x7168x2048 *10.7 / 12.8 / - / 15.5; 256x7168x2048 16.0 / *13.0 /
+// - / 20.3; 512x2048x7168 23.9 / *22.0 / 24.4 / 27.1; 1024x7168x2048 42.8 / 33.3 /
+// *32.6 / 36.7; 4096x7168x2048 - / 102 / 98.9 / *91.9.
+struct Choice {
+  int tile, ksplit, units;
+};
+Choice choose(bool fp4, int rows, int K, int N) {
+  static const int bf16_tiles[] = {32, 64, 128, 160}, fp4_tiles[] = {64, 160};
+  const int* tiles = fp4 ? fp4_tiles : bf16_tiles;
+  const int n_tiles = fp4 ? 2 : 4, kb = K / 128, sms = sm_count();
+  Choice best{};
+  double least = 0;
+  for (int i = 0; i < n_tiles; ++i) {
+    const int tile = tiles[i], n = rows < tile ? ceil_div(rows, 16) * 16 : tile;
+    const int pair = fp4 ? 0 : mx::side_by_side(tile, n);
+    const int per_kb = fp4 ? 4 * (n < 128 ? 64 : n / 2) : pair ? 8 * (pair < 64 ? 64 : pair) : 16 * (n < 128 ? 64 : n / 2);
+    const double drag = fp4 ? 1.0 : tile <= 64 ? 1.2 : tile == 128 ? 1.07 : 1.0;
+    const long long units = static_cast<long long>(ceil_div(rows, tile)) * ceil_div(N, 256);
+    const int split = units < sms ? mx::pick_ksplit(fp4, tile, static_cast<int>(units), kb) : 1;
+    const long long waves = split > 1 ? 1 : (units + sms - 1) / sms;
+    double t = waves * (ceil_div(kb, split) * drag * per_kb + 1500 + 25.0 * n);
+    if (split > 1) t += 1500 + 40.0 * n;
+    if (i == 0 || t < least) {
+      least = t;
+      best = {tile, split, static_cast<int>(units)};
+    }
+    if (rows <= tile) break;  // a larger tile holds no more rows and fewer stages
+  }
+  return best;
 }
-int linear_tile(int rows, int N) {
-  static const int sizes[3] = {32, 64, 160};
-  return single_tile(sizes, 3, rows, N);
-}
-int fp4_tile(int rows, int N) {
-  static const int sizes[2] = {64, 160};
-  return single_tile(sizes, 2, rows, N);
-}
-// Token tile where `rows` rows spread over `groups` experts.
+
+// Token tile where `rows` rows spread over `groups` experts: one that most
+// experts' rows fit. Routed FFN, 256 experts of 7168 x 2048 (ms for tiles 64 /
+// 160): T=768 1.26 / 1.38, T=1536 (48 rows per expert) 1.64 / 1.72, T=2048 2.13 /
+// 1.93; below 16 rows per expert tile 32 leaves room for more stages.
 int grouped_tile(long long rows, int groups) {
   const long long mean = (rows + groups - 1) / groups;
-  return mean <= 16 ? 32 : mean <= 32 ? 64 : 160;
+  return mean <= 16 ? 32 : mean <= 48 ? 64 : 160;
 }
 
 struct Plan {
@@ -80,17 +101,18 @@ struct Plan {
     next = take(8);
   }
   size_t atoms(int K) const { return static_cast<size_t>(tiles) * (K / 128) * mx::tile_atoms(tile) * 512; }
-  void split_k(bool fp4, int N, int K) {
-    units = static_cast<int>(tiles) * ceil_div(N, 256);
-    ksplit = mx::pick_ksplit(fp4, tile, units, K / 128);
+  void set(const Choice& c, int rows) {
+    tile = c.tile;
+    ksplit = c.ksplit;
+    units = c.units;
+    tiles = ceil_div(rows, tile);
+    P = rows;
   }
 };
 
 Plan plan_linear(int T, int K, int N) {
   Plan w;
-  w.tile = linear_tile(T, N);
-  w.P = T;
-  w.tiles = ceil_div(T, w.tile);
+  w.set(choose(false, T, K, N), T);
   w.xq = w.take(2 * static_cast<size_t>(T) * K);
   w.sf = w.take(w.atoms(K));
   return w;
@@ -98,9 +120,7 @@ Plan plan_linear(int T, int K, int N) {
 
 Plan plan_matmul(int T, int K, int N) {
   Plan w;
-  w.tile = fp4_tile(T, N);
-  w.P = T;
-  w.tiles = ceil_div(T, w.tile);
+  w.set(choose(true, T, K, N), T);
   w.sf = w.take(w.atoms(K));
   return w;
 }
@@ -269,9 +289,8 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: pointer NULL or not 16-byte aligned");
   if (tokens > 1 && (row_stride < in_features || row_stride % 8))
     return fail(DSMOE_ERR_INVALID, "mxfp4_linear: rows must not overlap and must start on 16 bytes");
-  Plan L = plan_linear(tokens, in_features, out_features);
+  const Plan L = plan_linear(tokens, in_features, out_features);
   if ((r = check_ws("mxfp4_linear", workspace, workspace_bytes, L.total))) return r;
-  L.split_k(false, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   mx::GemmArgs a{};
   a.g.n = 1;
@@ -304,9 +323,8 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   if ((r = check_weight("mxfp4_matmul", codes, atoms))) return r;
   if (!aligned(x_codes, 16) || !aligned(x_scales, 4) || !aligned(out, 16) || !aligned(device_status, 4))
     return fail(DSMOE_ERR_INVALID, "mxfp4_matmul: pointer NULL or unaligned");
-  Plan L = plan_matmul(tokens, in_features, out_features);
+  const Plan L = plan_matmul(tokens, in_features, out_features);
   if ((r = check_ws("mxfp4_matmul", workspace, workspace_bytes, L.total))) return r;
-  L.split_k(true, out_features, in_features);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   mx::GemmArgs a{};
   a.g.n = 1;

@@ -729,7 +729,8 @@ int pick_ksplit(bool fp4, int tile, int units, int kblocks) {
     int n = 0;
     if (fp4) n = tile == 64 ? resident_clusters<Cfg<true, 64, 4>>(s) : resident_clusters<Cfg<true, 160, 4>>(s);
     else n = tile == 32 ? resident_clusters<Cfg<false, 32, 5>>(s)
-             : tile == 64 ? resident_clusters<Cfg<false, 64, 4>>(s) : resident_clusters<Cfg<false, 160, 3>>(s);
+             : tile == 64 ? resident_clusters<Cfg<false, 64, 4>>(s)
+             : tile == 128 ? resident_clusters<Cfg<false, 128, 3>>(s) : resident_clusters<Cfg<false, 160, 3>>(s);
     if (n >= units) best = s;
   }
   return best;
@@ -751,6 +752,8 @@ cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUte
     case 64:
       return swiglu ? launch<Cfg<false, 64, 4>, true>(w0, w1, x, x32, a, grid, s)
                     : launch<Cfg<false, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
+    case 128:  // single-group products only
+      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 128, 3>, false>(w0, w1, x, x32, a, grid, s);
     case 160:
       return swiglu ? launch<Cfg<false, 160, 3>, true>(w0, w1, x, x32, a, grid, s)
                     : launch<Cfg<false, 160, 3>, false>(w0, w1, x, x32, a, grid, s);

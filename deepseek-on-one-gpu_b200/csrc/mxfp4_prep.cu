@@ -512,6 +512,7 @@ cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, in
   switch (tile) {
     case 32: return go(split_kernel<32, 1>, split_kernel<32, R>);
     case 64: return go(split_kernel<64, 1>, split_kernel<64, R>);
+    case 128: return go(split_kernel<128, 1>, split_kernel<128, R>);
     case 160: return go(split_kernel<160, 1>, split_kernel<160, R>);
     default: return cudaErrorInvalidValue;
   }
