@@ -63,8 +63,9 @@ struct GemmArgs {
   int K;
   int P;                 // first lo row of the split activations
   int ksplit;            // parts of K per tile, a cluster's CTAs (1 unless g.counts == NULL)
-  const uint8_t* sfa0;   // scale atoms of the weights [group][ceil(M/128)][K/128][512]
-  const uint8_t* sfa1;   // up projection (SwiGLU), else == sfa0
+  // Scale atoms of the weights, a unit's two A tiles together: [group][pair of
+  // tiles][K/128][2][512], SwiGLU [group][tile][K/128][gate, up][512].
+  const uint8_t* sfa;
   const uint8_t* sfb;    // scale atoms of the rows [tile][K/128][tile_atoms][512]
   __nv_bfloat16* y;      // [row][M]
   int32_t* next;         // counter of handed-out units, 0 before the launch; NULL: units in fixed turns

@@ -259,7 +259,7 @@ int dsmoe_mxfp4_dequantize(const void* codes, const void* scales, int64_t blocks
 
 size_t dsmoe_mxfp4_scale_atoms_bytes(int32_t matrices, int32_t out_features, int32_t in_features) {
   if (matrices < 1 || check_shape("mxfp4_scale_atoms", 0, in_features, out_features)) return 0;
-  return static_cast<size_t>(matrices) * ceil_div(out_features, 128) * (in_features / 128) * 512;
+  return static_cast<size_t>(matrices) * ceil_div(out_features, 256) * (in_features / 128) * 1024;
 }
 
 int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_features, int32_t in_features,
@@ -268,7 +268,7 @@ int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_fe
   if (r) return r;
   if (matrices < 1 || !aligned(scales, 4) || !aligned(atoms, 16))
     return fail(DSMOE_ERR_INVALID, "mxfp4_scale_atoms: no matrix, or pointer NULL or unaligned");
-  MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(scales), matrices, out_features, in_features, 128, 1,
+  MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(scales), matrices, out_features, in_features, 256, 2,
                                  static_cast<uint8_t*>(atoms), reinterpret_cast<cudaStream_t>(stream)));
   return DSMOE_OK;
 }
@@ -299,7 +299,7 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
   a.K = in_features;
   a.P = L.P;
   a.ksplit = L.ksplit;
-  a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
+  a.sfa = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
   a.status = device_status;
@@ -333,7 +333,7 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   a.K = in_features;
   a.P = tokens;
   a.ksplit = L.ksplit;
-  a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
+  a.sfa = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
   a.status = device_status;
@@ -374,7 +374,7 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
   a.K = in_features;
   a.P = L.P;
   a.ksplit = 1;
-  a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(atoms);
+  a.sfa = static_cast<const uint8_t*>(atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
   a.next = at<int32_t>(workspace, L.next);
@@ -416,8 +416,8 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   if (r) return r;
   if (!std::isfinite(scale)) return fail(DSMOE_ERR_INVALID, "mxfp4_moe: scale must be finite");
   if (tokens == 0) return DSMOE_OK;
-  if ((r = check_weight("mxfp4_moe", w->gate_codes, w->gate_atoms)) ||
-      (r = check_weight("mxfp4_moe", w->up_codes, w->up_atoms)) ||
+  if ((r = check_weight("mxfp4_moe", w->gate_codes, w->gate_up_atoms)) ||
+      (r = check_weight("mxfp4_moe", w->up_codes, w->gate_up_atoms)) ||
       (r = check_weight("mxfp4_moe", w->down_codes, w->down_atoms)))
     return r;
   if (!aligned(hidden, 16) || !aligned(out, 16) || !aligned(topk_idx, 8) || !aligned(topk_w, 4) ||
@@ -436,8 +436,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   a.K = H;
   a.P = L.P;
   a.ksplit = 1;
-  a.sfa0 = static_cast<const uint8_t*>(w->gate_atoms);
-  a.sfa1 = static_cast<const uint8_t*>(w->up_atoms);
+  a.sfa = static_cast<const uint8_t*>(w->gate_up_atoms);
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.hq = at<uint8_t>(workspace, L.hq);
   a.hsf = at<uint8_t>(workspace, L.hsf);
@@ -460,7 +459,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
     return r;
   a.M = H;
   a.K = F;
-  a.sfa0 = a.sfa1 = static_cast<const uint8_t*>(w->down_atoms);
+  a.sfa = static_cast<const uint8_t*>(w->down_atoms);
   a.sfb = at<uint8_t>(workspace, L.hsf);
   ++a.next;
   a.y = at<__nv_bfloat16>(workspace, L.y);

@@ -69,12 +69,12 @@ struct Cfg {
   static constexpr int A_TX = FP4 ? A_BYTES : A_BYTES / 2;
   static constexpr int B_OFF = 2 * A_BYTES;
   static constexpr int B_BYTES = TERMS * BN * 128;
-  static constexpr int SFA_BYTES = KB_STAGE * 512;
+  static constexpr int SFA_BYTES = KB_STAGE * 1024;  // both A tiles'
   static constexpr int SFB_BYTES = KB_STAGE * ATOMS * 512;
   // Operand tiles start on 1024 bytes (128-byte swizzle), so the scale atoms
   // of all stages live behind the operands of all stages.
   static constexpr int OP_BYTES = B_OFF + B_BYTES;
-  static constexpr int SF_BYTES = 2 * SFA_BYTES + SFB_BYTES;
+  static constexpr int SF_BYTES = SFA_BYTES + SFB_BYTES;
   static constexpr int SF0 = STAGES * OP_BYTES;
   // TMEM columns
   static constexpr int SF_COLS = KB_STAGE * (1 + ATOMS) * 4;  // of one issuer and stage
@@ -293,7 +293,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   if (p.g.counts) dependency_wait();
   const uint32_t tmem = *s_tmem;
   const int KB = p.K / 128;
-  const int MT = (p.M + BM - 1) / BM;
 
   if (warp == PLAN_WARP) {
     // ------------------------------------------------------------- planner
@@ -340,8 +339,8 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         mbar_arrive(&uempty[ri]);
         const int wrow = e.group * p.M;
         const bool two = e.m1 >= 0;
-        const uint8_t* fa0 = p.sfa0 + (static_cast<size_t>(e.group) * MT + e.m0 / BM) * KB * 512;
-        const uint8_t* fa1 = p.sfa1 + (static_cast<size_t>(e.group) * MT + (two ? e.m1 : 0) / BM) * KB * 512;
+        const int pairs = SWIGLU ? p.M / BM : (p.M + 2 * BM - 1) / (2 * BM);
+        const uint8_t* fa = p.sfa + (static_cast<size_t>(e.group) * pairs + e.m0 / (SWIGLU ? BM : 2 * BM)) * KB * 1024;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
         // Rows side by side come in 32-row boxes; where a small tile has at most
         // 16, in 8-row boxes (the columns behind them keep what an earlier stage
@@ -355,11 +354,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);  // an odd last K block: only its scales exist
           const int kx = FP4 ? kb * 64 : kb * 128;  // coordinate: bytes of packed codes, or numbers
-          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * (C::A_TX + nkb * 512) + xbytes + nkb * C::ATOMS * 512);
+          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * C::A_TX + nkb * 1024 + xbytes + nkb * C::ATOMS * 512);
           tma_load_2d(st, &tm_w0, &full[stage], kx, wrow + e.m0, pol_w);
           if (two) tma_load_2d(st + C::A_BYTES, &tm_w1, &full[stage], kx, wrow + e.m1, pol_w);
-          bulk_load(sf, fa0 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
-          if (two) bulk_load(sf + C::SFA_BYTES, fa1 + static_cast<size_t>(kb) * 512, nkb * 512, &full[stage]);
+          bulk_load(sf, fa + static_cast<size_t>(kb) * 1024, nkb * 1024, &full[stage]);
         };
         auto load_x = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES + C::B_OFF;
@@ -375,7 +373,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
             tma_load_2d(st, &tm_x, &full[stage], kx, e.row0, pol_x);
             if (!FP4) tma_load_2d(st + BN * 128, &tm_x, &full[stage], kx, p.P + e.row0, pol_x);
           }
-          bulk_load(smem + C::SF0 + stage * C::SF_BYTES + 2 * C::SFA_BYTES,
+          bulk_load(smem + C::SF0 + stage * C::SF_BYTES + C::SFA_BYTES,
                     fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512, &full[stage]);
         };
         int kb = e.kb0;
@@ -443,10 +441,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
 #pragma unroll
           for (int h = 0; h < C::KB_STAGE; ++h) {
             if (h < nkb) {
-              copy_scales(ta + h * 4, sf + me * C::SFA_BYTES + h * 512);
+              copy_scales(ta + h * 4, sf + h * 1024 + me * 512);
 #pragma unroll
               for (int a = 0; a < C::ATOMS; ++a)
-                copy_scales(tb + (h * C::ATOMS + a) * 4, sf + 2 * C::SFA_BYTES + (h * C::ATOMS + a) * 512);
+                copy_scales(tb + (h * C::ATOMS + a) * 4, sf + C::SFA_BYTES + (h * C::ATOMS + a) * 512);
             }
           }
 #pragma unroll

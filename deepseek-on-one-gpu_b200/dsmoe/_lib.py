@@ -59,8 +59,8 @@ class MXFP4ExpertsDesc(ctypes.Structure):
     _fields_ = [
         ("hidden", ctypes.c_int32), ("inter", ctypes.c_int32), ("n_routed", ctypes.c_int32),
         ("shared", ctypes.c_int32),
-        ("gate_codes", ctypes.c_void_p), ("gate_atoms", ctypes.c_void_p), ("up_codes", ctypes.c_void_p),
-        ("up_atoms", ctypes.c_void_p), ("down_codes", ctypes.c_void_p), ("down_atoms", ctypes.c_void_p),
+        ("gate_codes", ctypes.c_void_p), ("up_codes", ctypes.c_void_p), ("gate_up_atoms", ctypes.c_void_p),
+        ("down_codes", ctypes.c_void_p), ("down_atoms", ctypes.c_void_p),
     ]
 
 

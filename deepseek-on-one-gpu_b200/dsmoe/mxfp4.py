@@ -190,6 +190,22 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
     return out
 
 
+def _pack_scales(scales: torch.Tensor, mats: int, out_features: int, in_features: int, atoms: torch.Tensor) -> None:
+    with _on(scales.device):
+        check(lib().dsmoe_mxfp4_scale_atoms(ptr(scales), mats, out_features, in_features, ptr(atoms),
+                                            stream_handle(scales.device)), "dsmoe_mxfp4_scale_atoms")
+
+
+def _interleave(gate: torch.Tensor, up: torch.Tensor, mats: int, out_features: int, in_features: int) -> torch.Tensor:
+    """Scale atoms of gate and up [mats, pairs, K/128, 2, 512] -> [mats, out/128, K/128, (gate, up), 512]."""
+    tiles, kb = out_features // 128, in_features // 128
+
+    def by_tile(a):
+        return a.view(mats, -1, kb, 2, 512).transpose(2, 3).reshape(mats, -1, kb, 512)[:, :tiles]
+
+    return torch.stack([by_tile(gate), by_tile(up)], dim=3)
+
+
 class MXFP4Weight:
     """An MXFP4 weight ``[out, in]`` or a stack of experts ``[E, out, in]``,
     held for the products: the codes as they are (not copied when dense and
@@ -211,42 +227,13 @@ class MXFP4Weight:
         self.codes = _dense(codes, 32)
         self.atoms = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.status = _device_status(self.device)
-        self._pack(_dense(scales, 4), 0, mats)
-
-    def _pack(self, scales: torch.Tensor, first: int, mats: int) -> None:
-        per = self.atoms.numel() // (1 if self.experts is None else self.experts)
-        with _on(self.device):
-            check(lib().dsmoe_mxfp4_scale_atoms(ptr(scales), mats, self.out_features, self.in_features,
-                                                ptr(self.atoms) + first * per, stream_handle(self.device)),
-                  "dsmoe_mxfp4_scale_atoms")
+        _pack_scales(_dense(scales, 4), mats, self.out_features, K, self.atoms)
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, scale_inv: torch.Tensor | None = None) -> "MXFP4Weight":
         """From a bf16, fp16 or fp32 weight, or the checkpoint's e4m3 weight
         with its ``weight_scale_inv``."""
         return cls(*mxfp4_quantize(weight, scale_inv))
-
-    @classmethod
-    def _empty(cls, experts: int, out_features: int, in_features: int, device) -> "MXFP4Weight":
-        """A stack to be filled slot by slot (``_set``)."""
-        self = cls.__new__(cls)
-        self.in_features, self.out_features, self.experts = in_features, out_features, experts
-        self.device = _index(torch.device(device))
-        self.codes = torch.zeros(experts, out_features, in_features // 2, dtype=torch.uint8, device=self.device)
-        self.atoms = torch.zeros(lib().dsmoe_mxfp4_scale_atoms_bytes(experts, out_features, in_features),
-                                 dtype=torch.uint8, device=self.device)
-        self.status = _device_status(self.device)
-        return self
-
-    def _set(self, slot: int, weight: torch.Tensor, scale_inv: torch.Tensor | None) -> None:
-        if tuple(weight.shape) != (self.out_features, self.in_features):
-            raise ValueError(f"expert weight is {tuple(weight.shape)}, the stack holds "
-                             f"{(self.out_features, self.in_features)}")
-        if scale_inv is not None and tuple(scale_inv.shape) != (-(-self.out_features // 128), self.in_features // 128):
-            raise ValueError("scale_inv does not go with the weight")
-        scales = torch.empty(self.out_features, self.in_features // BLOCK, dtype=torch.uint8, device=self.device)
-        _quantize_into(weight, scale_inv, self.codes[slot], scales)
-        self._pack(scales, slot, 1)
 
     @property
     def nbytes(self) -> int:
@@ -352,19 +339,60 @@ class MXFP4Experts:
             raise ValueError("MXFP4Experts: gate and up are (G, inter, hidden), down is (G, hidden, inter)")
         if not gate.device == up.device == down.device:
             raise RuntimeError("MXFP4Experts: weights on different devices")
-        self.shared = bool(shared)
-        self.n_routed = gate.experts - int(self.shared)
+        if self.hidden % 128 or self.inter % 128:
+            raise ValueError("MXFP4Experts: hidden and inter must be multiples of 128")
+        self._set_up(gate.codes, up.codes, down.codes, _interleave(gate.atoms, up.atoms, gate.experts, self.inter,
+                                                                   self.hidden), down.atoms, shared)
+
+    def _set_up(self, gate, up, down, gate_up_atoms, down_atoms, shared: bool) -> None:
+        self.shared, self.device = bool(shared), gate.device
+        self.n_routed = gate.shape[0] - int(self.shared)
         if self.n_routed < 1:
             raise ValueError("MXFP4Experts: no routed expert")
-        self.gate, self.up, self.down, self.device = gate, up, down, gate.device
+        self.gate_codes, self.up_codes, self.down_codes = gate, up, down
+        self.gate_up_atoms, self.down_atoms = gate_up_atoms, down_atoms
+        self.status = _device_status(self.device)
         self.desc = _lib.MXFP4ExpertsDesc(
             hidden=self.hidden, inter=self.inter, n_routed=self.n_routed, shared=int(self.shared),
-            gate_codes=ptr(gate.codes), gate_atoms=ptr(gate.atoms), up_codes=ptr(up.codes), up_atoms=ptr(up.atoms),
-            down_codes=ptr(down.codes), down_atoms=ptr(down.atoms))
+            gate_codes=ptr(gate), up_codes=ptr(up), gate_up_atoms=ptr(gate_up_atoms), down_codes=ptr(down),
+            down_atoms=ptr(down_atoms))
+
+    @classmethod
+    def _empty(cls, experts: int, hidden: int, inter: int, device: torch.device) -> "MXFP4Experts":
+        """Room for ``experts`` matrices (the shared expert first), to be
+        written one by one (``_write``)."""
+        self = cls.__new__(cls)
+        self.hidden, self.inter = hidden, inter
+
+        def room(*shape):
+            return torch.zeros(*shape, dtype=torch.uint8, device=device)
+
+        self._set_up(room(experts, inter, hidden // 2), room(experts, inter, hidden // 2),
+                     room(experts, hidden, inter // 2), room(experts, inter // 128, hidden // 128, 2, 512),
+                     room(experts, -(-hidden // 256), inter // 128, 2, 512), True)
+        return self
+
+    def _write(self, slot: int, gate, up, down) -> None:
+        """Quantise one expert's FP8 ``(weight, scale_inv)`` pairs into ``slot``."""
+        packed = []
+        for (w, s), codes in ((gate, self.gate_codes), (up, self.up_codes), (down, self.down_codes)):
+            N, K = codes.shape[1], 2 * codes.shape[2]
+            if tuple(w.shape) != (N, K) or w.dtype != torch.float8_e4m3fn:
+                raise ValueError(f"expert weight is {w.dtype} {tuple(w.shape)}, the bank holds e4m3 {(N, K)}")
+            if tuple(s.shape) != (-(-N // 128), K // 128):
+                raise ValueError("scale_inv does not go with the weight")
+            scales = torch.empty(N, K // BLOCK, dtype=torch.uint8, device=self.device)
+            _quantize_into(w, s, codes[slot], scales)
+            atoms = torch.empty(-(-N // 256), K // 128, 2, 512, dtype=torch.uint8, device=self.device)
+            _pack_scales(scales, 1, N, K, atoms)
+            packed.append(atoms)
+        self.gate_up_atoms[slot].copy_(_interleave(packed[0], packed[1], 1, self.inter, self.hidden)[0])
+        self.down_atoms[slot].copy_(packed[2])
 
     @property
     def nbytes(self) -> int:
-        return self.gate.nbytes + self.up.nbytes + self.down.nbytes
+        return sum(t.numel() for t in (self.gate_codes, self.up_codes, self.down_codes, self.gate_up_atoms,
+                                       self.down_atoms))
 
 
 def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, experts: MXFP4Experts,
@@ -377,7 +405,7 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     rounded to bf16. An id outside the routed experts adds nothing."""
     if not isinstance(experts, MXFP4Experts):
         raise TypeError("mxfp4_moe expects MXFP4Experts")
-    _check_x("mxfp4_moe", hidden, experts.hidden, topk_idx, topk_w, experts.gate.codes)
+    _check_x("mxfp4_moe", hidden, experts.hidden, topk_idx, topk_w, experts.gate_codes)
     if topk_idx.dtype != torch.int64 or topk_w.dtype != torch.float32:
         raise TypeError("mxfp4_moe expects int64 indices and fp32 weights")
     lead = tuple(hidden.shape[:-1])
@@ -393,7 +421,7 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
             ws = _scratch(lib().dsmoe_mxfp4_moe_workspace_size(T, H, experts.inter, experts.n_routed,
                                                                int(experts.shared), K), hidden.device)
             check(lib().dsmoe_mxfp4_moe(ptr(x2), x2.stride(0), T, ctypes.byref(experts.desc), ptr(idx), ptr(w), K,
-                                        float(scale), ptr(out), ptr(ws) or None, ws.numel(), ptr(experts.gate.status),
+                                        float(scale), ptr(out), ptr(ws) or None, ws.numel(), ptr(experts.status),
                                         stream_handle(hidden.device)), "dsmoe_mxfp4_moe")
     return out
 
@@ -402,7 +430,7 @@ def moe_forward(x: torch.Tensor, gate_weight: torch.Tensor, bias: torch.Tensor |
                 experts: MXFP4Experts) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``moe_block``'s work on MXFP4 experts: dense bf16 ``x`` [T, hidden] ->
     output, routing indices and weights. Scratch is private to the call."""
-    _check_x("moe_forward", x, experts.hidden, gate_weight, bias, experts.gate.codes)
+    _check_x("moe_forward", x, experts.hidden, gate_weight, bias, experts.gate_codes)
     cfg = _lib.moe_config(config)
     T, K = x.shape[0], cfg.top_k
     out = torch.empty_like(x)
@@ -412,7 +440,7 @@ def moe_forward(x: torch.Tensor, gate_weight: torch.Tensor, bias: torch.Tensor |
         ws = _scratch(lib().dsmoe_mxfp4_moe_forward_workspace_size(cfg, T), x.device)
         check(lib().dsmoe_mxfp4_moe_forward(cfg, ptr(gate_weight), ptr(bias), ctypes.byref(experts.desc), ptr(x), T,
                                             ptr(out), ptr(idx), ptr(w), ptr(ws) or None, ws.numel(),
-                                            ptr(experts.gate.status), stream_handle(x.device)),
+                                            ptr(experts.status), stream_handle(x.device)),
               "dsmoe_mxfp4_moe_forward")
     return out, idx, w
 
@@ -427,10 +455,7 @@ class MXFP4LayerBank:
         E, H, F = config.n_routed_experts, config.hidden_size, config.moe_intermediate_size
         self.n_slots = self.n_groups = E + 1
         self.device = _index(torch.device(device))
-        self.w = {"gate_proj": MXFP4Weight._empty(E + 1, F, H, self.device),
-                  "up_proj": MXFP4Weight._empty(E + 1, F, H, self.device),
-                  "down_proj": MXFP4Weight._empty(E + 1, H, F, self.device)}
-        self.experts = MXFP4Experts(self.w["gate_proj"], self.w["up_proj"], self.w["down_proj"], shared=True)
+        self.experts = MXFP4Experts._empty(E + 1, H, F, self.device)
         self.slot_of_host = [-1] * (E + 1)
         self.last_use: torch.cuda.Event | None = None
         self.pending: torch.cuda.Event | None = None
@@ -450,15 +475,15 @@ class MXFP4LayerBank:
     def write_slot(self, slot: int, expert: dict, non_blocking: bool = False) -> int:
         """Quantise one FP8 expert ``{proj: (weight, scale_inv)}``, on the host
         or the device, into ``slot``; returns the FP8 bytes read."""
-        n = 0
-        for p, stack in self.w.items():
+        n, pairs = 0, []
+        for p in ("gate_proj", "up_proj", "down_proj"):
             w, s = expert[p]
             if isinstance(w, dict):  # ExpertCache entry form
                 w, s = w["weight"], w["weight_scale_inv"]
             n += w.nbytes + s.nbytes
-            w = w.to(self.device, non_blocking=non_blocking)
-            s = s.to(self.device, torch.float32, non_blocking=non_blocking).contiguous()
-            stack._set(slot, w, s)
+            pairs.append((w.to(self.device, non_blocking=non_blocking),
+                          s.to(self.device, torch.float32, non_blocking=non_blocking).contiguous()))
+        self.experts._write(slot, *pairs)
         return n
 
     def sync_table(self, non_blocking: bool = True) -> None:

@@ -455,7 +455,11 @@ DSMOE_API int dsmoe_mxfp4_dequantize(const void* codes, const void* scales, int6
 
 /*
  * The products read a weight's scales as 512-byte atoms (128 rows x 128
- * numbers): scales [matrices][out][in/32] -> atoms, once per weight.
+ * numbers; rows 32 j + l, j < 4, l < 32, have their four scale bytes at
+ * l * 16 + j * 4): scales [matrices][out][in/32] -> atoms
+ * [matrices][ceil(out/256)][in/128][2][512], once per weight, rows past `out`
+ * zero. The gate and up projections of dsmoe_mxfp4_experts_t are interleaved
+ * instead: gate_up_atoms [matrices][inter/128][hidden/128][gate, up][512].
  */
 DSMOE_API size_t dsmoe_mxfp4_scale_atoms_bytes(int32_t matrices, int32_t out_features, int32_t in_features);
 DSMOE_API int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int32_t out_features, int32_t in_features,
@@ -508,9 +512,8 @@ typedef struct {
   int32_t n_routed;  /* n_routed + shared <= 512 */
   int32_t shared;    /* 0 or 1 */
   const void* gate_codes; /* [n_routed + shared][inter][hidden/2] */
-  const void* gate_atoms;
   const void* up_codes;
-  const void* up_atoms;
+  const void* gate_up_atoms;
   const void* down_codes; /* [n_routed + shared][hidden][inter/2] */
   const void* down_atoms;
 } dsmoe_mxfp4_experts_t;

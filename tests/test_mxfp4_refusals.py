@@ -76,7 +76,7 @@ def test_dequantize_and_atoms_reject():
     assert L.dsmoe_mxfp4_dequantize(64, 64, 4, 0, 72, None) == -1
     assert L.dsmoe_mxfp4_dequantize(64, 64, -1, 0, 64, None) == -1
     assert L.dsmoe_mxfp4_dequantize(None, None, 0, 0, None, None) == 0
-    assert L.dsmoe_mxfp4_scale_atoms_bytes(2, 576, 256) == 2 * 5 * 2 * 512
+    assert L.dsmoe_mxfp4_scale_atoms_bytes(2, 576, 256) == 2 * 3 * 2 * 1024
     assert L.dsmoe_mxfp4_scale_atoms_bytes(0, 576, 256) == 0
     assert L.dsmoe_mxfp4_scale_atoms_bytes(2, 576, 192) == 0
     assert L.dsmoe_mxfp4_scale_atoms_bytes(2, 12, 256) == 0
@@ -139,7 +139,7 @@ def test_moe_rejects(kw, code):
     a.update(kw)
     L = _lib.lib()
     d = _lib.MXFP4ExpertsDesc(hidden=a["h"], inter=a["f"], n_routed=a["e"], shared=a["shared"], gate_codes=a["gate"],
-                              gate_atoms=256, up_codes=256, up_atoms=256, down_codes=a["down"], down_atoms=256)
+                              up_codes=256, gate_up_atoms=256, down_codes=a["down"], down_atoms=256)
     assert L.dsmoe_mxfp4_moe(a["x"], a["stride"], a["t"], ctypes.byref(d), a["idx"], a["w"], a["k"], a["scale"],
                              a["out"], a["ws"], a["bytes"], a["st"], None) == code
     assert L.dsmoe_mxfp4_moe(256, 512, 4, None, 256, 256, 2, 1.0, 256, 256, BIG, 256, None) == -1
@@ -151,8 +151,8 @@ def test_moe_forward_rejects():
     def call(cfg=None, d=None, gate=256, bias=None, x=256, t=4, out=256, idx=256, w=256, ws=256, nbytes=BIG, st=256):
         c = _lib.MoeConfig(**{**dict(hidden=512, inter=256, n_routed=64, n_group=2, topk_group=1, top_k=4, router_mode=0,
                                      norm_topk_prob=1, routed_scaling_factor=2.5), **(cfg or {})})
-        e = _lib.MXFP4ExpertsDesc(**{**dict(hidden=512, inter=256, n_routed=64, shared=1, gate_codes=256, gate_atoms=256,
-                                            up_codes=256, up_atoms=256, down_codes=256, down_atoms=256), **(d or {})})
+        e = _lib.MXFP4ExpertsDesc(**{**dict(hidden=512, inter=256, n_routed=64, shared=1, gate_codes=256, up_codes=256,
+                                            gate_up_atoms=256, down_codes=256, down_atoms=256), **(d or {})})
         return L.dsmoe_mxfp4_moe_forward(c, gate, bias, ctypes.byref(e), x, t, out, idx, w, ws, nbytes, st, None)
 
     assert call(t=-1) == -1 and call(t=0) == 0
