@@ -51,7 +51,7 @@ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 struct Choice {
   int tile, ksplit, units;
 };
-Choice choose(bool fp4, int rows, int K, int N) {
+Choice estimate(bool fp4, int rows, int K, int N) {
   static const int bf16_tiles[] = {32, 64, 128, 160}, fp4_tiles[] = {64, 160};
   const int* tiles = fp4 ? fp4_tiles : bf16_tiles;
   const int n_tiles = fp4 ? 2 : 4, kb = K / 128, sms = sm_count();
@@ -74,6 +74,25 @@ Choice choose(bool fp4, int rows, int K, int N) {
     if (rows <= tile) break;  // a larger tile holds no more rows and fewer stages
   }
   return best;
+}
+
+// The choice depends on sizes and the device only; the last ones asked for are
+// remembered (a decode loop asks for the same few, twice per call, and the
+// occupancy queries behind an estimate cost as much as a launch).
+Choice choose(bool fp4, int rows, int K, int N) {
+  struct Entry {
+    int dev, rows, K, N;
+    bool fp4;
+    Choice c;
+  };
+  static thread_local Entry memo[64] = {};  // rows == 0: empty
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint32_t h = (rows * 2654435761u) ^ (K * 40503u) ^ (N * 69069u) ^ (fp4 ? 977u : 0u);
+  Entry& e = memo[(h >> 16 ^ h) & 63];
+  if (e.rows != rows || e.K != K || e.N != N || e.fp4 != fp4 || e.dev != dev)
+    e = {dev, rows, K, N, fp4, estimate(fp4, rows, K, N)};
+  return e.c;
 }
 
 // Token tile where `rows` rows spread over `groups` experts: one that most

@@ -91,11 +91,13 @@ def _require(what: str, *tensors: torch.Tensor) -> None:
             raise TypeError(f"{what} expects tensors")
         if not t.is_cuda:
             raise RuntimeError("dsmoe runs on CUDA tensors only (no CPU fallback)")
-        if dev is not None and t.device != dev:
-            raise RuntimeError(f"{what}: tensors on different devices ({dev}, {t.device})")
-        dev = t.device
         if grad and t.requires_grad:
             raise RuntimeError(f"{what} has no backward: detach the inputs or call it under torch.no_grad()")
+        d = t.device
+        if dev is None:
+            dev = d
+        elif d != dev:
+            raise RuntimeError(f"{what}: tensors on different devices ({dev}, {d})")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -111,7 +113,8 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 
 def _dense(t: torch.Tensor, align: int) -> torch.Tensor:
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t.clone() if t.data_ptr() % align else t
 
 
@@ -167,11 +170,10 @@ def _check_pair(what: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
     _require(what, codes, scales)
     if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise TypeError(f"{what} expects uint8 codes and scales")
-    if codes.dim() < 1 or codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1] or \
-            codes.shape[-1] != 16 * scales.shape[-1]:
-        raise ValueError(f"{what}: codes [..., K/2] {tuple(codes.shape)} do not go with scales [..., K/32] "
-                         f"{tuple(scales.shape)}")
-    return 2 * codes.shape[-1]
+    c, s = codes.shape, scales.shape
+    if len(c) < 1 or c[:-1] != s[:-1] or len(c) != len(s) or c[-1] != 16 * s[-1]:
+        raise ValueError(f"{what}: codes [..., K/2] {tuple(c)} do not go with scales [..., K/32] {tuple(s)}")
+    return 2 * c[-1]
 
 
 def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
@@ -281,8 +283,8 @@ def mxfp4_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: MXFP4Weight)
     if K != weight.in_features:
         raise ValueError(f"mxfp4_matmul: activations have {K} features, the weight {weight.in_features}")
     shape, N = codes.shape[:-1], weight.out_features
-    c2, s2 = _dense(codes.reshape(-1, K // 2), 16), _dense(scales.reshape(-1, K // BLOCK), 4)
-    T = c2.shape[0]
+    c2, s2 = _dense(codes, 16), _dense(scales, 4)
+    T = c2.numel() // c2.shape[-1]
     out = torch.empty(*shape, N, dtype=torch.bfloat16, device=codes.device)
     if T:
         with _on(codes.device):

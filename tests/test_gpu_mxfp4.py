@@ -519,3 +519,107 @@ def test_current_device_and_default_stream_are_left_alone():
         assert torch.cuda.current_stream() == side
     side.synchronize()
     assert torch.equal(y, want) and torch.cuda.current_device() == 0
+
+
+# ------------------------------------------------- calls at the edge of the rules
+def test_no_rows_for_any_expert():
+    g = gen("none")
+    w = MXFP4Weight(*weight(g, 5, 256, 256))
+    x = torch.randn(40, 256, generator=g, device=DEV).to(torch.bfloat16)
+    off = torch.zeros(6, dtype=torch.int32, device=DEV)
+    assert bool((mxfp4_grouped_linear(x, w, off) == 0).all())
+    assert mxfp4_grouped_linear(x[:0], w, off).shape == (0, 256)
+    ws, _ = experts(g, 8, 256, 128)
+    idx = torch.full((40, 3), -1, dtype=torch.int64, device=DEV)
+    tw = torch.ones(40, 3, device=DEV)
+    assert bool((mxfp4_moe(x, idx, tw, MXFP4Experts(*ws, shared=False)) == 0).all())
+    assert mxfp4_moe(x[:0], idx[:0], tw[:0], MXFP4Experts(*ws)).shape == (0, 256)
+    assert mxfp4_status(DEV) == 0
+
+
+def test_matmul_nan_scale_is_one_row():
+    g = gen("mmnan")
+    ac, asc = weight(g, 70, 512, std=1.0)
+    w = MXFP4Weight(*weight(g, 264, 512))
+    clean = mxfp4_matmul(ac, asc, w)
+    asc[33, 7] = 255
+    y = mxfp4_matmul(ac, asc, w)
+    rest = torch.arange(70, device=DEV) != 33
+    assert bool(torch.isnan(y[33]).all()) and torch.equal(y[rest], clean[rest])
+
+
+def test_matmul_leading_dims_and_strides():
+    g = gen("mmst")
+    ac, asc = weight(g, 6, 4, 256, std=1.0)
+    codes, scales = weight(g, 64, 256)
+    w = MXFP4Weight(codes, scales)
+    wd = O.dequantize(codes, scales)
+    y = mxfp4_matmul(ac, asc, w)
+    assert y.shape == (6, 4, 64)
+    check_product(y.view(24, 64), O.dequantize(ac, asc).view(24, 256), wd)
+    assert torch.equal(mxfp4_matmul(ac[:, 1], asc[:, 1], w), y[:, 1])
+    assert torch.equal(mxfp4_matmul(ac.transpose(0, 1), asc.transpose(0, 1), w), y.transpose(0, 1))
+    assert mxfp4_matmul(ac[:0], asc[:0], w).shape == (0, 4, 64)
+
+
+def test_results_do_not_depend_on_the_sm_limit():
+    from dsmoe._lib import set_gemm_sm_limit
+    g = gen("lim")
+    ws, _ = experts(g, 17, 256, 256)
+    ex, lw = MXFP4Experts(*ws), MXFP4Weight(*weight(g, 512, 1024))
+    x = torch.randn(200, 256, generator=g, device=DEV).to(torch.bfloat16)
+    z = torch.randn(300, 1024, generator=g, device=DEV).to(torch.bfloat16)
+    r = routing(g, 200, 16, 4)
+    want = mxfp4_moe(x, *r, ex), mxfp4_linear(z, lw)
+    try:
+        for n in (1, 37, 100):
+            set_gemm_sm_limit(n)
+            assert torch.equal(mxfp4_moe(x, *r, ex), want[0]) and torch.equal(mxfp4_linear(z, lw), want[1])
+    finally:
+        set_gemm_sm_limit(0)
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    g = gen("thr")
+    ws, _ = experts(g, 33, 256, 256)
+    ex = MXFP4Experts(*ws)
+    xs = [torch.randn(n, 256, generator=g, device=DEV).to(torch.bfloat16) for n in (5, 300)]
+    rs = [routing(g, n, 32, 4) for n in (5, 300)]
+    want = [mxfp4_moe(x, *r, ex) for x, r in zip(xs, rs)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                y = mxfp4_moe(xs[i], *rs[i], ex)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    bad.append(i)
+
+    t = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [a.start() for a in t]
+    [a.join() for a in t]
+    assert not bad and mxfp4_status(DEV) == 0
+
+
+def test_first_call_inside_a_capture():
+    """A fresh process whose first product runs inside a graph capture."""
+    import subprocess
+    import sys
+    code = (
+        "import sys, torch; sys.path.insert(0, 'deepseek-on-one-gpu_b200')\n"
+        "from dsmoe import *\n"
+        "w = MXFP4Weight(*mxfp4_quantize(torch.ones(256, 512, device='cuda')))\n"
+        "e = [MXFP4Weight(*mxfp4_quantize(torch.full(s, 0.25, device='cuda'))) for s in ((5, 128, 512), (5, 128, 512), (5, 512, 128))]\n"
+        "e = MXFP4Experts(*e)\n"
+        "x = torch.ones(3, 512, dtype=torch.bfloat16, device='cuda')\n"
+        "i, t = torch.zeros(3, 2, dtype=torch.int64, device='cuda'), torch.ones(3, 2, device='cuda')\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    y, z = mxfp4_linear(x, w), mxfp4_moe(x, i, t, e)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert bool((y == 512).all()) and torch.equal(z, mxfp4_moe(x, i, t, e)) and mxfp4_status('cuda') == 0\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -124,3 +124,36 @@ def test_two_captured_blocks_at_once_and_a_larger_call_between():
 def test_no_tokens():
     cfg, store, gt = setup()
     assert moe_block(torch.zeros(0, H, dtype=torch.bfloat16, device=DEV), LAYER, store, gt, cfg).shape == (0, H)
+
+
+def test_quantise_one_layer_and_run_it_by_hand():
+    """The operators one after the other, as a caller without moe_block uses
+    them: checkpoint experts to MXFP4, route, the routed FFN; and the FFN out
+    of ragged products, with the same result up to its roundings."""
+    from dsmoe import (MXFP4Experts, MXFP4Weight, mxfp4_grouped_linear, mxfp4_linear, mxfp4_moe, route)
+    cfg, store, gt = setup()
+    x = activations(50, 90, H).to(DEV)
+    ex = [store.get_shared_expert_weights(LAYER)] + [store.device_expert(LAYER, e) for e in range(256)]
+    stacks = [MXFP4Weight.quantize(torch.stack([e[p][0] for e in ex]), torch.stack([e[p][1] for e in ex])) for p in PROJS]
+    idx, w = route(x, store.get_gate_weight(LAYER), cfg)
+    y = mxfp4_moe(x, idx, w, MXFP4Experts(*stacks), cfg.routed_scaling_factor)
+    assert torch.equal(y, moe_block(x, LAYER, store, gt, cfg))
+    # by ragged products: rows sorted by expert, silu and the sum in torch
+    flat = idx.reshape(-1)
+    order = torch.argsort(flat, stable=True)
+    rows = x[order // 8]
+    offsets = torch.cat([flat.new_zeros(1), torch.bincount(flat, minlength=256).cumsum(0)]).int()
+    routed = [MXFP4Weight.quantize(torch.stack([e[p][0] for e in ex[1:]]), torch.stack([e[p][1] for e in ex[1:]]))
+              for p in PROJS]
+    g, u = (mxfp4_grouped_linear(rows, s, offsets).float() for s in routed[:2])
+    out = mxfp4_grouped_linear((torch.nn.functional.silu(g) * u).bfloat16(), routed[2], offsets).float()
+    acc = torch.zeros_like(x, dtype=torch.float32).index_add_(0, order // 8, out * w.reshape(-1)[order, None])
+    one = [MXFP4Weight.quantize(*ex[0][p]) for p in PROJS]
+    sh = mxfp4_linear((torch.nn.functional.silu(mxfp4_linear(x, one[0]).float()) *
+                       mxfp4_linear(x, one[1]).float()).bfloat16(), one[2]).float()
+    z = acc * cfg.routed_scaling_factor + sh
+    # g, u, h and each row are rounded to bf16 (2^-8 each) where mxfp4_moe keeps
+    # fp32 or 2^-9, both sides round their rows: 6 roundings of at most 2^-8
+    # between them, and the terms of a sum are within 3 times it
+    err = float((y.float() - z).norm() / z.norm())
+    assert err <= 3 * 6 * 2.0 ** -8 / math.sqrt(3), err
