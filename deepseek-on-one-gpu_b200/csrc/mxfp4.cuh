@@ -170,13 +170,18 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
 cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const Groups& g, int tile,
                          const int64_t* idx, const int32_t* pos, int top_k, int shared, int P, uint8_t* xq, uint8_t* sf,
                          __nv_bfloat16* zero_out, int M, cudaStream_t s);
-// launch_route_plan and launch_split in one kernel, for a few tokens: tile 32,
-// at most kRouteTokens tokens and 256 pairs.
-constexpr int kRouteTokens = 32;
+// launch_route_plan and launch_split in one kernel, for up to kRoutePairs pairs.
+constexpr int kRoutePairs = 1024;
 cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
-                               int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
+                               int n_routed, int shared, int tile, int P, int32_t* counts, int32_t* row_start,
                                int32_t* tile_start, int32_t* next, int32_t* pos, uint8_t* xq, uint8_t* sf,
                                cudaStream_t s);
+// launch_segments and launch_split in one kernel, for few rows.
+constexpr int kSegmentRows = 1024;
+cudaError_t launch_segments_split(const __nv_bfloat16* x, long long row_stride, int rows, int K, const int32_t* offsets,
+                                  int n, int tile, int32_t* counts, int32_t* row_start, int32_t* tile_start,
+                                  int32_t* next, int* status, uint8_t* xq, uint8_t* sf, __nv_bfloat16* zero_out, int M,
+                                  cudaStream_t s);
 // out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
                            int shared, float scale, __nv_bfloat16* out, cudaStream_t s);

@@ -398,13 +398,20 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
   a.y = static_cast<__nv_bfloat16*>(out);
   a.next = at<int32_t>(workspace, L.next);
   a.status = device_status;
-  MX_CUDA(mx::launch_segments(offsets, n_experts, rows, L.tile, at<int32_t>(workspace, L.counts),
-                              at<int32_t>(workspace, L.row_start), at<int32_t>(workspace, L.tile_start), a.next,
-                              device_status, s));
-  MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, rows, in_features, a.g, L.tile, nullptr,
-                           nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf),
-                           clear_rest ? a.y : nullptr, out_features, s));
-  return run_gemm(false, false, codes, codes, n_experts, at<uint8_t>(workspace, L.xq), a, L.tile,
+  const __nv_bfloat16* rx = static_cast<const __nv_bfloat16*>(x);
+  int32_t *counts = at<int32_t>(workspace, L.counts), *row_start = at<int32_t>(workspace, L.row_start),
+          *tile_start = at<int32_t>(workspace, L.tile_start);
+  uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
+  __nv_bfloat16* clear = clear_rest ? a.y : nullptr;
+  if (rows <= mx::kSegmentRows) {
+    MX_CUDA(mx::launch_segments_split(rx, row_stride, rows, in_features, offsets, n_experts, L.tile, counts, row_start,
+                                      tile_start, a.next, device_status, xq, sf, clear, out_features, s));
+  } else {
+    MX_CUDA(mx::launch_segments(offsets, n_experts, rows, L.tile, counts, row_start, tile_start, a.next, device_status, s));
+    MX_CUDA(mx::launch_split(rx, row_stride, rows, in_features, a.g, L.tile, nullptr, nullptr, 0, 0, L.P, xq, sf, clear,
+                             out_features, s));
+  }
+  return run_gemm(false, false, codes, codes, n_experts, xq, a, L.tile,
                   L.tiles * ceil_div(out_features, 256), s);
 }
 
@@ -465,8 +472,8 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   int32_t *counts = at<int32_t>(workspace, L.counts), *row_start = at<int32_t>(workspace, L.row_start),
           *tile_start = at<int32_t>(workspace, L.tile_start);
   uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
-  if (tokens <= mx::kRouteTokens && L.tile == 32) {
-    MX_CUDA(mx::launch_route_split(x, row_stride, tokens, H, topk_idx, top_k, E, shared, L.P, counts, row_start,
+  if (tokens * top_k <= mx::kRoutePairs) {
+    MX_CUDA(mx::launch_route_split(x, row_stride, tokens, H, topk_idx, top_k, E, shared, L.tile, L.P, counts, row_start,
                                    tile_start, a.next, pos, xq, sf, s));
   } else {
     MX_CUDA(mx::launch_route_plan(topk_idx, tokens, top_k, E, shared, L.tile, counts, row_start, tile_start, a.next, pos,

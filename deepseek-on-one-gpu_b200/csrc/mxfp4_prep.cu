@@ -334,73 +334,84 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __nv_bfloat1
   }
 }
 
-// Plan and split for a few tokens. Every block builds the group tables for
-// itself (a 512-entry histogram and scan in shared memory, ~1 us) instead of
-// waiting for a kernel that does; block 0 also writes them out. A group has at
-// most 32 rows, one token tile.
-__global__ void __launch_bounds__(kSplitThreads) route_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride,
-                                                          int T, int K, const int64_t* __restrict__ idx, int top_k,
-                                                          int n_routed, int shared, int P,
-                                                          int32_t* __restrict__ counts, int32_t* __restrict__ row_start,
-                                                          int32_t* __restrict__ tile_start, int32_t* __restrict__ next,
-                                                          int32_t* __restrict__ pos, uint8_t* __restrict__ xq,
-                                                          uint8_t* __restrict__ sf) {
-  constexpr int TILE = 32;
-  static_assert(kRouteTokens <= TILE, "one tile per group");
-  __shared__ int s_e[256], s_cnt[kMaxGroups], s_start[kMaxGroups], s_tile[kMaxGroups];
-  constexpr int NT = kSplitThreads, GT = kMaxGroups / NT;  // groups per thread
-  __shared__ int s_sum[2][NT / 32];
-  __shared__ int s_row[MAXR];
-  __shared__ SfSpot s_spot[MAXR];
-  launch_dependents();
-  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int pairs = T * top_k, G = n_routed + shared;
-  const Cols q = load_cols(x + t * row_stride, K);
-  for (int p = tid; p < 256; p += NT) {
-    int e = -1;
-    if (p < pairs) {
-      const int64_t v = __ldg(idx + p);
-      if (v >= 0 && v < n_routed) e = static_cast<int>(v) + shared;
-    }
-    s_e[p] = e;
-  }
-  for (int g = tid; g < kMaxGroups; g += NT) s_cnt[g] = 0;
-  __syncthreads();
-  for (int p = tid; p < pairs; p += NT)
-    if (s_e[p] >= 0) atomicAdd(&s_cnt[s_e[p]], 1);
-  if (shared && tid == 0) s_cnt[0] = T;
-  __syncthreads();
-  // Exclusive scans of rows and tiles; thread tid has groups GT * tid and up.
-  int c[GT], rows = 0, tiles = 0;
+// Tables and split for a few rows: every block builds the group tables for
+// itself in shared memory (~1 us) instead of waiting for a kernel that does;
+// block 0 also writes them out.
+struct SmallTables {
+  int cnt[kMaxGroups], start[kMaxGroups], tile[kMaxGroups];
+  int sum[2][kSplitThreads / 32];
+};
+constexpr int kGroupsPerThread = kMaxGroups / kSplitThreads;
+
+// Exclusive scan of the token tiles (and with ROWS of the rows) of t.cnt;
+// thread tid has groups kGroupsPerThread * tid and up.
+template <int TILE, bool ROWS>
+__device__ __forceinline__ void scan_tables(SmallTables& t) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int c[kGroupsPerThread], rows = 0, tiles = 0;
 #pragma unroll
-  for (int j = 0; j < GT; ++j) {
-    c[j] = s_cnt[GT * tid + j];
+  for (int j = 0; j < kGroupsPerThread; ++j) {
+    c[j] = t.cnt[kGroupsPerThread * tid + j];
     rows += c[j];
-    tiles += c[j] > 0;
+    tiles += (c[j] + TILE - 1) / TILE;
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int a = __shfl_up_sync(0xffffffffu, rows, o), b = __shfl_up_sync(0xffffffffu, tiles, o);
     if (lane >= o) rows += a, tiles += b;
   }
-  if (lane == 31) s_sum[0][warp] = rows, s_sum[1][warp] = tiles;
+  if (lane == 31) t.sum[0][warp] = rows, t.sum[1][warp] = tiles;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) rows += s_sum[0][w], tiles += s_sum[1][w];
+  for (int w = 0; w < warp; ++w) rows += t.sum[0][w], tiles += t.sum[1][w];
 #pragma unroll
-  for (int j = GT - 1; j >= 0; --j) {
+  for (int j = kGroupsPerThread - 1; j >= 0; --j) {
     rows -= c[j];
-    tiles -= c[j] > 0;
-    s_start[GT * tid + j] = rows;
-    s_tile[GT * tid + j] = tiles;
+    tiles -= (c[j] + TILE - 1) / TILE;
+    if (ROWS) t.start[kGroupsPerThread * tid + j] = rows;
+    t.tile[kGroupsPerThread * tid + j] = tiles;
   }
   __syncthreads();
-  if (blockIdx.x == 0 && blockIdx.y == 0) {
-    if (tid < 2) next[tid] = 0;
-    for (int g = tid; g <= G; g += NT) {
-      if (g < G) counts[g] = s_cnt[g], row_start[g] = s_start[g], tile_start[g] = s_tile[g];
-      else tile_start[g] = s_tile[G - 1] + (s_cnt[G - 1] > 0);
-    }
+}
+
+template <int TILE>
+__device__ __forceinline__ void write_tables(const SmallTables& t, int G, int32_t* counts, int32_t* row_start,
+                                             int32_t* tile_start, int32_t* next) {
+  if (blockIdx.x != 0 || blockIdx.y != 0) return;
+  if (threadIdx.x < 2) next[threadIdx.x] = 0;
+  for (int g = threadIdx.x; g <= G; g += kSplitThreads) {
+    if (g < G) counts[g] = t.cnt[g], row_start[g] = t.start[g], tile_start[g] = t.tile[g];
+    else tile_start[g] = t.tile[G - 1] + (t.cnt[G - 1] + TILE - 1) / TILE;
   }
+}
+
+template <int TILE>
+__global__ void __launch_bounds__(kSplitThreads)
+route_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T, int K,
+                   const int64_t* __restrict__ idx, int top_k, int n_routed, int shared, int P,
+                   int32_t* __restrict__ counts, int32_t* __restrict__ row_start, int32_t* __restrict__ tile_start,
+                   int32_t* __restrict__ next, int32_t* __restrict__ pos, uint8_t* __restrict__ xq,
+                   uint8_t* __restrict__ sf) {
+  constexpr int NT = kSplitThreads;
+  __shared__ SmallTables tab;
+  __shared__ int s_e[kRoutePairs];
+  __shared__ int s_row[MAXR];
+  __shared__ SfSpot s_spot[MAXR];
+  launch_dependents();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pairs = T * top_k;
+  const Cols q = load_cols(x + t * row_stride, K);
+  for (int p = tid; p < pairs; p += NT) {
+    const int64_t v = __ldg(idx + p);
+    s_e[p] = v >= 0 && v < n_routed ? static_cast<int>(v) + shared : -1;
+  }
+  for (int g = tid; g < kMaxGroups; g += NT) tab.cnt[g] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += NT)
+    if (s_e[p] >= 0) atomicAdd(&tab.cnt[s_e[p]], 1);
+  if (shared && tid == 0) tab.cnt[0] = T;
+  __syncthreads();
+  scan_tables<TILE, true>(tab);
+  write_tables<TILE>(tab, n_routed + shared, counts, row_start, tile_start, next);
   // A warp places a pair of the token: earlier pairs of the same expert first.
   const int n = top_k + shared;
   for (int k = warp; k < top_k; k += NT / 32) {
@@ -408,9 +419,9 @@ __global__ void __launch_bounds__(kSplitThreads) route_split_kernel(const __nv_b
     int rank = 0;
     for (int b = 0; b < p; b += 32) rank += __popc(__ballot_sync(0xffffffffu, b + lane < p && s_e[b + lane] == mine));
     if (lane == 0) {
-      const int row = mine >= 0 ? s_start[mine] + rank : -1;
+      const int row = mine >= 0 ? tab.start[mine] + rank : -1;
       s_row[shared + k] = row;
-      if (mine >= 0) s_spot[shared + k] = sf_spot<TILE>(s_tile[mine], s_cnt[mine], rank, K / 128);
+      if (mine >= 0) s_spot[shared + k] = sf_spot<TILE>(tab.tile[mine], tab.cnt[mine], rank, K / 128);
       if (blockIdx.y == 0) pos[p] = row;
     }
   }
@@ -420,6 +431,74 @@ __global__ void __launch_bounds__(kSplitThreads) route_split_kernel(const __nv_b
   }
   __syncthreads();
   split_row(q, K, P, n, s_row, s_spot, tile_atoms(TILE), xq, sf);
+}
+
+// segments_kernel and split_kernel in one; offsets are clamped the same way.
+template <int TILE>
+__global__ void __launch_bounds__(kSplitThreads)
+segments_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int rows, int K,
+                      const int32_t* __restrict__ offsets, int E, int32_t* __restrict__ counts,
+                      int32_t* __restrict__ row_start, int32_t* __restrict__ tile_start, int32_t* __restrict__ next,
+                      int* __restrict__ status, uint8_t* __restrict__ xq, uint8_t* __restrict__ sf,
+                      __nv_bfloat16* __restrict__ zero_out, int M) {
+  constexpr int GT = kGroupsPerThread;
+  __shared__ SmallTables tab;
+  __shared__ int s_row[1];
+  __shared__ SfSpot s_spot[1];
+  launch_dependents();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Cols q = load_cols(x + t * row_stride, K);
+  // Ends: the running maximum of the clamped offsets.
+  const int first = min(max(__ldg(offsets), 0), rows);
+  int end[GT], top = first;
+#pragma unroll
+  for (int j = 0; j < GT; ++j) {
+    const int g = GT * tid + j;
+    if (g < E) {
+      const int lo = __ldg(offsets + g), hi = __ldg(offsets + g + 1);
+      if (blockIdx.x == 0 && blockIdx.y == 0 && (lo < 0 || hi < lo || hi > rows)) atomicCAS(status, 0, kDevBadCount);
+      top = max(top, min(max(hi, 0), rows));
+    }
+    end[j] = top;
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, top, o);
+    if (lane >= o) top = max(top, a);
+  }
+  if (lane == 31) tab.sum[0][warp] = top;
+  int before = __shfl_up_sync(0xffffffffu, top, 1);
+  if (lane == 0) before = first;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) before = max(before, tab.sum[0][w]);
+#pragma unroll
+  for (int j = 0; j < GT; ++j) {
+    const int start = j ? max(before, end[j - 1]) : before;
+    tab.start[GT * tid + j] = start;
+    tab.cnt[GT * tid + j] = max(before, end[j]) - start;
+  }
+  __syncthreads();  // also: tab.sum is free again
+  scan_tables<TILE, false>(tab);
+  write_tables<TILE>(tab, E, counts, row_start, tile_start, next);
+  if (tid == 0) {
+    int lo = 0, hi = E;  // last group that starts at or before the row
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tab.start[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int local = t - tab.start[lo];
+    const bool in = local >= 0 && local < tab.cnt[lo];
+    s_row[0] = in ? t : -1;
+    if (in) s_spot[0] = sf_spot<TILE>(tab.tile[lo], tab.cnt[lo], local, K / 128);
+  }
+  __syncthreads();
+  if (s_row[0] < 0) {
+    if (zero_out && blockIdx.y == 0)
+      for (int c = tid; c < M / 8; c += kSplitThreads)
+        reinterpret_cast<uint4*>(zero_out + static_cast<size_t>(t) * M)[c] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  split_row(q, K, rows, 1, s_row, s_spot, tile_atoms(TILE), xq, sf);
 }
 
 __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, int T, int H,
@@ -519,13 +598,38 @@ cudaError_t launch_split(const __nv_bfloat16* x, long long row_stride, int T, in
 }
 
 cudaError_t launch_route_split(const __nv_bfloat16* x, long long row_stride, int T, int K, const int64_t* idx, int top_k,
-                               int n_routed, int shared, int P, int32_t* counts, int32_t* row_start,
+                               int n_routed, int shared, int tile, int P, int32_t* counts, int32_t* row_start,
                                int32_t* tile_start, int32_t* next, int32_t* pos, uint8_t* xq, uint8_t* sf,
                                cudaStream_t s) {
-  if (T > kRouteTokens || T * top_k > 256 || n_routed + shared > kMaxGroups) return cudaErrorInvalidValue;
-  route_split_kernel<<<dim3(T, (K + kSplitCols - 1) / kSplitCols), kSplitThreads, 0, s>>>(x, row_stride, T, K, idx, top_k, n_routed, shared, P,
-                                                                 counts, row_start, tile_start, next, pos, xq, sf);
-  return cudaGetLastError();
+  if (T * top_k > kRoutePairs || n_routed + shared > kMaxGroups) return cudaErrorInvalidValue;
+  const dim3 grid(T, (K + kSplitCols - 1) / kSplitCols);
+  auto go = [&](auto kern) {
+    return launch_chained(false, kern, grid, kSplitThreads, 0, s, x, row_stride, T, K, idx, top_k, n_routed, shared, P,
+                          counts, row_start, tile_start, next, pos, xq, sf);
+  };
+  switch (tile) {
+    case 32: return go(route_split_kernel<32>);
+    case 64: return go(route_split_kernel<64>);
+    case 160: return go(route_split_kernel<160>);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
+cudaError_t launch_segments_split(const __nv_bfloat16* x, long long row_stride, int rows, int K, const int32_t* offsets,
+                                  int n, int tile, int32_t* counts, int32_t* row_start, int32_t* tile_start,
+                                  int32_t* next, int* status, uint8_t* xq, uint8_t* sf, __nv_bfloat16* zero_out, int M,
+                                  cudaStream_t s) {
+  const dim3 grid(rows, (K + kSplitCols - 1) / kSplitCols);
+  auto go = [&](auto kern) {
+    return launch_chained(false, kern, grid, kSplitThreads, 0, s, x, row_stride, rows, K, offsets, n, counts, row_start,
+                          tile_start, next, status, xq, sf, zero_out, M);
+  };
+  switch (tile) {
+    case 32: return go(segments_split_kernel<32>);
+    case 64: return go(segments_split_kernel<64>);
+    case 160: return go(segments_split_kernel<160>);
+    default: return cudaErrorInvalidValue;
+  }
 }
 
 cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,

@@ -623,3 +623,29 @@ def test_first_call_inside_a_capture():
         "assert bool((y == 512).all()) and torch.equal(z, mxfp4_moe(x, i, t, e)) and mxfp4_status('cuda') == 0\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("off", [[0, 900, 200, 1500], [-3, 10, 1499, 1900], [100, 700, 700, 1400]])
+def test_grouped_many_rows_with_odd_offsets(off):
+    """More rows than the one-kernel form of the segment tables takes: the same
+    clamping, and rows outside every segment."""
+    g = gen("bo2")
+    codes, scales = weight(g, 3, 256, 256)
+    x = torch.randn(1500, 256, generator=g, device=DEV).to(torch.bfloat16)
+    w = MXFP4Weight(codes, scales)
+    y = mxfp4_grouped_linear(x, w, torch.tensor(off, dtype=torch.int32, device=DEV))
+    bad = off[0] < 0 or off[-1] > 1500 or any(a > b for a, b in zip(off, off[1:]))
+    assert mxfp4_status(DEV) == (6 if bad else 0)
+    clean = [min(max(o, 0), 1500) for o in off]
+    for i in range(1, 4):
+        clean[i] = max(clean[i], clean[i - 1])
+    wd = O.dequantize(codes, scales)
+    for e in range(3):
+        if clean[e + 1] > clean[e]:
+            check_product(y[clean[e]:clean[e + 1]], x[clean[e]:clean[e + 1]].double(), wd[e])
+    assert bool((y[:clean[0]] == 0).all()) and bool((y[clean[3]:] == 0).all())
+    # the one-kernel form on the first rows
+    n = 1000
+    part = torch.tensor([min(c, n) for c in clean], dtype=torch.int32, device=DEV)
+    small = mxfp4_grouped_linear(x[:n], w, part)
+    check_product(small[int(part[0]):int(part[1])], x[int(part[0]):int(part[1])].double(), wd[0])
