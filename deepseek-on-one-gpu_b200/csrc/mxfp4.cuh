@@ -35,14 +35,18 @@ constexpr int kMaxSplit = 8;  // CTAs of a cluster that share one tile's K
 // scale atoms per token tile and K block.
 constexpr int tile_atoms(int bn) { return bn > 64 ? 2 : 1; }
 
-// bf16 activations: columns of a tile that run hi and lo side by side in one
-// MMA (rounded to 32, hi columns then lo columns), or 0 where hi and lo are
-// two MMAs. Side by side the MMA is twice as wide, which pays while a narrow
-// one does not fill the tensor pipe; the accumulators then take 4 columns of
-// TMEM per token, which caps it at 96.
+// bf16 activations: columns n of a tile that run hi and lo side by side in one
+// MMA of N = 2 n (hi columns then lo columns), or 0 where hi and lo are two
+// MMAs. Side by side the MMA is twice as wide, which pays while a narrow one
+// does not fill the tensor pipe; the accumulators then take 4 columns of TMEM
+// per token, which caps it at 96. n follows the rows in the tile in steps of
+// the boxes they are loaded in: 8 where small tiles have at most 16 rows (every
+// column beyond costs energy, and a long run of decode steps is held back by
+// the power limit), else 32.
+__host__ __device__ constexpr bool few_rows(int bn, int ncols) { return bn <= 64 && ncols <= 16; }
 __host__ __device__ constexpr int side_by_side(int bn, int ncols) {
-  const int n32 = (ncols + 31) & ~31;
-  return bn <= 64 ? n32 : (n32 <= 96 ? n32 : 0);
+  const int n = few_rows(bn, ncols) ? (ncols + 7) & ~7 : (ncols + 31) & ~31;
+  return bn <= 64 || n <= 96 ? n : 0;
 }
 
 enum { kTypeBf16 = 0, kTypeF16 = 1, kTypeF32 = 2, kTypeE4m3 = 3 };

@@ -202,9 +202,9 @@ __device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tile
   e.tile = tile0 + nt;
   e.m0 = mt * (SWIGLU ? BM : 2 * BM);
   e.m1 = SWIGLU ? e.m0 : (e.m0 + BM < p.M ? e.m0 + BM : -1);
-  const int n32 = C::FP4 ? 0 : side_by_side(C::BN, e.ncols);
-  e.both = n32 > 0;
-  e.n = n32 ? n32 : (e.ncols + 15) & ~15;
+  const int n = C::FP4 ? 0 : side_by_side(C::BN, e.ncols);
+  e.both = n > 0;
+  e.n = n ? n : (e.ncols + 15) & ~15;
   const int KB = p.K / 128;
   e.kb0 = 0;
   e.kb1 = KB;
@@ -343,12 +343,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         const uint8_t* fa = p.sfa + (static_cast<size_t>(e.group) * pairs + e.m0 / (SWIGLU ? BM : 2 * BM)) * KB * 1024;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
         // Rows side by side come in 32-row boxes; where a small tile has at most
-        // 16, in 8-row boxes (the columns behind them keep what an earlier stage
-        // left, and are not stored): 64 rows instead of 16 per stage took a
-        // tenth of a one-token FFN.
-        const bool few = BN <= 64 && e.ncols <= 16;
-        const int step = few ? 8 : 32, xrows = few ? (e.ncols + 7) & ~7 : e.n;
-        const uint32_t xbytes = e.both ? 2 * xrows * 128 : C::B_BYTES;
+        // 16, in 8-row boxes: 64 rows instead of 16 per stage took a tenth of a
+        // one-token FFN.
+        const bool few = few_rows(BN, e.ncols);
+        const int step = few ? 8 : 32;
+        const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
         auto load_w = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES;
           uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
@@ -365,7 +364,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           const int kx = FP4 ? kb * 64 : kb * 128;
           if (!FP4 && e.both) {
             const CUtensorMap* tm = few ? &tm_x : &tm_x32;
-            for (int s = 0; s < xrows; s += step) {
+            for (int s = 0; s < e.n; s += step) {
               tma_load_2d(st + s * 128, tm, &full[stage], kx, e.row0 + s, pol_x);
               tma_load_2d(st + (e.n + s) * 128, tm, &full[stage], kx, p.P + e.row0 + s, pol_x);
             }

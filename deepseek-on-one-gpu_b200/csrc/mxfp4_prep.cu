@@ -190,10 +190,10 @@ struct SfSpot {
 template <int TILE>
 __device__ __forceinline__ SfSpot sf_spot(int tile0, int count, int local, int KB) {
   const int t = local / TILE, c = local - t * TILE;
-  const int n32 = side_by_side(TILE, min(TILE, count - t * TILE));
+  const int n = side_by_side(TILE, min(TILE, count - t * TILE));
   const long long base = static_cast<long long>(tile0 + t) * KB * tile_atoms(TILE) * 128;
   auto word = [](int col) { return (col >> 7) * 128 + (col & 31) * 4 + ((col >> 5) & 3); };
-  return {base + word(c), n32 ? base + word(c + n32) : -1};
+  return {base + word(c), n ? base + word(c + n) : -1};
 }
 
 // Split kernels: blocks of kSplitThreads, 16 columns of a row per thread.
