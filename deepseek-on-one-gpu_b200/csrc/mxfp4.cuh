@@ -61,8 +61,18 @@ struct Groups {
   int rows;
 };
 
+// What the tables of a few rows are made from: a product with a small tile
+// builds them for itself (`tiles` up to 64), so that it can start on its
+// weights while the kernel that splits the rows still runs.
+struct TableSource {
+  const int64_t* idx;      // a routing's pairs, or
+  const int32_t* offsets;  // segments of g.rows rows, or neither
+  int pairs, n_routed, shared, tokens;
+};
+
 struct GemmArgs {
   Groups g;
+  TableSource own;
   int M;                 // features of one weight matrix
   int K;
   int P;                 // first lo row of the split activations

@@ -404,6 +404,8 @@ int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int32_t rows, 
   uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
   __nv_bfloat16* clear = clear_rest ? a.y : nullptr;
   if (rows <= mx::kSegmentRows) {
+    a.g.rows = rows;
+    a.own.offsets = offsets;
     MX_CUDA(mx::launch_segments_split(rx, row_stride, rows, in_features, offsets, n_experts, L.tile, counts, row_start,
                                       tile_start, a.next, device_status, xq, sf, clear, out_features, s));
   } else {
@@ -473,6 +475,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
           *tile_start = at<int32_t>(workspace, L.tile_start);
   uint8_t *xq = at<uint8_t>(workspace, L.xq), *sf = at<uint8_t>(workspace, L.sf);
   if (tokens * top_k <= mx::kRoutePairs) {
+    a.own = {topk_idx, nullptr, tokens * top_k, E, shared, tokens};
     MX_CUDA(mx::launch_route_split(x, row_stride, tokens, H, topk_idx, top_k, E, shared, L.tile, L.P, counts, row_start,
                                    tile_start, a.next, pos, xq, sf, s));
   } else {

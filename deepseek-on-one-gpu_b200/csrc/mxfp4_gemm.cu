@@ -88,7 +88,9 @@ struct Cfg {
   static constexpr int MISC_OFF = BAR_OFF + 8 * NUM_BARS;
   static constexpr int PLAN_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
   static constexpr int TAB_OFF = PLAN_OFF + RING * static_cast<int>(sizeof(Unit));
-  static constexpr int SMEM = TAB_OFF + (FP4 ? 0 : 4 * (kMaxGroups + 1)) + 1024;  // group table; kind::mxf4 has none
+  static constexpr bool OWN = !FP4 && BN <= 64;  // builds the group tables of a few rows itself
+  // Group tables: kind::mxf4 has none.
+  static constexpr int SMEM = TAB_OFF + (FP4 ? 0 : OWN ? 4 * (3 * kMaxGroups + 1) : 4 * (kMaxGroups + 1)) + 1024;
   static_assert(SMEM <= 232448, "shared memory");
   static_assert(STAGES * OP_BYTES >= BN * 2 * BM * 4, "a K part's sums");
   static_assert(OP_BYTES % 1024 == 0, "operand alignment");
@@ -174,9 +176,79 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// `tiles` is the tile_start table (in shared memory), unused without groups.
+// The planner's group tables in shared memory: tile_start, and where the kernel
+// builds its own also counts and row_start. Unused without groups.
+template <class C>
+struct Tables {
+  int* tiles;  // [kMaxGroups + 1]
+  __device__ __forceinline__ int* counts() const { return tiles + kMaxGroups + 1; }
+  __device__ __forceinline__ int* starts() const { return counts() + kMaxGroups; }
+};
+
+// One warp, from a routing or from offsets: what route_split_kernel and
+// segments_split_kernel compute, lane l for groups 16 l and up.
+template <class C>
+__device__ __forceinline__ void build_tables(const Tables<C>& t, const GemmArgs& p, int lane) {
+  constexpr int GL = kMaxGroups / 32;
+  int *cnt = t.counts(), *start = t.starts();
+  const TableSource& o = p.own;
+  if (o.idx) {
+    for (int g = lane; g < kMaxGroups; g += 32) cnt[g] = 0;
+    __syncwarp();
+    for (int i = lane; i < o.pairs; i += 32) {
+      const int64_t e = __ldg(o.idx + i);
+      if (e >= 0 && e < o.n_routed) atomicAdd(&cnt[e + o.shared], 1);
+    }
+    __syncwarp();
+    if (o.shared && lane == 0) cnt[0] = o.tokens;
+    __syncwarp();
+  } else {
+    const int R = p.g.rows, first = min(max(__ldg(o.offsets), 0), R);
+    int end[GL], top = first;
+#pragma unroll
+    for (int j = 0; j < GL; ++j) {
+      const int g = GL * lane + j;
+      if (g < p.g.n) top = max(top, min(max(__ldg(o.offsets + g + 1), 0), R));
+      end[j] = top;
+    }
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, top, s);
+      if (lane >= s) top = max(top, a);
+    }
+    int before = __shfl_up_sync(0xffffffffu, top, 1);
+    if (lane == 0) before = first;
+#pragma unroll
+    for (int j = 0; j < GL; ++j) {
+      const int a = j ? max(before, end[j - 1]) : before;
+      start[GL * lane + j] = a;
+      cnt[GL * lane + j] = max(before, end[j]) - a;
+    }
+  }
+  int rows = 0, tiles = 0;
+  for (int j = 0; j < GL; ++j) {
+    const int c = cnt[GL * lane + j];
+    rows += c;
+    tiles += (c + C::BN - 1) / C::BN;
+  }
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, rows, s), b = __shfl_up_sync(0xffffffffu, tiles, s);
+    if (lane >= s) rows += a, tiles += b;
+  }
+  if (lane == 31) t.tiles[kMaxGroups] = tiles;
+  for (int j = GL - 1; j >= 0; --j) {
+    const int c = cnt[GL * lane + j];
+    rows -= c;
+    tiles -= (c + C::BN - 1) / C::BN;
+    if (o.idx) start[GL * lane + j] = rows;
+    t.tiles[GL * lane + j] = tiles;
+  }
+  __syncwarp();
+}
+
 template <class C, bool SWIGLU>
-__device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tiles) {
+__device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const Tables<C>& t, bool own) {
   Unit e;
   const int per = SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
   const int id = p.ksplit > 1 ? u / p.ksplit : u;
@@ -186,12 +258,12 @@ __device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tile
     int lo = 0, hi = p.g.n;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (tiles[mid] * per <= id) lo = mid; else hi = mid;
+      if (t.tiles[mid] * per <= id) lo = mid; else hi = mid;
     }
     g = lo;
-    rows = load_dep(p.g.counts + g);
-    row_start = load_dep(p.g.row_start + g);
-    tile0 = tiles[g];
+    rows = own ? t.counts()[g] : load_dep(p.g.counts + g);
+    row_start = own ? t.starts()[g] : load_dep(p.g.row_start + g);
+    tile0 = t.tiles[g];
   }
   ntiles = (rows + C::BN - 1) / C::BN;
   const int local = id - tile0 * per;
@@ -215,12 +287,6 @@ __device__ __forceinline__ Unit decode(int u, const GemmArgs& p, const int* tile
     e.kb1 = min(KB, static_cast<int>(static_cast<long long>(st) * (e.part + 1) / p.ksplit) * C::KB_STAGE);
   }
   return e;
-}
-
-__device__ __forceinline__ int unit_count(const GemmArgs& p, int bn, bool swiglu) {
-  const int per = swiglu ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM);
-  const int tiles = p.g.counts ? load_dep(p.g.tile_start + p.g.n) : (p.g.rows + bn - 1) / bn;
-  return tiles * per * p.ksplit;
 }
 
 // Four tokens' bf16 values of 32 features, packed by token pairs (p01: tokens 0
@@ -287,10 +353,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   tc_fence_after();
 
   launch_dependents();
-  // With group tables every role needs what earlier kernels of the chain
-  // wrote. Without, only the copies of the rows do: the producer waits, after
-  // it has started on the weights.
-  if (p.g.counts) dependency_wait();
+  // With group tables of an earlier kernel of the chain every role waits for
+  // it. Without, only the copies of the rows do: the producer waits, after it
+  // has started on the weights.
+  const bool own = C::OWN && (p.own.idx || p.own.offsets);
+  const bool early = !p.g.counts || own;
+  if (!early) dependency_wait();
   const uint32_t tmem = *s_tmem;
   const int KB = p.K / 128;
 
@@ -298,21 +366,31 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     // ------------------------------------------------------------- planner
     // The search for a unit's group walks a shared-memory copy of the table:
     // nine dependent global loads would be ~3 us before the first copy.
-    int* tiles = reinterpret_cast<int*>(smem + C::TAB_OFF);
-    const int total = unit_count(p, BN, SWIGLU);
-    if (p.g.counts)
-      for (int t = lane; t <= p.g.n; t += 32) tiles[t] = load_dep(p.g.tile_start + t);
-    __syncwarp();
+    const Tables<C> tab{reinterpret_cast<int*>(smem + C::TAB_OFF)};
+    int tiles = (p.g.rows + BN - 1) / BN;
+    if (p.g.counts) {
+      if (own) {
+        if constexpr (C::OWN) build_tables<C>(tab, p, lane);
+      } else {
+        for (int t = lane; t <= p.g.n; t += 32) tab.tiles[t] = load_dep(p.g.tile_start + t);
+        __syncwarp();
+      }
+      tiles = tab.tiles[p.g.n];
+    }
+    const int total = tiles * (SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM)) * p.ksplit;
     if (lane == 0) {
       int u = blockIdx.x;
       for (int i = 0;; ++i) {
         Unit e;
         e.ncols = 0;  // the end
-        if (u < total) e = decode<C, SWIGLU>(u, p, tiles);
+        if (u < total) e = decode<C, SWIGLU>(u, p, tab, own);
         const int ri = i % RING;
         if (!mbar_wait(&uempty[ri], ((i / RING) & 1) ^ 1, p.status, kDevTimeoutProducer, s_abort)) break;
         plan[ri] = e;
         mbar_arrive(&ufull[ri]);
+        // Also in a CTA without a unit, so that this kernel does not end before
+        // its predecessor; and before p.next, which an earlier kernel clears.
+        if (i == 0 && own) dependency_wait();
         if (u >= total) break;
         // Units of ragged groups cost between 64 and 160 columns: handed out
         // as CTAs become free. (In fixed turns the slowest of 148 CTAs got
@@ -376,7 +454,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
                     fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512, &full[stage]);
         };
         int kb = e.kb0;
-        if (i == 0 && !p.g.counts) {
+        if (i == 0 && early) {
           // The first stages' weights are on their way while the kernel before
           // this one still prepares the rows.
           const int n = min(STAGES, (e.kb1 - kb + C::KB_STAGE - 1) / C::KB_STAGE);
