@@ -24,10 +24,22 @@
 //              its TMEM columns (tcgen05.cp) and issues the MMAs behind them
 //   warp 3     unit planner, a shared-memory ring of decoded units
 //   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 8-column chunks
+// Two issuing threads because one that waits on a barrier between its batches
+// leaves the tensor pipe idle: one thread for both tiles ran 512 rows over 256
+// experts 5% slower, a T=4096 product 1%. Sharing A between the hi and the lo MMA
+// (collector::a) needs one thread and gave back half a percent: not kept.
 // TMEM: two halves of accumulator columns, then one set of scale columns per
 // stage (a stage's scales are overwritten only after its MMAs released it). A
 // unit that fits a half alternates between them, so its epilogue overlaps the
 // next unit's MMAs; a larger one takes both.
+//
+// What bounds it. Few rows: the weights' bytes from HBM (512 rows over 256
+// experts of 7168 x 2048: 255 us, 6.75 TB/s; gate and up of a 64-token FFN 570 us,
+// 6.1 TB/s). Many: the tensor pipe under the power limit. T=4096 x 7168 x 18432
+// takes 700 us (1545 TFLOP/s in useful operations; the SM clock falls to 1.39 GHz
+// with the pipe 87% busy), and 4-bit rows x 18432 x 7168 212 us (5.1 PFLOP/s). A
+// stage's copies take ~2000 cycles from issue to use; three stages of 76 KB hide
+// them at 1280 MMA cycles a stage.
 #include "common.cuh"
 #include "mxfp4.cuh"
 

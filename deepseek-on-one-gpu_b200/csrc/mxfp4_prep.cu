@@ -62,8 +62,8 @@ __global__ void __launch_bounds__(kMaxGroups) segments_kernel(const int32_t* __r
 // CTAs: each warp owns a contiguous range of pairs, counts it, and after the
 // scans over warps, CTAs (through shared memory) and groups walks it again in
 // order; lanes of one step that hold the same expert are ranked by lane. The
-// row of a pair therefore depends on the routing only. One CTA took 63 us for
-// 32768 pairs.
+// row of a pair therefore depends on the routing only. 32768 pairs: 15.5 us,
+// latency of the chain of scans; one CTA took 63.
 constexpr int kPlanWarps = 32;
 constexpr int kPlanCtas = 8;
 
@@ -270,7 +270,7 @@ constexpr int MAXR = 9;  // rows of a token: the shared expert's and top_k <= 8
 // The place of a row is found by one thread each: for a routing the group is
 // known from idx, for segments it is searched in a shared-memory copy of their
 // starts (nine dependent global loads took twice as long as the split itself:
-// 322 us for 32768 rows of 7168).
+// 322 us for 32768 rows of 7168; 165 us now, 5.7 TB/s of what is read and written).
 template <int TILE, int R>
 __global__ void __launch_bounds__(kSplitThreads) split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride, int T,
                                                     int K, const Groups g, const int64_t* __restrict__ idx,
@@ -501,6 +501,8 @@ segments_split_kernel(const __nv_bfloat16* __restrict__ x, long long row_stride,
   split_row(q, K, rows, 1, s_row, s_spot, tile_atoms(TILE), xq, sf);
 }
 
+// Bound by memory: the token's rows are loaded together and summed in fp32 in
+// top-k order. 4096 tokens x 9 rows of 7168: 88 us, 6.7 TB/s.
 __global__ void __launch_bounds__(256) combine_kernel(const __nv_bfloat16* y, int T, int H,
                                                       const int32_t* pos, const float* __restrict__ w,
                                                       int top_k, int shared, float scale,

@@ -17,7 +17,9 @@
 // are shared by as many numbers as the registers allow; codes leave in 4- or
 // 8-byte words, contiguous over the warp. Row and matrix indexes come from
 // multiplications (FastDiv): two integer divisions per thread cost more than
-// the quantisation.
+// the quantisation. 7169 x 18432 in fp32: 90 us, 6.7 TB/s; 32 x 2048 x 7168 in
+// e4m3: 231 us, 3.1 TB/s, bound by issue (two directed products and a select per
+// number for the exact rounding).
 #include "common.cuh"
 #include "mxfp4.cuh"
 
@@ -258,7 +260,8 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
 }
 
 // A thread takes 8 codes at a time, 4 such groups a block's width apart with
-// their loads together. code * 2^(b - 127) is exact in fp32 and bf16.
+// their loads together. code * 2^(b - 127) is exact in fp32 and bf16. Bound by
+// the stores: 470 M numbers to bf16 in 213 us, 5.6 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, uint64_t units,
@@ -294,8 +297,8 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restr
 // Scales to atoms. One block: one atom's 128 rows and up to KC K blocks, read
 // along the rows (4 KC contiguous bytes each), turned in shared
 // memory and written as whole atoms. Words of an atom that belong to no row are
-// zero. Memory-bound in principle (118 MB in and out for 256 matrices of 2048 x
-// 7168); read word by word in atom order it was eight times over-read, 148 us.
+// zero. 256 matrices of 7168 x 2048 (118 MB in and out): 74 us; read word by
+// word in atom order every sector came in eight times, 148 us.
 template <int KC>
 __global__ void __launch_bounds__(256) tile_scales_kernel(const uint32_t* __restrict__ scales, int N, int KB, int tile,
                                                           int tiles, int atoms, uint32_t* __restrict__ out) {
