@@ -39,13 +39,11 @@ constexpr int tile_atoms(int bn) { return bn > 64 ? 2 : 1; }
 // MMA of N = 2 n (hi columns then lo columns), or 0 where hi and lo are two
 // MMAs. Side by side the MMA is twice as wide, which pays while a narrow one
 // does not fill the tensor pipe; the accumulators then take 4 columns of TMEM
-// per token, which caps it at 96. n follows the rows in the tile in steps of
-// the boxes they are loaded in: 8 where small tiles have at most 16 rows (every
-// column beyond costs energy, and a long run of decode steps is held back by
-// the power limit), else 32.
-__host__ __device__ constexpr bool few_rows(int bn, int ncols) { return bn <= 64 && ncols <= 16; }
+// per token, which caps it at 96. n follows the rows in the tile in steps of 8:
+// every column beyond costs energy, and a long run is held back by the power
+// limit.
 __host__ __device__ constexpr int side_by_side(int bn, int ncols) {
-  const int n = few_rows(bn, ncols) ? (ncols + 7) & ~7 : (ncols + 31) & ~31;
+  const int n = (ncols + 7) & ~7;
   return bn <= 64 || n <= 96 ? n : 0;
 }
 
@@ -204,10 +202,10 @@ cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* 
 // K split of a single-group product of `units` (feature tile pair, token tile)
 // pairs on the current device.
 int pick_ksplit(bool fp4, int tile, int units, int kblocks);
-// x: rows in boxes of the token tile (bf16 activations in tiles up to 64: of 8),
-// x32: of 32.
+// x: rows in boxes of the token tile, x32 and x8: of 32 and 8.
 cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
-                        const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s);
+                        const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a, int tile, int grid,
+                        cudaStream_t s);
 
 }  // namespace mx
 }  // namespace dsmoe

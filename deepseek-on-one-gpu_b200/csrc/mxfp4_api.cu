@@ -202,7 +202,7 @@ int check_weight(const char* what, const void* codes, const void* atoms) {
 // A product with bf16 activations (split rows xq) or, with fp4, MXFP4 rows.
 int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, const uint8_t* x, mx::GemmArgs& a,
              int tile, long long max_units, cudaStream_t s) {
-  CUtensorMap m_w0, m_w1, m_x, m_x32;
+  CUtensorMap m_w0, m_w1, m_x, m_x32, m_x8;
   const uint64_t wrows = static_cast<uint64_t>(mats) * a.M;
   const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   int r;
@@ -211,20 +211,21 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
     if ((r = make_tma_map(&m_w0, u8, kb, w0, kb, wrows, 128, 128))) return r;
     m_w1 = m_w0;
     if ((r = make_tma_map(&m_x, u8, kb, x, kb, a.P, 128, tile))) return r;
-    m_x32 = m_x;
+    m_x32 = m_x8 = m_x;
   } else {
     const auto u4 = CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B;
     if ((r = make_tma_map(&m_w0, u4, a.K / 2, w0, a.K, wrows, 128, 128))) return r;
     m_w1 = m_w0;
     if (w1 != w0 && (r = make_tma_map(&m_w1, u4, a.K / 2, w1, a.K, wrows, 128, 128))) return r;
     const uint64_t rows = 2 * static_cast<uint64_t>(a.P);
-    // Tiles up to 64 rows never load as one box: their first map has 8-row boxes.
-    if ((r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile <= 64 ? 8 : tile))) return r;
     if ((r = make_tma_map(&m_x32, u8, a.K, x, a.K, rows, 128, 32))) return r;
+    if ((r = make_tma_map(&m_x8, u8, a.K, x, a.K, rows, 128, 8))) return r;
+    m_x = m_x32;  // tiles up to 64 rows never load as one box
+    if (tile > 64 && (r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
   }
   // A split tile is a cluster, one unit per CTA; otherwise persistent CTAs.
   const int g = a.ksplit > 1 ? static_cast<int>(max_units) : gemm_grid();
-  MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, a, tile, max_units < g ? static_cast<int>(max_units) : g, s));
+  MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, m_x8, a, tile, max_units < g ? static_cast<int>(max_units) : g, s));
   return DSMOE_OK;
 }
 

@@ -321,7 +321,7 @@ template <class C, bool SWIGLU>
 __global__ void __launch_bounds__(THREADS, 1)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant__ CUtensorMap tm_w1,
                const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
-               const GemmArgs p) {
+               const __grid_constant__ CUtensorMap tm_x8, const GemmArgs p) {
   constexpr bool FP4 = C::FP4;
   constexpr int BN = C::BN, STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -358,6 +358,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
     prefetch_tmap(&tm_w1);
     prefetch_tmap(&tm_x);
     prefetch_tmap(&tm_x32);
+    prefetch_tmap(&tm_x8);
   }
   if (warp == 1) tmem_alloc(s_tmem, 512);
   tc_fence_before();
@@ -432,11 +433,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         const int pairs = SWIGLU ? p.M / BM : (p.M + 2 * BM - 1) / (2 * BM);
         const uint8_t* fa = p.sfa + (static_cast<size_t>(e.group) * pairs + e.m0 / (SWIGLU ? BM : 2 * BM)) * KB * 1024;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
-        // Rows side by side come in 32-row boxes; where a small tile has at most
-        // 16, in 8-row boxes: 64 rows instead of 16 per stage took a tenth of a
-        // one-token FFN.
-        const bool few = few_rows(BN, e.ncols);
-        const int step = few ? 8 : 32;
         const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
         auto load_w = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES;
@@ -453,8 +449,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);
           const int kx = FP4 ? kb * 64 : kb * 128;
           if (!FP4 && e.both) {
-            const CUtensorMap* tm = few ? &tm_x : &tm_x32;
-            for (int s = 0; s < e.n; s += step) {
+            // 32-row boxes and 8-row boxes for the rest (64 rows instead of 16
+            // per stage took a tenth of a one-token FFN).
+            for (int s = 0, step; s < e.n; s += step) {
+              step = e.n - s >= 32 ? 32 : 8;
+              const CUtensorMap* tm = step == 32 ? &tm_x32 : &tm_x8;
               tma_load_2d(st + s * 128, tm, &full[stage], kx, e.row0 + s, pol_x);
               tma_load_2d(st + (e.n + s) * 128, tm, &full[stage], kx, p.P + e.row0 + s, pol_x);
             }
@@ -783,13 +782,13 @@ cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int
 
 template <class C, bool SWIGLU>
 cudaError_t launch(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& x32,
-                   const GemmArgs& a, int grid, cudaStream_t s) {
+                   const CUtensorMap& x8, const GemmArgs& a, int grid, cudaStream_t s) {
   int dev = 0;
   const cudaError_t e = prepare<C, SWIGLU>(&dev);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg = config<C>(grid, s, at, a.ksplit);
-  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<C, SWIGLU>, w0, w1, x, x32, a);
+  return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<C, SWIGLU>, w0, w1, x, x32, x8, a);
 }
 
 // Clusters of `split` CTAs that run at the same time on the current device.
@@ -824,26 +823,27 @@ int pick_ksplit(bool fp4, int tile, int units, int kblocks) {
 }
 
 cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
-                        const CUtensorMap& x32, const GemmArgs& a, int tile, int grid, cudaStream_t s) {
+                        const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a, int tile, int grid,
+                        cudaStream_t s) {
   if (fp4) {
     switch (tile) {
-      case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
-      case 160: return launch<Cfg<true, 160, 4>, false>(w0, w1, x, x32, a, grid, s);
+      case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
+      case 160: return launch<Cfg<true, 160, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
       default: return cudaErrorInvalidValue;
     }
   }
   switch (tile) {
     case 32:
-      return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, a, grid, s)
-                    : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, a, grid, s);
+      return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 64:
-      return swiglu ? launch<Cfg<false, 64, 4>, true>(w0, w1, x, x32, a, grid, s)
-                    : launch<Cfg<false, 64, 4>, false>(w0, w1, x, x32, a, grid, s);
+      return swiglu ? launch<Cfg<false, 64, 4>, true>(w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 64, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 128:  // single-group products only
-      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 128, 3>, false>(w0, w1, x, x32, a, grid, s);
+      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 128, 3>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 160:
-      return swiglu ? launch<Cfg<false, 160, 3>, true>(w0, w1, x, x32, a, grid, s)
-                    : launch<Cfg<false, 160, 3>, false>(w0, w1, x, x32, a, grid, s);
+      return swiglu ? launch<Cfg<false, 160, 3>, true>(w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 160, 3>, false>(w0, w1, x, x32, x8, a, grid, s);
     default: return cudaErrorInvalidValue;
   }
 }
