@@ -23,7 +23,6 @@ is no CPU path and no backward: tensors that require a gradient are rejected.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import threading
 
@@ -74,12 +73,17 @@ def stream_handle(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch; free when it already is."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _call(device: torch.device, name: str, *args) -> None:
+    """One library call on ``device``'s current stream (the last argument),
+    with the device current."""
+    fn = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_handle(device))
+    if rc:
+        check(rc, name)
 
 
 def _require(what: str, *tensors: torch.Tensor) -> None:
@@ -127,10 +131,8 @@ def _quantize_into(x: torch.Tensor, scale_inv: torch.Tensor | None, codes: torch
     fp8 = x.dtype == torch.float8_e4m3fn
     x2 = _rows(x)
     per = x.shape[-2] if fp8 else 1
-    with _on(x.device):
-        check(lib().dsmoe_mxfp4_quantize(ptr(x2), _DTYPES[x.dtype], x2.shape[0], K, x2.stride(0), ptr(scale_inv),
-                                         max(per, 1), ptr(codes), ptr(scales), stream_handle(x.device)),
-              "dsmoe_mxfp4_quantize")
+    _call(x.device, "dsmoe_mxfp4_quantize", x2.data_ptr(), _DTYPES[x.dtype], x2.shape[0], K, x2.stride(0),
+          ptr(scale_inv), max(per, 1), codes.data_ptr(), scales.data_ptr())
 
 
 def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -145,9 +147,9 @@ def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tu
     _require("mxfp4_quantize", x, scale_inv)
     if x.dtype not in _DTYPES:
         raise TypeError("mxfp4_quantize expects bf16, fp16, fp32 or e4m3")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % BLOCK:
+    *lead, K = x.shape or (0,)
+    if K == 0 or K % BLOCK:
         raise ValueError(f"the last dimension must be a multiple of {BLOCK}")
-    K = x.shape[-1]
     if x.dtype == torch.float8_e4m3fn:
         if scale_inv is None or scale_inv.dtype != torch.float32:
             raise TypeError("e4m3 needs fp32 scale_inv")
@@ -159,8 +161,8 @@ def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tu
         scale_inv = scale_inv.contiguous()
     elif scale_inv is not None:
         raise TypeError("scale_inv goes with e4m3 only")
-    codes = torch.empty(*x.shape[:-1], K // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-1], K // BLOCK, dtype=torch.uint8, device=x.device)
+    codes = torch.empty(*lead, K // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*lead, K // BLOCK, dtype=torch.uint8, device=x.device)
     if x.numel():
         _quantize_into(x, scale_inv, codes, scales)
     return codes, scales
@@ -186,16 +188,14 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
     codes, scales = _dense(codes, 4), scales.contiguous()
     out = torch.empty(*codes.shape[:-1], K, dtype=out_dtype, device=codes.device)
     if out.numel():
-        with _on(codes.device):
-            check(lib().dsmoe_mxfp4_dequantize(ptr(codes), ptr(scales), scales.numel(), _DTYPES[out_dtype], ptr(out),
-                                               stream_handle(codes.device)), "dsmoe_mxfp4_dequantize")
+        _call(codes.device, "dsmoe_mxfp4_dequantize", codes.data_ptr(), scales.data_ptr(), scales.numel(),
+              _DTYPES[out_dtype], out.data_ptr())
     return out
 
 
 def _pack_scales(scales: torch.Tensor, mats: int, out_features: int, in_features: int, atoms: torch.Tensor) -> None:
-    with _on(scales.device):
-        check(lib().dsmoe_mxfp4_scale_atoms(ptr(scales), mats, out_features, in_features, ptr(atoms),
-                                            stream_handle(scales.device)), "dsmoe_mxfp4_scale_atoms")
+    _call(scales.device, "dsmoe_mxfp4_scale_atoms", scales.data_ptr(), mats, out_features, in_features,
+          atoms.data_ptr())
 
 
 def _interleave(gate: torch.Tensor, up: torch.Tensor, mats: int, out_features: int, in_features: int) -> torch.Tensor:
@@ -229,6 +229,8 @@ class MXFP4Weight:
         self.codes = _dense(codes, 32)
         self.atoms = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.status = _device_status(self.device)
+        self._ptrs = self.codes.data_ptr(), self.atoms.data_ptr(), self.status.data_ptr()
+        self._need: dict[tuple, int] = {}  # scratch bytes by call form and rows
         _pack_scales(_dense(scales, 4), mats, self.out_features, K, self.atoms)
 
     @classmethod
@@ -236,6 +238,17 @@ class MXFP4Weight:
         """From a bf16, fp16 or fp32 weight, or the checkpoint's e4m3 weight
         with its ``weight_scale_inv``."""
         return cls(*mxfp4_quantize(weight, scale_inv))
+
+    def _scratch(self, form: str, rows: int) -> torch.Tensor:
+        need = self._need.get((form, rows))
+        if need is None:
+            sizes = (rows, self.in_features, self.out_features) + (() if self.experts is None else (self.experts,))
+            with torch.cuda.device(self.device):
+                need = getattr(lib(), form + "_workspace_size")(*sizes)
+            if len(self._need) >= 1024:
+                self._need.clear()
+            self._need[form, rows] = need
+        return self.codes.new_empty(need)
 
     @property
     def nbytes(self) -> int:
@@ -249,8 +262,10 @@ def _check_weight(what: str, w: MXFP4Weight, stacked: bool) -> None:
         raise ValueError(f"{what} expects " + ("a stack of experts" if stacked else "a single weight (out, in)"))
 
 
-def _check_x(what: str, x: torch.Tensor, K: int, *others: torch.Tensor) -> None:
+def _check_x(what: str, x: torch.Tensor, K: int, device: torch.device, *others: torch.Tensor) -> None:
     _require(what, x, *others)
+    if x.device != device:
+        raise RuntimeError(f"{what}: activations on {x.device}, weights on {device}")
     if x.dtype != torch.bfloat16:
         raise TypeError(f"{what} expects bf16 activations")
     if x.dim() < 1 or x.shape[-1] != K:
@@ -261,16 +276,16 @@ def mxfp4_linear(x: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
     """``bf16(x @ W.T)`` for bf16 ``x`` [..., in], fp32 sums. A row with an
     infinity or a NaN comes out as NaN."""
     _check_weight("mxfp4_linear", weight, False)
-    _check_x("mxfp4_linear", x, weight.in_features, weight.codes)
+    K, N = weight.in_features, weight.out_features
+    _check_x("mxfp4_linear", x, K, weight.device)
     x2 = _rows(x)
-    T, K, N = x2.shape[0], weight.in_features, weight.out_features
+    T = x2.shape[0]
     out = torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device)
     if T:
-        with _on(x.device):
-            ws = _scratch(lib().dsmoe_mxfp4_linear_workspace_size(T, K, N), x.device)
-            check(lib().dsmoe_mxfp4_linear(ptr(x2), x2.stride(0), T, K, N, ptr(weight.codes), ptr(weight.atoms),
-                                           ptr(out), ptr(ws), ws.numel(), ptr(weight.status),
-                                           stream_handle(x.device)), "dsmoe_mxfp4_linear")
+        codes, atoms, status = weight._ptrs
+        ws = weight._scratch("dsmoe_mxfp4_linear", T)
+        _call(weight.device, "dsmoe_mxfp4_linear", x2.data_ptr(), x2.stride(0), T, K, N, codes, atoms, out.data_ptr(),
+              ws.data_ptr(), ws.numel(), status)
     return out
 
 
@@ -279,7 +294,8 @@ def mxfp4_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: MXFP4Weight)
     [..., in/2] and scales [..., in/32]), fp32 sums."""
     _check_weight("mxfp4_matmul", weight, False)
     K = _check_pair("mxfp4_matmul", codes, scales)
-    _require("mxfp4_matmul", codes, weight.codes)
+    if codes.device != weight.device:
+        raise RuntimeError(f"mxfp4_matmul: activations on {codes.device}, weights on {weight.device}")
     if K != weight.in_features:
         raise ValueError(f"mxfp4_matmul: activations have {K} features, the weight {weight.in_features}")
     shape, N = codes.shape[:-1], weight.out_features
@@ -287,11 +303,10 @@ def mxfp4_matmul(codes: torch.Tensor, scales: torch.Tensor, weight: MXFP4Weight)
     T = c2.numel() // c2.shape[-1]
     out = torch.empty(*shape, N, dtype=torch.bfloat16, device=codes.device)
     if T:
-        with _on(codes.device):
-            ws = _scratch(lib().dsmoe_mxfp4_matmul_workspace_size(T, K, N), codes.device)
-            check(lib().dsmoe_mxfp4_matmul(ptr(c2), ptr(s2), T, K, N, ptr(weight.codes), ptr(weight.atoms), ptr(out),
-                                           ptr(ws), ws.numel(), ptr(weight.status), stream_handle(codes.device)),
-                  "dsmoe_mxfp4_matmul")
+        wc, wa, status = weight._ptrs
+        ws = weight._scratch("dsmoe_mxfp4_matmul", T)
+        _call(weight.device, "dsmoe_mxfp4_matmul", c2.data_ptr(), s2.data_ptr(), T, K, N, wc, wa, out.data_ptr(),
+              ws.data_ptr(), ws.numel(), status)
     return out
 
 
@@ -303,7 +318,7 @@ def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Te
     segment are zero in a new output and left as they are in ``out`` (dense
     bf16 [R, out], which must not overlap ``x``)."""
     _check_weight("mxfp4_grouped_linear", weight, True)
-    _check_x("mxfp4_grouped_linear", x, weight.in_features, offsets, out, weight.codes)
+    _check_x("mxfp4_grouped_linear", x, weight.in_features, weight.device, offsets, out)
     if x.dim() != 2:
         raise ValueError("mxfp4_grouped_linear expects (rows, in) activations")
     if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() != weight.experts + 1:
@@ -316,13 +331,10 @@ def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Te
         raise ValueError(f"out must be a dense, 16-byte aligned bf16 tensor ({R}, {N})")
     if R:
         x2, off = _rows(x), offsets.contiguous()
-        with _on(x.device):
-            need = lib().dsmoe_mxfp4_grouped_linear_workspace_size(R, K, N, weight.experts)
-            ws = _scratch(need, x.device)
-            check(lib().dsmoe_mxfp4_grouped_linear(ptr(x2), x2.stride(0), R, K, N, weight.experts, ptr(off),
-                                                   ptr(weight.codes), ptr(weight.atoms), ptr(out), int(clear),
-                                                   ptr(ws) or None, ws.numel(), ptr(weight.status),
-                                                   stream_handle(x.device)), "dsmoe_mxfp4_grouped_linear")
+        codes, atoms, status = weight._ptrs
+        ws = weight._scratch("dsmoe_mxfp4_grouped_linear", R)
+        _call(weight.device, "dsmoe_mxfp4_grouped_linear", x2.data_ptr(), x2.stride(0), R, K, N, weight.experts,
+              off.data_ptr(), codes, atoms, out.data_ptr(), int(clear), ws.data_ptr() or None, ws.numel(), status)
     return out
 
 
@@ -407,7 +419,7 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     rounded to bf16. An id outside the routed experts adds nothing."""
     if not isinstance(experts, MXFP4Experts):
         raise TypeError("mxfp4_moe expects MXFP4Experts")
-    _check_x("mxfp4_moe", hidden, experts.hidden, topk_idx, topk_w, experts.gate_codes)
+    _check_x("mxfp4_moe", hidden, experts.hidden, experts.device, topk_idx, topk_w)
     if topk_idx.dtype != torch.int64 or topk_w.dtype != torch.float32:
         raise TypeError("mxfp4_moe expects int64 indices and fp32 weights")
     lead = tuple(hidden.shape[:-1])
@@ -419,12 +431,10 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     out = torch.empty(*lead, H, dtype=torch.bfloat16, device=hidden.device)
     if T:
         idx, w = topk_idx.contiguous(), topk_w.contiguous()
-        with _on(hidden.device):
-            ws = _scratch(lib().dsmoe_mxfp4_moe_workspace_size(T, H, experts.inter, experts.n_routed,
-                                                               int(experts.shared), K), hidden.device)
-            check(lib().dsmoe_mxfp4_moe(ptr(x2), x2.stride(0), T, ctypes.byref(experts.desc), ptr(idx), ptr(w), K,
-                                        float(scale), ptr(out), ptr(ws) or None, ws.numel(), ptr(experts.status),
-                                        stream_handle(hidden.device)), "dsmoe_mxfp4_moe")
+        ws = _scratch(lib().dsmoe_mxfp4_moe_workspace_size(T, H, experts.inter, experts.n_routed, int(experts.shared),
+                                                           K), hidden.device)
+        _call(experts.device, "dsmoe_mxfp4_moe", x2.data_ptr(), x2.stride(0), T, experts.desc, idx.data_ptr(),
+              w.data_ptr(), K, float(scale), out.data_ptr(), ws.data_ptr() or None, ws.numel(), ptr(experts.status))
     return out
 
 
@@ -432,18 +442,15 @@ def moe_forward(x: torch.Tensor, gate_weight: torch.Tensor, bias: torch.Tensor |
                 experts: MXFP4Experts) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``moe_block``'s work on MXFP4 experts: dense bf16 ``x`` [T, hidden] ->
     output, routing indices and weights. Scratch is private to the call."""
-    _check_x("moe_forward", x, experts.hidden, gate_weight, bias, experts.gate_codes)
+    _check_x("moe_forward", x, experts.hidden, experts.device, gate_weight, bias)
     cfg = _lib.moe_config(config)
     T, K = x.shape[0], cfg.top_k
     out = torch.empty_like(x)
     idx = torch.empty(T, K, dtype=torch.int64, device=x.device)
     w = torch.empty(T, K, dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        ws = _scratch(lib().dsmoe_mxfp4_moe_forward_workspace_size(cfg, T), x.device)
-        check(lib().dsmoe_mxfp4_moe_forward(cfg, ptr(gate_weight), ptr(bias), ctypes.byref(experts.desc), ptr(x), T,
-                                            ptr(out), ptr(idx), ptr(w), ptr(ws) or None, ws.numel(),
-                                            ptr(experts.status), stream_handle(x.device)),
-              "dsmoe_mxfp4_moe_forward")
+    ws = _scratch(lib().dsmoe_mxfp4_moe_forward_workspace_size(cfg, T), x.device)
+    _call(experts.device, "dsmoe_mxfp4_moe_forward", cfg, ptr(gate_weight), ptr(bias), experts.desc, x.data_ptr(), T,
+          out.data_ptr(), idx.data_ptr(), w.data_ptr(), ws.data_ptr() or None, ws.numel(), ptr(experts.status))
     return out, idx, w
 
 
