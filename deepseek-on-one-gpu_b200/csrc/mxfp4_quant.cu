@@ -177,7 +177,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
 
 // The checkpoint's e4m3 with block scales. A block of 32 has one scale_inv s
 // (128 is a multiple of 32), so its largest product is that of its largest
-// number, and s 2^-e is exact: one rounded product per number.
+// number, and s 2^-e is exact: one rounded product per number. Products beyond
+// fp32 have their exponent taken 16 lower; a block of zeros keeps s as it is,
+// since s times its 2^127 may not be finite.
 __global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* __restrict__ x, uint32_t units,
                                                            FastDiv per_row, long long row_stride,
                                                            const float* __restrict__ scale_inv, FastDiv rows_per_mat,
@@ -202,8 +204,12 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* 
     for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(v[i]));
     m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
     const float wmax = __half2float(__hmax_nan(__low2half(m), __high2half(m)));
-    const uint32_t byte = scale_byte(__float_as_uint(mul_odd(wmax, s)) & 0x7fffffffu);
-    const float sc = s * __uint_as_float((254u - byte) << 23);
+    const bool large = fabsf(s) >= 0x1p64f;
+    const uint32_t amax = __float_as_uint(mul_odd(wmax, large ? s * 0x1p-16f : s)) & 0x7fffffffu;
+    uint32_t byte = scale_byte(amax);
+    if (large && amax && byte != 255) byte = min(byte + 16, 254u);  // from 2^55 on: far from scale_byte's lower end
+    float sc = s;
+    if (amax) sc *= __uint_as_float(byte < 254 ? (254u - byte) << 23 : 0x00400000u);  // 2^(127 - byte)
     uint32_t w[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {

@@ -181,7 +181,7 @@ def _check_pair(what: str, codes: torch.Tensor, scales: torch.Tensor) -> int:
 def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
                      out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The numbers MXFP4 data stands for, in bf16 or fp32 (exact) or fp16
-    (rounded; beyond its range infinite)."""
+    (rounded); beyond the type's range infinite."""
     K = _check_pair("mxfp4_dequantize", codes, scales)
     if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError("mxfp4_dequantize produces bf16, fp16 or fp32")
