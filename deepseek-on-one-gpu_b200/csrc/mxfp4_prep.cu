@@ -560,7 +560,10 @@ cudaError_t launch_route_plan(const int64_t* idx, int T, int top_k, int n_routed
                               cudaStream_t s) {
   const int smem = kPlanWarps * n_routed * 4;
   if (smem > 40 * 1024) {  // static shared memory counts against the default limit too
-    const cudaError_t e = cudaFuncSetAttribute(route_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // Always the largest: the limit is the function's, and another thread may be
+    // between its own setting and its launch.
+    const cudaError_t e = cudaFuncSetAttribute(route_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kPlanWarps * kMaxGroups * 4);
     if (e != cudaSuccess) return e;
   }
   // A CTA's warps take 32 pairs a step: a few steps each before more CTAs help.

@@ -75,3 +75,33 @@ def test_zeros_under_large_scales_add_nothing():
     assert bool((y == 64.0).all())
     y = mxfp4_matmul(*mxfp4_quantize(x), w)
     assert bool((y == 64.0).all())
+
+
+def test_threads_with_different_expert_counts():
+    """The planner's shared memory follows the number of experts; two threads
+    that launch it for 512 and for 400 do not disturb one another."""
+    g = gen(4)
+    sets = []
+    for n in (512, 400):
+        x = torch.randn(256, 128, generator=g, device=DEV).to(torch.bfloat16)
+        idx = torch.randint(0, n, (256, 8), generator=g, device=DEV)
+        sets.append((x, idx, torch.rand(256, 8, generator=g, device=DEV), experts(g, n, 128, 128, shared=False)))
+    want = [mxfp4_moe(*s) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    y = mxfp4_moe(*sets[i])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    bad.append(i)
+        except RuntimeError as e:
+            bad.append(str(e))
+
+    t = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [a.start() for a in t]
+    [a.join() for a in t]
+    assert not bad and mxfp4_status(DEV) == 0
