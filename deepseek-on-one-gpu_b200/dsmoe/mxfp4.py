@@ -220,18 +220,34 @@ class MXFP4Weight:
             raise ValueError("a weight is (out, in/2) or (experts, out, in/2)")
         self.in_features, self.out_features = K, codes.shape[-2]
         self.experts = codes.shape[0] if codes.dim() == 3 else None
-        self.device = codes.device
         mats = 1 if self.experts is None else self.experts
         nbytes = lib().dsmoe_mxfp4_scale_atoms_bytes(mats, self.out_features, K)
         if nbytes == 0:
             raise ValueError("MXFP4Weight: in features must be a multiple of 128 up to 32768, out features a multiple "
                              "of 8, with at least one expert")
-        self.codes = _dense(codes, 32)
-        self.atoms = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self._codes = _dense(codes, 32)
+        self._atoms = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
+        self._bind()
+        _pack_scales(_dense(scales, 4), mats, self.out_features, K, self._atoms)
+
+    def _bind(self) -> None:
+        """What follows from where the tensors are."""
+        self.device = self._codes.device
         self.status = _device_status(self.device)
-        self._ptrs = self.codes.data_ptr(), self.atoms.data_ptr(), self.status.data_ptr()
+        self._ptrs = self._codes.data_ptr(), self._atoms.data_ptr(), self.status.data_ptr()
         self._need: dict[tuple, int] = {}  # scratch bytes by call form and rows
-        _pack_scales(_dense(scales, 4), mats, self.out_features, K, self.atoms)
+
+    # The tensors cannot be replaced: calls use the addresses in _ptrs. A copy or
+    # an unpickled weight finds its own.
+    codes = property(lambda self: self._codes)
+    atoms = property(lambda self: self._atoms)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("device", "status", "_ptrs", "_need")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, scale_inv: torch.Tensor | None = None) -> "MXFP4Weight":
@@ -248,11 +264,11 @@ class MXFP4Weight:
             if len(self._need) >= 1024:
                 self._need.clear()
             self._need[form, rows] = need
-        return self.codes.new_empty(need)
+        return self._codes.new_empty(need)
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.atoms.numel()
+        return self._codes.numel() + self._atoms.numel()
 
 
 def _check_weight(what: str, w: MXFP4Weight, stacked: bool) -> None:
@@ -359,17 +375,35 @@ class MXFP4Experts:
                                                                    self.hidden), down.atoms, shared)
 
     def _set_up(self, gate, up, down, gate_up_atoms, down_atoms, shared: bool) -> None:
-        self.shared, self.device = bool(shared), gate.device
+        self.shared = bool(shared)
         self.n_routed = gate.shape[0] - int(self.shared)
         if self.n_routed < 1:
             raise ValueError("MXFP4Experts: no routed expert")
-        self.gate_codes, self.up_codes, self.down_codes = gate, up, down
-        self.gate_up_atoms, self.down_atoms = gate_up_atoms, down_atoms
+        self._tensors = gate, up, down, gate_up_atoms, down_atoms
+        self._bind()
+
+    def _bind(self) -> None:
+        gate, up, down, gate_up_atoms, down_atoms = self._tensors
+        self.device = gate.device
         self.status = _device_status(self.device)
         self.desc = _lib.MXFP4ExpertsDesc(
             hidden=self.hidden, inter=self.inter, n_routed=self.n_routed, shared=int(self.shared),
             gate_codes=ptr(gate), up_codes=ptr(up), gate_up_atoms=ptr(gate_up_atoms), down_codes=ptr(down),
             down_atoms=ptr(down_atoms))
+
+    # As with MXFP4Weight: not replaced, and a copy describes its own tensors.
+    gate_codes = property(lambda self: self._tensors[0])
+    up_codes = property(lambda self: self._tensors[1])
+    down_codes = property(lambda self: self._tensors[2])
+    gate_up_atoms = property(lambda self: self._tensors[3])
+    down_atoms = property(lambda self: self._tensors[4])
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("device", "status", "desc")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._bind()
 
     @classmethod
     def _empty(cls, experts: int, hidden: int, inter: int, device: torch.device) -> "MXFP4Experts":
@@ -405,8 +439,7 @@ class MXFP4Experts:
 
     @property
     def nbytes(self) -> int:
-        return sum(t.numel() for t in (self.gate_codes, self.up_codes, self.down_codes, self.gate_up_atoms,
-                                       self.down_atoms))
+        return sum(t.numel() for t in self._tensors)
 
 
 def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, experts: MXFP4Experts,

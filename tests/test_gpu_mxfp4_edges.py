@@ -77,6 +77,39 @@ def test_zeros_under_large_scales_add_nothing():
     assert bool((y == 64.0).all())
 
 
+def test_copies_are_weights_of_their_own():
+    g = gen(2)
+    x = torch.randn(6, 256, generator=g, device=DEV).to(torch.bfloat16)
+    off = torch.tensor([0, 2, 6], dtype=torch.int32, device=DEV)
+    idx = torch.randint(0, 4, (6, 2), generator=g, device=DEV)
+    tw = torch.rand(6, 2, generator=g, device=DEV)
+    w, st, ex = MXFP4Weight(*weight(g, 64, 256)), MXFP4Weight(*weight(g, 2, 64, 256)), experts(g, 5, 256, 128)
+
+    def run(w, st, ex):
+        return mxfp4_linear(x, w), mxfp4_grouped_linear(x, st, off), mxfp4_moe(x, idx, tw, ex)
+
+    want = run(w, st, ex)
+    copies = [[copy.deepcopy(v) for v in (w, st, ex)], [pickle.loads(pickle.dumps(v)) for v in (w, st, ex)]]
+    for t in (w.codes, w.atoms, st.codes, st.atoms, ex.gate_codes, ex.up_codes, ex.gate_up_atoms, ex.down_codes,
+              ex.down_atoms):
+        t.zero_()
+    for c in copies:
+        for a, b in zip(run(*c), want):
+            assert torch.equal(a, b)
+    assert all(bool((a == 0).all()) for a in run(w, st, ex))
+
+
+def test_weights_keep_their_tensors():
+    """The library is handed addresses taken once: another tensor cannot be put in their place."""
+    g = gen(3)
+    w, ex = MXFP4Weight(*weight(g, 64, 256)), experts(g, 3, 128, 128)
+    for v, names in ((w, ("codes", "atoms")),
+                     (ex, ("gate_codes", "up_codes", "gate_up_atoms", "down_codes", "down_atoms"))):
+        for n in names:
+            with pytest.raises(AttributeError):
+                setattr(v, n, getattr(v, n).clone())
+
+
 def test_threads_with_different_expert_counts():
     """The planner's shared memory follows the number of experts; two threads
     that launch it for 512 and for 400 do not disturb one another."""
