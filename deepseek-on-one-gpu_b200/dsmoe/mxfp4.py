@@ -477,6 +477,14 @@ def moe_forward(x: torch.Tensor, gate_weight: torch.Tensor, bias: torch.Tensor |
     output, routing indices and weights. Scratch is private to the call."""
     _check_x("moe_forward", x, experts.hidden, experts.device, gate_weight, bias)
     cfg = _lib.moe_config(config)
+    if x.dim() != 2 or not x.is_contiguous():
+        raise ValueError("moe_forward expects dense (tokens, hidden) activations")
+    if gate_weight.dtype != torch.bfloat16 or (bias is not None and bias.dtype != torch.float32):
+        raise TypeError("moe_forward expects a bf16 gate weight and an fp32 bias")
+    if tuple(gate_weight.shape) != (cfg.n_routed, cfg.hidden) or not gate_weight.is_contiguous() or \
+            (bias is not None and (bias.numel() != cfg.n_routed or not bias.is_contiguous())):
+        raise ValueError(f"moe_forward expects a dense gate weight {(cfg.n_routed, cfg.hidden)} and a bias of "
+                         f"{cfg.n_routed}")
     T, K = x.shape[0], cfg.top_k
     out = torch.empty_like(x)
     idx = torch.empty(T, K, dtype=torch.int64, device=x.device)

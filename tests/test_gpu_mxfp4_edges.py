@@ -110,6 +110,32 @@ def test_weights_keep_their_tensors():
                 setattr(v, n, getattr(v, n).clone())
 
 
+def test_moe_forward_refuses_what_it_would_misread():
+    cfg = DeepSeekConfig(hidden_size=256, moe_intermediate_size=128)
+    E = cfg.n_routed_experts
+    ex = MXFP4Experts._empty(E + 1, 256, 128, DEV)
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device=DEV)
+    gate = torch.zeros(E, 256, dtype=torch.bfloat16, device=DEV)
+    out, idx, tw = moe_forward(x, gate, None, cfg, ex)
+    assert out.shape == x.shape and bool((out == 0).all())
+    with pytest.raises(ValueError):
+        moe_forward(torch.zeros(4, 512, dtype=torch.bfloat16, device=DEV)[:, ::2], gate, None, cfg, ex)
+    with pytest.raises(ValueError):
+        moe_forward(x.view(2, 2, 256), gate, None, cfg, ex)
+    with pytest.raises(ValueError):
+        moe_forward(x, gate[:-1], None, cfg, ex)
+    with pytest.raises(ValueError):
+        moe_forward(x, gate.t().contiguous().t(), None, cfg, ex)
+    with pytest.raises(TypeError):
+        moe_forward(x, gate.float(), None, cfg, ex)
+    v3 = DeepSeekConfig(hidden_size=256, moe_intermediate_size=128, router_mode="v3")
+    with pytest.raises(TypeError):
+        moe_forward(x, gate, torch.zeros(E, dtype=torch.bfloat16, device=DEV), v3, ex)
+    with pytest.raises(ValueError):
+        moe_forward(x, gate, torch.zeros(E - 1, device=DEV), v3, ex)
+    assert mxfp4_status(DEV) == 0
+
+
 def test_threads_with_different_expert_counts():
     """The planner's shared memory follows the number of experts; two threads
     that launch it for 512 and for 400 do not disturb one another."""
