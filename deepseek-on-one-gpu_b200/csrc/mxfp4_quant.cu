@@ -13,13 +13,13 @@
 // product.
 //
 // Bound by memory. A thread holds N numbers: 8 of fp32 (two 16-byte loads), 16
-// of the narrower types, so that index arithmetic, shuffles and scale bytes
-// are shared by as many numbers as the registers allow; codes leave in 4- or
-// 8-byte words, contiguous over the warp. Row and matrix indexes come from
+// of bf16 and fp16, a block of e4m3, so that index arithmetic, shuffles and scale
+// bytes are shared by as many numbers as the registers allow; codes leave in 4-
+// to 16-byte words, contiguous over the warp. Row and matrix indexes come from
 // multiplications (FastDiv): two integer divisions per thread cost more than
-// the quantisation. 7169 x 18432 in fp32: 90 us, 6.7 TB/s; 32 x 2048 x 7168 in
-// e4m3: 231 us, 3.1 TB/s, bound by issue (two directed products and a select per
-// number for the exact rounding).
+// the quantisation. 7169 x 18432 in fp32: 102 us, 5.9 TB/s; 32 x 2048 x 7168 in
+// e4m3: 137 us, 5.3 TB/s (16 numbers per thread, each rounded to odd: 225 us, at
+// 70% of the issue slots).
 #include "common.cuh"
 #include "mxfp4.cuh"
 
@@ -95,9 +95,8 @@ __device__ __forceinline__ void load(const __nv_fp8_e4m3* p, __half2* v) {
 // set (rounding to odd).
 __device__ __forceinline__ float odd(float a, float b) { return __float_as_uint(a) & 1 ? a : b; }
 __device__ __forceinline__ float mul_odd(float w, float s) { return odd(__fmul_rd(w, s), __fmul_ru(w, s)); }
-// Both products of a pair by s, two packed multiplications.
-__device__ __forceinline__ float2 mul_odd(float2 w, float s) {
-  float2 a, b;
+// The lower and the upper neighbours of a pair's products by s.
+__device__ __forceinline__ void mul_both(float2 w, float s, float* a, float* b) {
   asm("{\n\t.reg .b64 pw, ps, pa, pb;\n\t"
       "mov.b64 pw, {%4, %5};\n\t"
       "mov.b64 ps, {%6, %6};\n\t"
@@ -105,9 +104,8 @@ __device__ __forceinline__ float2 mul_odd(float2 w, float s) {
       "mul.rp.f32x2 pb, pw, ps;\n\t"
       "mov.b64 {%0, %1}, pa;\n\t"
       "mov.b64 {%2, %3}, pb;\n\t}"
-      : "=f"(a.x), "=f"(a.y), "=f"(b.x), "=f"(b.y)
+      : "=f"(a[0]), "=f"(a[1]), "=f"(b[0]), "=f"(b[1])
       : "f"(w.x), "f"(w.y), "f"(s));
-  return make_float2(odd(a.x, b.x), odd(a.y, b.y));
 }
 
 // 8 numbers to e2m1 codes, the first in the lowest nibble.
@@ -175,34 +173,30 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ x, 
   }
 }
 
-// The checkpoint's e4m3 with block scales. A block of 32 has one scale_inv s
-// (128 is a multiple of 32), so its largest product is that of its largest
-// number, and s 2^-e is exact: one rounded product per number. Products beyond
-// fp32 have their exponent taken 16 lower; a block of zeros keeps s as it is,
-// since s times its 2^127 may not be finite.
-__global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* __restrict__ x, uint32_t units,
+// The checkpoint's e4m3 with block scales, a block of 32 per thread. It has one
+// scale_inv s (128 is a multiple of 32), so its largest product is that of its
+// largest number, and s 2^-e is exact: one rounded product per number. Products
+// beyond fp32 have their exponent taken 16 lower; a block of zeros keeps s as it
+// is, since s times its 2^127 may not be finite. A product lies between its two
+// fp32 neighbours: where both round to the same codes these are the exact
+// product's; only the rare others (next to a tie) are rounded to odd.
+__global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* __restrict__ x, uint32_t blocks,
                                                            FastDiv per_row, long long row_stride,
                                                            const float* __restrict__ scale_inv, FastDiv rows_per_mat,
                                                            uint32_t sc_rows, uint32_t sc_cols,
                                                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const uint64_t bound = (static_cast<uint64_t>(units) + 31) & ~31ull;
-  for (uint64_t u64 = blockIdx.x * 256u + threadIdx.x; u64 < bound; u64 += gridDim.x * 256u) {
-    const uint32_t u = static_cast<uint32_t>(u64);
-    const bool in = u64 < units;
-    __half2 v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __half2half2(__ushort_as_half(0));
-    float s = 1.f;
-    if (in) {
-      const uint32_t row = per_row(u), c = u - row * per_row.d;
-      load(x + row * row_stride + c * 16, v);
-      const uint32_t mat = rows_per_mat(row), r = row - mat * rows_per_mat.d;
-      s = __ldg(scale_inv + (static_cast<size_t>(mat) * sc_rows + r / 128) * sc_cols + c / 8);
-    }
+  for (uint64_t b = blockIdx.x * 256u + threadIdx.x; b < blocks; b += gridDim.x * 256u) {
+    const uint32_t u = static_cast<uint32_t>(b);
+    const uint32_t row = per_row(u), c = u - row * per_row.d;
+    const __nv_fp8_e4m3* p = x + row * row_stride + c * 32;
+    __half2 v[16];
+    load(p, v);
+    load(p + 16, v + 8);
+    const uint32_t mat = rows_per_mat(row), r = row - mat * rows_per_mat.d;
+    const float s = __ldg(scale_inv + (static_cast<size_t>(mat) * sc_rows + r / 128) * sc_cols + c / 4);
     __half2 m = __habs2(v[0]);
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(v[i]));
-    m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    for (int i = 1; i < 16; ++i) m = __hmax2_nan(m, __habs2(v[i]));
     const float wmax = __half2float(__hmax_nan(__low2half(m), __high2half(m)));
     const bool large = fabsf(s) >= 0x1p64f;
     const uint32_t amax = __float_as_uint(mul_odd(wmax, large ? s * 0x1p-16f : s)) & 0x7fffffffu;
@@ -210,22 +204,32 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const __nv_fp8_e4m3* 
     if (large && amax && byte != 255) byte = min(byte + 16, 254u);  // from 2^55 on: far from scale_byte's lower end
     float sc = s;
     if (amax) sc *= __uint_as_float(byte < 254 ? (254u - byte) << 23 : 0x00400000u);  // 2^(127 - byte)
-    uint32_t w[2];
+    uint32_t w[4], differ = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float p[8];
+    for (int j = 0; j < 4; ++j) {
+      float lo[8], hi[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 o = mul_odd(__half22float2(v[4 * j + i]), sc);
-        p[2 * i] = o.x;
-        p[2 * i + 1] = o.y;
+      for (int i = 0; i < 4; ++i) mul_both(__half22float2(v[4 * j + i]), sc, lo + 2 * i, hi + 2 * i);
+      w[j] = e2m1x8(lo);
+      differ |= w[j] ^ e2m1x8(hi);
+    }
+    if (differ) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(v[4 * j + i]);
+          q[2 * i] = mul_odd(f.x, sc);
+          q[2 * i + 1] = mul_odd(f.y, sc);
+        }
+        w[j] = e2m1x8(q);
       }
-      w[j] = byte == 255 ? 0 : e2m1x8(p);
     }
-    if (in) {
-      reinterpret_cast<uint2*>(codes)[u] = make_uint2(w[0], w[1]);
-      if ((u & 1) == 0) scales[u >> 1] = static_cast<uint8_t>(byte);
-    }
+    if (byte == 255) w[0] = w[1] = w[2] = w[3] = 0;
+    reinterpret_cast<uint2*>(codes)[2 * static_cast<size_t>(u)] = make_uint2(w[0], w[1]);
+    reinterpret_cast<uint2*>(codes)[2 * static_cast<size_t>(u) + 1] = make_uint2(w[2], w[3]);
+    scales[u] = static_cast<uint8_t>(byte);
   }
 }
 
@@ -267,7 +271,7 @@ __device__ __forceinline__ void store8(float* p, const float* v) {
 
 // A thread takes 8 codes at a time, 4 such groups a block's width apart with
 // their loads together. code * 2^(b - 127) is exact in fp32 and bf16. Bound by
-// the stores: 470 M numbers to bf16 in 213 us, 5.6 TB/s.
+// the stores: 470 M numbers to bf16 in 178 us, 6.7 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint32_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, uint64_t units,
@@ -326,9 +330,14 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint32_t* __rest
   for (int i = threadIdx.x; i < nkb * 128; i += 256) dst[static_cast<size_t>(i >> 7) * atoms * 128 + (i & 127)] = s[i >> 7][i & 127];
 }
 
-int grid_for(uint64_t units, int per_block) {
+// Blocks for `units`, up to `most`; the kernels stride over the rest. Quantise:
+// 64 per SM (a few waves hide one another's ends, and constants are made once for
+// several steps; 16 per SM 4% slower, no limit 12%). Dequantise: no limit (16 per
+// SM 18% slower).
+constexpr uint64_t kQuantBlocks = 148 * 64;
+int grid_for(uint64_t units, int per_block, uint64_t most = kQuantBlocks) {
   const uint64_t b = (units + per_block - 1) / per_block;
-  return static_cast<int>(b < 148 * 16 ? (b ? b : 1) : 148 * 16);
+  return static_cast<int>(b < most ? (b ? b : 1) : most);
 }
 
 }  // namespace
@@ -337,10 +346,10 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
                             const float* scale_inv, long long rows_per_mat, uint8_t* codes, uint8_t* scales,
                             cudaStream_t s) {
   if (type == kTypeE4m3) {
-    const FastDiv per_row(K / 16), rpm(static_cast<uint32_t>(rows_per_mat));
-    const uint64_t units = static_cast<uint64_t>(rows) * per_row.d;
-    quantize_fp8_kernel<<<grid_for(units, 256), 256, 0, s>>>(
-        static_cast<const __nv_fp8_e4m3*>(x), static_cast<uint32_t>(units), per_row, row_stride, scale_inv, rpm,
+    const FastDiv per_row(K / 32), rpm(static_cast<uint32_t>(rows_per_mat));
+    const uint64_t blocks = static_cast<uint64_t>(rows) * per_row.d;
+    quantize_fp8_kernel<<<grid_for(blocks, 256), 256, 0, s>>>(
+        static_cast<const __nv_fp8_e4m3*>(x), static_cast<uint32_t>(blocks), per_row, row_stride, scale_inv, rpm,
         static_cast<uint32_t>((rows_per_mat + 127) / 128), (K + 127) / 128, codes, scales);
     return cudaGetLastError();
   }
@@ -368,7 +377,7 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
 cudaError_t launch_dequantize(const uint8_t* codes, const uint8_t* scales, long long blocks, int type, void* out,
                               cudaStream_t s) {
   const uint64_t units = static_cast<uint64_t>(blocks) * 4;
-  const int grid = grid_for(units, 1024);
+  const int grid = grid_for(units, 1024, 0x7fffffff);
   const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
   switch (type) {
     case kTypeBf16: dequantize_kernel<<<grid, 256, 0, s>>>(c, scales, units, static_cast<__nv_bfloat16*>(out)); break;
