@@ -28,7 +28,8 @@ namespace dsmoe {
 namespace mx {
 
 constexpr int kMaxGroups = 512;
-constexpr int kEpiWarps = 16;
+constexpr int kWorkWarps = 16;  // epilogue warps, and those that prepare rows in the kernel
+constexpr int kRawRows = 16;   // bf16 rows that a single-group product splits itself
 constexpr int kMaxSplit = 8;  // CTAs of a cluster that share one tile's K
 
 // Token tiles of the product kernels: columns of one work unit, and 512-byte
@@ -81,6 +82,10 @@ struct GemmArgs {
   const uint8_t* sfb;    // scale atoms of the rows [tile][K/128][tile_atoms][512]
   __nv_bfloat16* y;      // [row][M]
   int32_t* next;         // counter of handed-out units, 0 before the launch; NULL: units in fixed turns
+  // The rows themselves, where the kernel prepares them: bf16 numbers, rows
+  // raw_stride apart, or the scale bytes of dense MXFP4 rows.
+  const void* raw;
+  long long raw_stride;
   uint8_t* hq;           // SwiGLU: split rows [2][P][M] and their atoms
   uint8_t* hsf;
   int* status;
@@ -109,6 +114,38 @@ __device__ __forceinline__ void split4(uint32_t x01, uint32_t x23, uint32_t& hi,
 __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bf16 numbers, two threads (lanes l and l ^ 1) per 32-number block and eight
+// (an aligned group of lanes) per K block of 128, to their two e4m3 terms and the
+// K block's scale word. Every lane of the warp takes part.
+struct Cols {
+  uint4 a, b;
+};
+__device__ __forceinline__ void split_cols(const Cols& q, uint32_t* hw, uint32_t* lw, uint32_t& word) {
+  const uint32_t w[8] = {q.a.x, q.a.y, q.a.z, q.a.w, q.b.x, q.b.y, q.b.z, q.b.w};
+  // |bf16| bit patterns order like the numbers; two at a time
+  uint32_t m2 = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m2 = __vmaxu2(m2, w[i] & 0x7fff7fffu);
+  m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
+  const uint32_t amax = max(m2 & 0xffffu, m2 >> 16);
+  const uint32_t ef = amax >> 7;
+  const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
+  // 2^(127 - byte); the product is exact (or below all that the terms hold)
+  const __nv_bfloat162 inv = __bfloat162bfloat162(__ushort_as_bfloat16(ef == 255 ? 0 : (254u - byte) << 7));
+  uint32_t x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = __bfloat1622float2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), inv));
+    x[i] = f16_pair(f.x, f.y);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split4(x[2 * i], x[2 * i + 1], hw[i], lw[i]);
+  // bytes from lanes 0, 2, 4, 6 of the K block's 8
+  word = byte << (8 * ((threadIdx.x >> 1) & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
 }
 
 // The kernels of one call are chained by programmatic dependent launches: the

@@ -52,12 +52,13 @@ struct Choice {
   int tile, ksplit, units;
 };
 Choice estimate(bool fp4, int rows, int K, int N) {
-  static const int bf16_tiles[] = {32, 64, 128, 160}, fp4_tiles[] = {64, 160};
+  static const int bf16_tiles[] = {16, 32, 64, 128, 160}, fp4_tiles[] = {64, 160};
   const int* tiles = fp4 ? fp4_tiles : bf16_tiles;
-  const int n_tiles = fp4 ? 2 : 4, kb = K / 128, sms = sm_count();
+  const int n_tiles = fp4 ? 2 : 5, kb = K / 128, sms = sm_count();
   Choice best{};
   double least = 0;
-  for (int i = 0; i < n_tiles; ++i) {
+  const int first = !fp4 && rows > mx::kRawRows ? 1 : 0;
+  for (int i = first; i < n_tiles; ++i) {
     const int tile = tiles[i], n = rows < tile ? ceil_div(rows, 16) * 16 : tile;
     const int pair = fp4 ? 0 : mx::side_by_side(tile, n);
     const int per_kb = fp4 ? 4 * (n < 128 ? 64 : n / 2) : pair ? 8 * (pair < 64 ? 64 : pair) : 16 * (n < 128 ? 64 : n / 2);
@@ -67,7 +68,7 @@ Choice estimate(bool fp4, int rows, int K, int N) {
     const long long waves = split > 1 ? 1 : (units + sms - 1) / sms;
     double t = waves * (ceil_div(kb, split) * drag * per_kb + 1500 + 25.0 * n);
     if (split > 1) t += 1500 + 40.0 * n;
-    if (i == 0 || t < least) {
+    if (i == first || t < least) {
       least = t;
       best = {tile, split, static_cast<int>(units)};
     }
@@ -108,6 +109,7 @@ struct Plan {
   size_t counts = 0, row_start = 0, tile_start = 0, next = 0, pos = 0, xq = 0, sf = 0, hq = 0, hsf = 0, y = 0, total = 0;
   int tile = 32, P = 0, ksplit = 1, units = 0;
   long long tiles = 0;
+  bool raw = false;  // the product prepares its rows: the workspace is asked for, but not used
   size_t take(size_t bytes) {
     const size_t at = total;
     total = up(total + bytes);
@@ -132,15 +134,17 @@ struct Plan {
 Plan plan_linear(int T, int K, int N) {
   Plan w;
   w.set(choose(false, T, K, N), T);
-  w.xq = w.take(2 * static_cast<size_t>(T) * K);
-  w.sf = w.take(w.atoms(K));
+  w.raw = w.tile == mx::kRawRows;
+  w.xq = w.take(w.raw ? 1 : 2 * static_cast<size_t>(T) * K);
+  if (!w.raw) w.sf = w.take(w.atoms(K));
   return w;
 }
 
 Plan plan_matmul(int T, int K, int N) {
   Plan w;
   w.set(choose(true, T, K, N), T);
-  w.sf = w.take(w.atoms(K));
+  w.raw = w.tile == 64;
+  w.sf = w.take(w.raw ? 1 : w.atoms(K));
   return w;
 }
 
@@ -200,6 +204,7 @@ int check_weight(const char* what, const void* codes, const void* atoms) {
 }
 
 // A product with bf16 activations (split rows xq) or, with fp4, MXFP4 rows.
+// With a.raw bf16 rows need no map.
 int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, const uint8_t* x, mx::GemmArgs& a,
              int tile, long long max_units, cudaStream_t s) {
   CUtensorMap m_w0, m_w1, m_x, m_x32, m_x8;
@@ -218,10 +223,11 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
     m_w1 = m_w0;
     if (w1 != w0 && (r = make_tma_map(&m_w1, u4, a.K / 2, w1, a.K, wrows, 128, 128))) return r;
     const uint64_t rows = 2 * static_cast<uint64_t>(a.P);
-    if ((r = make_tma_map(&m_x32, u8, a.K, x, a.K, rows, 128, 32))) return r;
-    if ((r = make_tma_map(&m_x8, u8, a.K, x, a.K, rows, 128, 8))) return r;
-    m_x = m_x32;  // tiles up to 64 rows never load as one box
-    if (tile > 64 && (r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
+    m_x = m_x32 = m_x8 = m_w0;
+    if (!a.raw && (r = make_tma_map(&m_x32, u8, a.K, x, a.K, rows, 128, 32))) return r;
+    if (!a.raw && (r = make_tma_map(&m_x8, u8, a.K, x, a.K, rows, 128, 8))) return r;
+    if (tile > 64 &&  // smaller ones never load as one box
+        (r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
   }
   // A split tile is a cluster, one unit per CTA; otherwise persistent CTAs.
   const int g = a.ksplit > 1 ? static_cast<int>(max_units) : gemm_grid();
@@ -323,8 +329,14 @@ int dsmoe_mxfp4_linear(const void* x, int64_t row_stride, int32_t tokens, int32_
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
   a.status = device_status;
-  MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, tokens, in_features, a.g, L.tile, nullptr,
-                           nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0, s));
+  if (L.raw) {
+    a.raw = x;
+    a.raw_stride = row_stride;
+  } else {
+    MX_CUDA(mx::launch_split(static_cast<const __nv_bfloat16*>(x), row_stride, tokens, in_features, a.g, L.tile, nullptr,
+                             nullptr, 0, 0, L.P, at<uint8_t>(workspace, L.xq), at<uint8_t>(workspace, L.sf), nullptr, 0,
+                             s));
+  }
   return run_gemm(false, false, codes, codes, 1, at<uint8_t>(workspace, L.xq), a, L.tile,
                   static_cast<long long>(L.units) * L.ksplit, s);
 }
@@ -357,8 +369,11 @@ int dsmoe_mxfp4_matmul(const void* x_codes, const void* x_scales, int32_t tokens
   a.sfb = at<uint8_t>(workspace, L.sf);
   a.y = static_cast<__nv_bfloat16*>(out);
   a.status = device_status;
-  MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(x_scales), 1, tokens, in_features, L.tile,
-                                 mx::tile_atoms(L.tile), at<uint8_t>(workspace, L.sf), s));
+  if (L.raw)
+    a.raw = x_scales;
+  else
+    MX_CUDA(mx::launch_tile_scales(static_cast<const uint8_t*>(x_scales), 1, tokens, in_features, L.tile,
+                                   mx::tile_atoms(L.tile), at<uint8_t>(workspace, L.sf), s));
   return run_gemm(true, false, codes, codes, 1, static_cast<const uint8_t*>(x_codes), a, L.tile,
                   static_cast<long long>(L.units) * L.ksplit, s);
 }

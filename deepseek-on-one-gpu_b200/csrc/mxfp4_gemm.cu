@@ -23,7 +23,11 @@
 //              for each A tile: per stage the thread copies the scale atoms to
 //              its TMEM columns (tcgen05.cp) and issues the MMAs behind them
 //   warp 3     unit planner, a shared-memory ring of decoded units
-//   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 8-column chunks
+//   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 8-column chunks. With few
+//              rows (RAW) a part of them prepares the rows instead, one stage
+//              per warp in turn: splits bf16 rows into the stage's operand and
+//              atom, or gathers MXFP4 rows' scales into the atom. What a kernel
+//              of its own in front costs, a launch and 2-3 us, is then gone.
 // Two issuing threads because one that waits on a barrier between its batches
 // leaves the tensor pipe idle: one thread for both tiles ran 512 rows over 256
 // experts 5% slower, a T=4096 product 1%. Sharing A between the hi and the lo MMA
@@ -51,9 +55,8 @@ constexpr int BM = 128;
 constexpr int RING = 4;
 constexpr int PLAN_WARP = 3;
 constexpr int EPI_WARP0 = 4;
-constexpr int NUM_CG = kEpiWarps / 4;
 constexpr int CHUNK = 8;
-constexpr int THREADS = (EPI_WARP0 + kEpiWarps) * 32;
+constexpr int THREADS = (EPI_WARP0 + kWorkWarps) * 32;
 
 struct Unit {
   int32_t ncols;   // valid rows of the token tile; 0: no more units
@@ -67,9 +70,15 @@ struct Unit {
   int32_t part;    // K part
 };
 
-template <bool FP4_, int BN_, int STAGES_>
+template <bool FP4_, int BN_, int STAGES_, bool RAW_ = false>
 struct Cfg {
   static constexpr bool FP4 = FP4_;
+  static constexpr bool RAW = RAW_;  // the kernel prepares the rows
+  static constexpr int EPI = !RAW ? kWorkWarps : FP4 ? 12 : 4;  // epilogue warps
+  // Warps that prepare rows, each those of one stage: a warp that skipped a fill
+  // of a stage could take that fill's phase of `empty` for its own.
+  static constexpr int PREP = RAW ? STAGES_ : 0;
+  static constexpr int NUM_CG = EPI / 4;
   static constexpr int BN = BN_;
   static constexpr int STAGES = STAGES_;
   static constexpr int KB_STAGE = FP4 ? 2 : 1;  // 128-number K blocks per stage (128 bytes of a row)
@@ -100,10 +109,11 @@ struct Cfg {
   static constexpr int MISC_OFF = BAR_OFF + 8 * NUM_BARS;
   static constexpr int PLAN_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
   static constexpr int TAB_OFF = PLAN_OFF + RING * static_cast<int>(sizeof(Unit));
-  static constexpr bool OWN = !FP4 && BN <= 64;  // builds the group tables of a few rows itself
-  // Group tables: kind::mxf4 has none.
-  static constexpr int SMEM = TAB_OFF + (FP4 ? 0 : OWN ? 4 * (3 * kMaxGroups + 1) : 4 * (kMaxGroups + 1)) + 1024;
+  static constexpr bool OWN = !FP4 && !RAW && BN <= 64;  // builds the group tables of a few rows itself
+  // Group tables: kind::mxf4 and RAW have none.
+  static constexpr int SMEM = TAB_OFF + (FP4 || RAW ? 0 : OWN ? 4 * (3 * kMaxGroups + 1) : 4 * (kMaxGroups + 1)) + 1024;
   static_assert(SMEM <= 232448, "shared memory");
+  static_assert(EPI + PREP <= kWorkWarps, "warps");
   static_assert(STAGES * OP_BYTES >= BN * 2 * BM * 4, "a K part's sums");
   static_assert(OP_BYTES % 1024 == 0, "operand alignment");
   static_assert(HALF >= BN && (FP4 || 4 * (BN < 96 ? BN : 96) <= 2 * HALF), "accumulator columns");
@@ -114,6 +124,9 @@ __device__ __forceinline__ uint64_t policy_evict_normal() {
   asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
   return p;
 }
+
+// Shared memory written by this thread is read by the tensor core next.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -340,17 +353,17 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], C::RAW ? 2 : 1);  // producer; the warp that prepares the stage's rows
       mbar_init(&empty[s], 2);  // both issuers
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 2);
-      mbar_init(&tempty[b], kEpiWarps);
+      mbar_init(&tempty[b], C::EPI);
     }
     mbar_init(done_bar, 2);
     for (int r = 0; r < RING; ++r) {
       mbar_init(&ufull[r], 1);
-      mbar_init(&uempty[r], 3 + kEpiWarps);  // producer, issuers, epilogue warps
+      mbar_init(&uempty[r], 3 + C::EPI + C::PREP);  // producer, issuers, epilogue and preparing warps
     }
     *s_abort = 0;
     fence_mbar_init();
@@ -433,18 +446,19 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         const int pairs = SWIGLU ? p.M / BM : (p.M + 2 * BM - 1) / (2 * BM);
         const uint8_t* fa = p.sfa + (static_cast<size_t>(e.group) * pairs + e.m0 / (SWIGLU ? BM : 2 * BM)) * KB * 1024;
         const uint8_t* fb = p.sfb + static_cast<size_t>(e.tile) * KB * (C::ATOMS * 512);
-        const uint32_t xbytes = e.both ? 2 * e.n * 128 : C::B_BYTES;
+        const uint32_t xbytes = C::RAW && !FP4 ? 0 : e.both ? 2 * e.n * 128 : C::B_BYTES;
         auto load_w = [&](int kb, int stage) {
           uint8_t* st = smem + stage * C::OP_BYTES;
           uint8_t* sf = smem + C::SF0 + stage * C::SF_BYTES;
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);  // an odd last K block: only its scales exist
           const int kx = FP4 ? kb * 64 : kb * 128;  // coordinate: bytes of packed codes, or numbers
-          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * C::A_TX + nkb * 1024 + xbytes + nkb * C::ATOMS * 512);
+          mbar_arrive_expect_tx(&full[stage], (two ? 2 : 1) * C::A_TX + nkb * 1024 + xbytes + (C::RAW ? 0 : nkb * C::ATOMS * 512));
           tma_load_2d(st, &tm_w0, &full[stage], kx, wrow + e.m0, pol_w);
           if (two) tma_load_2d(st + C::A_BYTES, &tm_w1, &full[stage], kx, wrow + e.m1, pol_w);
           bulk_load(sf, fa + static_cast<size_t>(kb) * 1024, nkb * 1024, &full[stage]);
         };
         auto load_x = [&](int kb, int stage) {
+          if (C::RAW && !FP4) return;
           uint8_t* st = smem + stage * C::OP_BYTES + C::B_OFF;
           const int nkb = min(C::KB_STAGE, e.kb1 - kb);
           const int kx = FP4 ? kb * 64 : kb * 128;
@@ -461,6 +475,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
             tma_load_2d(st, &tm_x, &full[stage], kx, e.row0, pol_x);
             if (!FP4) tma_load_2d(st + BN * 128, &tm_x, &full[stage], kx, p.P + e.row0, pol_x);
           }
+          if (C::RAW) return;
           bulk_load(smem + C::SF0 + stage * C::SF_BYTES + C::SFA_BYTES,
                     fb + static_cast<size_t>(kb) * (C::ATOMS * 512), nkb * C::ATOMS * 512, &full[stage]);
         };
@@ -565,6 +580,84 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
       mma_commit(done_bar);
       mbar_wait_settle(done_bar, 0, p.status, kDevTimeoutMma);
     }
+  } else if (C::RAW && warp >= EPI_WARP0 + C::EPI) {
+    if constexpr (C::RAW) {
+      // -------------------------------------------------------- rows (RAW only)
+      // One token tile: rows 0 to ncols - 1 of every unit. Loads are issued before
+      // the wait for the stage.
+      const int me = warp - EPI_WARP0 - C::EPI;  // this warp's stage
+      int done = 0;  // stages of earlier units
+      bool ok = me < STAGES;
+      for (int i = 0; ok; ++i) {
+        const int ri = i % RING;
+        if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutProducer, s_abort)) break;
+        const Unit e = plan[ri];
+        if (e.ncols == 0) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&uempty[ri]);
+        const int stages = (e.kb1 - e.kb0 + C::KB_STAGE - 1) / C::KB_STAGE;
+        for (int j = (me + STAGES - done % STAGES) % STAGES; j < stages; j += STAGES) {
+          const int kb = e.kb0 + j * C::KB_STAGE, stage = me;
+          const uint32_t phase = (done + j) / STAGES & 1;
+          uint8_t* sfb = smem + C::SF0 + stage * C::SF_BYTES + C::SFA_BYTES;
+          if constexpr (FP4) {
+            const uint32_t* words = static_cast<const uint32_t*>(p.raw) + static_cast<long long>(e.row0) * KB + kb;
+            uint32_t v[C::KB_STAGE][BN / 32];
+#pragma unroll
+            for (int h = 0; h < C::KB_STAGE; ++h)
+#pragma unroll
+              for (int r = 0; r < BN / 32; ++r)
+                v[h][r] = kb + h < e.kb1 && 32 * r + lane < e.ncols
+                            ? __ldg(words + (32 * r + lane) * static_cast<long long>(KB) + h) : 0;
+            if (!(ok = mbar_wait(&empty[stage], phase ^ 1, p.status, kDevTimeoutProducer, s_abort))) break;
+#pragma unroll
+            for (int h = 0; h < C::KB_STAGE; ++h)
+#pragma unroll
+              for (int r = 0; r < BN / 32; ++r)
+                reinterpret_cast<uint32_t*>(sfb + h * C::ATOMS * 512)[lane * 4 + r] = v[h][r];
+          } else {
+            const int sub = lane & 7;  // 16 columns of the K block
+            Cols c[BN / 4];
+#pragma unroll
+            for (int t = 0; t < BN / 4; ++t) {
+              const int r = 4 * t + (lane >> 3);
+              c[t] = Cols{};
+              if (r < e.ncols) {
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.raw) +
+                                                                  r * p.raw_stride + kb * 128 + sub * 16);
+                c[t].a = __ldg(src);
+                c[t].b = __ldg(src + 1);
+              }
+            }
+            if (!(ok = mbar_wait(&empty[stage], phase ^ 1, p.status, kDevTimeoutProducer, s_abort))) break;
+            __syncwarp();
+            uint8_t* b = smem + stage * C::OP_BYTES + C::B_OFF;
+#pragma unroll
+            for (int t = 0; t < BN / 4; ++t) {
+              if (4 * t < e.ncols) {  // warp-uniform
+                const int r = 4 * t + (lane >> 3), lo = e.n + r;  // hi and lo side by side
+                uint32_t hw[4], lw[4], word;
+                split_cols(c[t], hw, lw, word);
+                if (r < e.ncols) {
+                  // n is a multiple of 8: both rows have the same place in the swizzle
+                  const int chunk = (sub ^ (r & 7)) * 16;
+                  *reinterpret_cast<uint4*>(b + r * 128 + chunk) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                  *reinterpret_cast<uint4*>(b + lo * 128 + chunk) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                  if (sub == 0) {
+                    reinterpret_cast<uint32_t*>(sfb)[r * 4] = word;
+                    reinterpret_cast<uint32_t*>(sfb)[lo * 4] = word;
+                  }
+                }
+              }
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        done += stages;
+      }
+    }
   } else if (warp >= EPI_WARP0) {
     // ------------------------------------------------------------ epilogue
     const int quad = warp & 3;
@@ -605,7 +698,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
           tmem_ld_wait();
         }
       };
-      auto column = [&](int j) { return (j * NUM_CG + cg) * CHUNK; };  // of this warp's j-th chunk
+      auto column = [&](int j) { return (j * C::NUM_CG + cg) * CHUNK; };  // of this warp's j-th chunk
       // The accumulators are read into registers and given back before the
       // results are rounded and stored: a large unit's MMAs start behind
       // nothing but that read.
@@ -703,7 +796,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
         // This part's sums, fp32, into the (now unused) operand stages:
         // [column][256 features].
         float* part = reinterpret_cast<float*>(smem) + quad * 32 + lane;
-        for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += NUM_CG * CHUNK) {
+        for (int c0 = cg * CHUNK; c0 < e.ncols; c0 += C::NUM_CG * CHUNK) {
           float v[CHUNK];
           for (int a = 0; a < (two ? 2 : 1); ++a) {
             load(a ? d1 : d0, c0, v);
@@ -771,12 +864,16 @@ cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = at;
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (!C::RAW) {  // else it is the call's first kernel
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
   return cfg;
 }
 
@@ -813,8 +910,9 @@ int pick_ksplit(bool fp4, int tile, int units, int kblocks) {
   int best = 1;
   for (int s = 2; s <= kMaxSplit && s * 4 <= kblocks; ++s) {
     int n = 0;
-    if (fp4) n = tile == 64 ? resident_clusters<Cfg<true, 64, 4>>(s) : resident_clusters<Cfg<true, 160, 4>>(s);
-    else n = tile == 32 ? resident_clusters<Cfg<false, 32, 5>>(s)
+    if (fp4) n = tile == 64 ? resident_clusters<Cfg<true, 64, 4, true>>(s) : resident_clusters<Cfg<true, 160, 4>>(s);
+    else n = tile == 16 ? resident_clusters<Cfg<false, 16, 6, true>>(s)
+             : tile == 32 ? resident_clusters<Cfg<false, 32, 5>>(s)
              : tile == 64 ? resident_clusters<Cfg<false, 64, 4>>(s)
              : tile == 128 ? resident_clusters<Cfg<false, 128, 3>>(s) : resident_clusters<Cfg<false, 160, 3>>(s);
     if (n >= units) best = s;
@@ -827,12 +925,14 @@ cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUte
                         cudaStream_t s) {
   if (fp4) {
     switch (tile) {
-      case 64: return launch<Cfg<true, 64, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
+      case 64: return launch<Cfg<true, 64, 4, true>, false>(w0, w1, x, x32, x8, a, grid, s);
       case 160: return launch<Cfg<true, 160, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
       default: return cudaErrorInvalidValue;
     }
   }
   switch (tile) {
+    case 16:  // single-group products of up to 16 rows only
+      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 16, 6, true>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 32:
       return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, x8, a, grid, s)
                     : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, x8, a, grid, s);

@@ -200,10 +200,6 @@ __device__ __forceinline__ SfSpot sf_spot(int tile0, int count, int local, int K
 constexpr int kSplitThreads = 128;
 constexpr int kSplitCols = kSplitThreads * 16;
 
-struct Cols {
-  uint4 a, b;
-};
-
 // This thread's 16 columns of a row (zero past its end): block y of the grid
 // has columns kSplitCols * y and up.
 __device__ __forceinline__ Cols load_cols(const __nv_bfloat16* row, int K) {
@@ -224,29 +220,8 @@ __device__ __forceinline__ void split_row(const Cols& q, int K, int P, int n, co
   const int tid = threadIdx.x;
   const int col = blockIdx.y * kSplitCols + tid * 16;
   const bool in = col < K;  // K is a multiple of 128: 8 threads of a K block are in or out together
-  const uint32_t w[8] = {q.a.x, q.a.y, q.a.z, q.a.w, q.b.x, q.b.y, q.b.z, q.b.w};
-  // |bf16| bit patterns order like the numbers; two at a time
-  uint32_t m2 = w[0] & 0x7fff7fffu;
-#pragma unroll
-  for (int i = 1; i < 8; ++i) m2 = __vmaxu2(m2, w[i] & 0x7fff7fffu);
-  m2 = __vmaxu2(m2, __shfl_xor_sync(0xffffffffu, m2, 1));
-  const uint32_t amax = max(m2 & 0xffffu, m2 >> 16);
-  const uint32_t ef = amax >> 7;
-  const uint32_t byte = ef == 255 ? 255u : (ef > 7 ? ef - 7 : 0u);
-  // 2^(127 - byte); the product is exact (or below all that the terms hold)
-  const __nv_bfloat162 inv = __bfloat162bfloat162(__ushort_as_bfloat16(ef == 255 ? 0 : (254u - byte) << 7));
-  uint32_t x[8], hw[4], lw[4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = __bfloat1622float2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), inv));
-    x[i] = f16_pair(f.x, f.y);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split4(x[2 * i], x[2 * i + 1], hw[i], lw[i]);
-  // scale word of the K block: bytes from threads 0, 2, 4, 6 of its 8
-  uint32_t word = byte << (8 * ((tid >> 1) & 3));
-  word |= __shfl_xor_sync(0xffffffffu, word, 2);
-  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  uint32_t hw[4], lw[4], word;
+  split_cols(q, hw, lw, word);
   if (!in) return;
   uint32_t* s32 = reinterpret_cast<uint32_t*>(sf) + static_cast<long long>(col >> 7) * atoms * 128;
   const size_t lo_rows = static_cast<size_t>(P) * K;

@@ -32,6 +32,7 @@ from . import _lib
 from ._lib import check, lib, ptr
 
 BLOCK = 32
+_IDLE = 256  # bytes of the workspace of calls that use none
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
 _status: dict[int, torch.Tensor] = {}
 _status_lock = threading.Lock()
@@ -236,6 +237,7 @@ class MXFP4Weight:
         self.status = _device_status(self.device)
         self._ptrs = self._codes.data_ptr(), self._atoms.data_ptr(), self.status.data_ptr()
         self._need: dict[tuple, int] = {}  # scratch bytes by call form and rows
+        self._idle = self._codes.new_empty(_IDLE)
 
     # The tensors cannot be replaced: calls use the addresses in _ptrs. A copy or
     # an unpickled weight finds its own.
@@ -243,7 +245,7 @@ class MXFP4Weight:
     atoms = property(lambda self: self._atoms)
 
     def __getstate__(self):
-        return {k: v for k, v in self.__dict__.items() if k not in ("device", "status", "_ptrs", "_need")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("device", "status", "_ptrs", "_need", "_idle")}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -264,7 +266,7 @@ class MXFP4Weight:
             if len(self._need) >= 1024:
                 self._need.clear()
             self._need[form, rows] = need
-        return self._codes.new_empty(need)
+        return self._idle if need <= _IDLE else self._codes.new_empty(need)
 
     @property
     def nbytes(self) -> int:
