@@ -29,7 +29,7 @@ namespace mx {
 
 constexpr int kMaxGroups = 512;
 constexpr int kWorkWarps = 16;  // epilogue warps, and those that prepare rows in the kernel
-constexpr int kRawRows = 16;   // bf16 rows that a single-group product splits itself
+constexpr int kRawRows = 32;   // most bf16 rows that a single-group product splits itself
 constexpr int kMaxSplit = 8;  // CTAs of a cluster that share one tile's K
 
 // Token tiles of the product kernels: columns of one work unit, and 512-byte

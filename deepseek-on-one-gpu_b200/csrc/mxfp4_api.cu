@@ -57,7 +57,7 @@ Choice estimate(bool fp4, int rows, int K, int N) {
   const int n_tiles = fp4 ? 2 : 5, kb = K / 128, sms = sm_count();
   Choice best{};
   double least = 0;
-  const int first = !fp4 && rows > mx::kRawRows ? 1 : 0;
+  const int first = !fp4 && rows > 16 ? 1 : 0;
   for (int i = first; i < n_tiles; ++i) {
     const int tile = tiles[i], n = rows < tile ? ceil_div(rows, 16) * 16 : tile;
     const int pair = fp4 ? 0 : mx::side_by_side(tile, n);
@@ -131,10 +131,19 @@ struct Plan {
   }
 };
 
+// Rows that a product splits itself. One launch less is worth 5 us of host time
+// and 1-2 us between the kernels, but 17 to 32 rows are split faster ahead (us in a
+// captured graph, itself / ahead: 17 x 7168 x 2048 8.8 / 8.5, 32 x 2048 x 7168 11.2 /
+// 10.5, 32 x 7168 x 18432 22.9 / 20.7; calls one by one take 11.5 / 17 at least):
+// so only where a call's launches take longer than its kernels.
+bool splits_itself(int T, int K, int N) {
+  return T <= 16 || (T <= mx::kRawRows && static_cast<long long>(N) * K <= 1 << 26);
+}
+
 Plan plan_linear(int T, int K, int N) {
   Plan w;
   w.set(choose(false, T, K, N), T);
-  w.raw = w.tile == mx::kRawRows;
+  w.raw = splits_itself(T, K, N);  // tile 16 or 32
   w.xq = w.take(w.raw ? 1 : 2 * static_cast<size_t>(T) * K);
   if (!w.raw) w.sf = w.take(w.atoms(K));
   return w;

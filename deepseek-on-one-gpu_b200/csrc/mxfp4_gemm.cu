@@ -75,9 +75,10 @@ struct Cfg {
   static constexpr bool FP4 = FP4_;
   static constexpr bool RAW = RAW_;  // the kernel prepares the rows
   static constexpr int EPI = !RAW ? kWorkWarps : FP4 ? 12 : 4;  // epilogue warps
-  // Warps that prepare rows, each those of one stage: a warp that skipped a fill
-  // of a stage could take that fill's phase of `empty` for its own.
-  static constexpr int PREP = RAW ? STAGES_ : 0;
+  // Warps that prepare rows, each for one stage (16 bf16 rows of it): a warp that
+  // skipped a fill of a stage could take that fill's phase of `empty` for its own.
+  static constexpr int PREP_STAGE = !RAW ? 0 : FP4 ? 1 : BN_ / 16;
+  static constexpr int PREP = PREP_STAGE * STAGES_;
   static constexpr int NUM_CG = EPI / 4;
   static constexpr int BN = BN_;
   static constexpr int STAGES = STAGES_;
@@ -353,7 +354,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], C::RAW ? 2 : 1);  // producer; the warp that prepares the stage's rows
+      mbar_init(&full[s], 1 + C::PREP_STAGE);  // producer, the warps that prepare the stage's rows
       mbar_init(&empty[s], 2);  // both issuers
     }
     for (int b = 0; b < 2; ++b) {
@@ -583,11 +584,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
   } else if (C::RAW && warp >= EPI_WARP0 + C::EPI) {
     if constexpr (C::RAW) {
       // -------------------------------------------------------- rows (RAW only)
-      // One token tile: rows 0 to ncols - 1 of every unit. Loads are issued before
-      // the wait for the stage.
-      const int me = warp - EPI_WARP0 - C::EPI;  // this warp's stage
+      // bf16: one token tile, rows 0 to ncols - 1 of every unit. Loads are issued
+      // before the wait for the stage.
+      const int me = (warp - EPI_WARP0 - C::EPI) % STAGES;      // this warp's stage
+      const int row0 = (warp - EPI_WARP0 - C::EPI) / STAGES * 16;  // and its first bf16 row
       int done = 0;  // stages of earlier units
-      bool ok = me < STAGES;
+      bool ok = warp < EPI_WARP0 + C::EPI + C::PREP;
       for (int i = 0; ok; ++i) {
         const int ri = i % RING;
         if (!mbar_wait(&ufull[ri], (i / RING) & 1, p.status, kDevTimeoutProducer, s_abort)) break;
@@ -617,10 +619,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
                 reinterpret_cast<uint32_t*>(sfb + h * C::ATOMS * 512)[lane * 4 + r] = v[h][r];
           } else {
             const int sub = lane & 7;  // 16 columns of the K block
-            Cols c[BN / 4];
+            Cols c[4];
 #pragma unroll
-            for (int t = 0; t < BN / 4; ++t) {
-              const int r = 4 * t + (lane >> 3);
+            for (int t = 0; t < 4; ++t) {
+              const int r = row0 + 4 * t + (lane >> 3);
               c[t] = Cols{};
               if (r < e.ncols) {
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.raw) +
@@ -633,9 +635,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
             __syncwarp();
             uint8_t* b = smem + stage * C::OP_BYTES + C::B_OFF;
 #pragma unroll
-            for (int t = 0; t < BN / 4; ++t) {
-              if (4 * t < e.ncols) {  // warp-uniform
-                const int r = 4 * t + (lane >> 3), lo = e.n + r;  // hi and lo side by side
+            for (int t = 0; t < 4; ++t) {
+              if (row0 + 4 * t < e.ncols) {  // warp-uniform
+                const int r = row0 + 4 * t + (lane >> 3), lo = e.n + r;  // hi and lo side by side
                 uint32_t hw[4], lw[4], word;
                 split_cols(c[t], hw, lw, word);
                 if (r < e.ncols) {
@@ -645,7 +647,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
                   *reinterpret_cast<uint4*>(b + lo * 128 + chunk) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
                   if (sub == 0) {
                     reinterpret_cast<uint32_t*>(sfb)[r * 4] = word;
-                    reinterpret_cast<uint32_t*>(sfb)[lo * 4] = word;
+                    reinterpret_cast<uint32_t*>(sfb)[(lo & 31) * 4 + (lo >> 5)] = word;
                   }
                 }
               }
@@ -934,6 +936,7 @@ cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUte
     case 16:  // single-group products of up to 16 rows only
       return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 16, 6, true>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 32:
+      if (a.raw) return launch<Cfg<false, 32, 5, true>, false>(w0, w1, x, x32, x8, a, grid, s);
       return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, x8, a, grid, s)
                     : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, x8, a, grid, s);
     case 64:

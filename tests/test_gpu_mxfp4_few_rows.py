@@ -1,5 +1,5 @@
 """MXFP4 products of a few rows, which prepare their rows inside the product
-(bf16 rows up to 16, MXFP4 rows in small token tiles), against the 64-bit
+(bf16 rows up to 32, MXFP4 rows in small token tiles), against the 64-bit
 oracle: several work units per CTA, K longer than the ring of stages, odd
 numbers of K blocks, rows apart, K split over a cluster.
 
@@ -36,8 +36,8 @@ def test_linear(N, K):
     g = gen(N, K)
     c = mxfp4_quantize(torch.randn(N, K, generator=g, device=DEV) * 0.02)
     w, wd = MXFP4Weight(*c), O.dequantize(*c)
-    big = torch.randn(17, K + 24, generator=g, device=DEV).to(torch.bfloat16)
-    for T in (1, 4, 5, 8, 9, 15, 16, 17):
+    big = torch.randn(33, K + 24, generator=g, device=DEV).to(torch.bfloat16)
+    for T in (1, 4, 5, 8, 9, 15, 16, 17, 23, 24, 25, 32, 33):
         x = big[:T, 8:K + 8]  # rows apart, 16-byte aligned
         y = mxfp4_linear(x, w)
         check(y, x.double(), wd)
@@ -75,7 +75,7 @@ def test_many_calls_in_a_graph_and_on_two_streams():
     """No call uses another's memory: the calls have no scratch of their own."""
     g = gen(4)
     w = MXFP4Weight(*mxfp4_quantize(torch.randn(4096, 2048, generator=g, device=DEV) * 0.02))
-    xs = [torch.randn(t, 2048, generator=g, device=DEV).to(torch.bfloat16) for t in (1, 3, 16, 7)]
+    xs = [torch.randn(t, 2048, generator=g, device=DEV).to(torch.bfloat16) for t in (1, 3, 32, 7)]
     qs = [mxfp4_quantize(x) for x in xs]
     want = [(mxfp4_linear(x, w), mxfp4_matmul(*q, w)) for x, q in zip(xs, qs)]
     torch.cuda.synchronize()
