@@ -38,9 +38,9 @@
 // next unit's MMAs; a larger one takes both.
 //
 // What bounds it. Few rows: the weights' bytes from HBM (512 rows over 256
-// experts of 7168 x 2048: 255 us, 6.75 TB/s; gate and up of a 64-token FFN 570 us,
-// 6.1 TB/s). Many: the tensor pipe under the power limit. T=4096 x 7168 x 18432
-// takes 700 us (1545 TFLOP/s in useful operations; the SM clock falls to 1.39 GHz
+// experts of 7168 x 2048: 255 to 259 us, 6.7 TB/s; gate and up of a 64-token FFN
+// 570 to 585 us, 6.0 TB/s). Many: the tensor pipe under the power limit. T=4096 x 7168 x 18432
+// takes 680 to 700 us (1545 to 1590 TFLOP/s in useful operations; the SM clock falls to 1.39 GHz
 // with the pipe 87% busy), and 4-bit rows x 18432 x 7168 212 us (5.1 PFLOP/s). A
 // stage's copies take ~2000 cycles from issue to use; three stages of 76 KB hide
 // them at 1280 MMA cycles a stage.

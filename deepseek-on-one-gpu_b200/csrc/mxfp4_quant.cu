@@ -17,8 +17,8 @@
 // bytes are shared by as many numbers as the registers allow; codes leave in 4-
 // to 16-byte words, contiguous over the warp. Row and matrix indexes come from
 // multiplications (FastDiv): two integer divisions per thread cost more than
-// the quantisation. 7169 x 18432 in fp32: 102 us, 5.9 TB/s; 32 x 2048 x 7168 in
-// e4m3: 137 us, 5.3 TB/s (16 numbers per thread, each rounded to odd: 225 us, at
+// the quantisation. 7169 x 18432 in fp32: 90 us, 6.7 TB/s; 32 x 2048 x 7168 in
+// e4m3: 135 us, 5.3 TB/s (16 numbers per thread, each rounded to odd: 225 us, at
 // 70% of the issue slots).
 #include "common.cuh"
 #include "mxfp4.cuh"

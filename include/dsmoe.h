@@ -431,7 +431,8 @@ DSMOE_API int dsmoe_sample_top_p(const float* logits, int32_t rows, int32_t voca
  * run at the same time (two streams, two captured graphs) need two. Kernel
  * errors (code of dsmoe_read_status) go to *device_status, a device int32 that
  * starts at 0 and keeps the first error until the caller clears it. Row strides
- * are in elements.
+ * are in elements. `out` must not overlap an input. A product of few rows may
+ * leave the workspace unused; its size is asked for all the same.
  */
 enum { DSMOE_BF16 = 0, DSMOE_F16 = 1, DSMOE_F32 = 2, DSMOE_E4M3 = 3 };
 
