@@ -24,10 +24,10 @@
 //              its TMEM columns (tcgen05.cp) and issues the MMAs behind them
 //   warp 3     unit planner, a shared-memory ring of decoded units
 //   warps 4..  epilogue, 16 warps: lane quadrant w % 4, 8-column chunks. With few
-//              rows (RAW) a part of them prepares the rows instead, one stage
-//              per warp in turn: splits bf16 rows into the stage's operand and
-//              atom, or gathers MXFP4 rows' scales into the atom. What a kernel
-//              of its own in front costs, a launch and 2-3 us, is then gone.
+//              rows (RAW) some of them prepare the rows instead, each for one
+//              stage of the ring: split bf16 rows into the stage's operand and
+//              atom, or gather MXFP4 rows' scales into the atom. What a kernel
+//              in front costs, a launch and 1-2 us, is then gone.
 // Two issuing threads because one that waits on a barrier between its batches
 // leaves the tensor pipe idle: one thread for both tiles ran 512 rows over 256
 // experts 5% slower, a T=4096 product 1%. Sharing A between the hi and the lo MMA
@@ -39,11 +39,11 @@
 //
 // What bounds it. Few rows: the weights' bytes from HBM (512 rows over 256
 // experts of 7168 x 2048: 255 to 259 us, 6.7 TB/s; gate and up of a 64-token FFN
-// 570 to 585 us, 6.0 TB/s). Many: the tensor pipe under the power limit. T=4096 x 7168 x 18432
-// takes 680 to 700 us (1545 to 1590 TFLOP/s in useful operations; the SM clock falls to 1.39 GHz
-// with the pipe 87% busy), and 4-bit rows x 18432 x 7168 212 us (5.1 PFLOP/s). A
-// stage's copies take ~2000 cycles from issue to use; three stages of 76 KB hide
-// them at 1280 MMA cycles a stage.
+// 570 to 585 us, 6.0 TB/s). Many: the tensor pipe under the power limit. T=4096 x
+// 7168 x 18432 takes 680 to 700 us (1545 to 1590 TFLOP/s in useful operations; the
+// SM clock falls to 1.39 GHz with the pipe 87% busy), and 4-bit rows x 18432 x 7168
+// 211 us (5.1 PFLOP/s). A stage's copies take ~2000 cycles from issue to use; three
+// stages of 76 KB hide them at 1280 MMA cycles a stage.
 #include "common.cuh"
 #include "mxfp4.cuh"
 
