@@ -32,6 +32,7 @@ from . import _lib
 from ._lib import check, lib, ptr
 
 BLOCK = 32
+_INT_MAX = 2 ** 31 - 1  # of the library's sizes: ctypes hands on the lower 32 bits of a larger one
 _IDLE = 256  # bytes of the workspace of calls that use none
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2, torch.float8_e4m3fn: 3}
 _status: dict[int, torch.Tensor] = {}
@@ -149,8 +150,8 @@ def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tu
     if x.dtype not in _DTYPES:
         raise TypeError("mxfp4_quantize expects bf16, fp16, fp32 or e4m3")
     *lead, K = x.shape or (0,)
-    if K == 0 or K % BLOCK:
-        raise ValueError(f"the last dimension must be a multiple of {BLOCK}")
+    if K == 0 or K % BLOCK or K > _INT_MAX:
+        raise ValueError(f"the last dimension must be a multiple of {BLOCK} below 2^31")
     if x.dtype == torch.float8_e4m3fn:
         if scale_inv is None or scale_inv.dtype != torch.float32:
             raise TypeError("e4m3 needs fp32 scale_inv")
@@ -222,10 +223,12 @@ class MXFP4Weight:
         self.in_features, self.out_features = K, codes.shape[-2]
         self.experts = codes.shape[0] if codes.dim() == 3 else None
         mats = 1 if self.experts is None else self.experts
-        nbytes = lib().dsmoe_mxfp4_scale_atoms_bytes(mats, self.out_features, K)
+        nbytes = 0
+        if max(mats, self.out_features, K) <= _INT_MAX:
+            nbytes = lib().dsmoe_mxfp4_scale_atoms_bytes(mats, self.out_features, K)
         if nbytes == 0:
             raise ValueError("MXFP4Weight: in features must be a multiple of 128 up to 32768, out features a multiple "
-                             "of 8, with at least one expert")
+                             "of 8 up to 2^18, with at least one expert")
         self._codes = _dense(codes, 32)
         self._atoms = torch.empty(nbytes, dtype=torch.uint8, device=codes.device)
         self._bind()
@@ -461,6 +464,8 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     if topk_idx.dim() < 1 or topk_idx.shape != topk_w.shape or tuple(topk_idx.shape[:-1]) != lead:
         raise ValueError(f"mxfp4_moe: indices {tuple(topk_idx.shape)} and weights {tuple(topk_w.shape)} do not go with "
                          f"hidden {tuple(hidden.shape)}")
+    if topk_idx.shape[-1] > _INT_MAX:
+        raise ValueError("mxfp4_moe: top_k must be in [1, 8]")
     x2 = _rows(hidden)
     T, H, K = x2.shape[0], experts.hidden, topk_idx.shape[-1]
     out = torch.empty(*lead, H, dtype=torch.bfloat16, device=hidden.device)
