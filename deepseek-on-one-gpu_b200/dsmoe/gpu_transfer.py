@@ -212,7 +212,6 @@ class GPUTransfer:
                 b = MXFP4LayerBank(self.config, self.device)
             else:
                 b = LayerBank(self.config, self.slots, self.device)
-            self.banks[layer] = b
             if self.resident and hasattr(self.weight_store, "fill_bank"):
                 self.weight_store.fill_bank(layer, b)
             else:
@@ -222,6 +221,7 @@ class GPUTransfer:
                         b.write_slot(b.assign(e + 1), self.weight_store.get_expert(layer, e))
             b.sync_table(non_blocking=False)
             torch.cuda.current_stream(self.device).synchronize()
+            self.banks[layer] = b  # only a filled bank: where filling fails the next call starts anew
         return b
 
     def device_cache(self, layer: int) -> DeviceSlotCache | None:
