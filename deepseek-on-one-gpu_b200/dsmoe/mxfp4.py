@@ -48,7 +48,8 @@ def _device_status(device: torch.device) -> torch.Tensor:
             if t is None:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the first MXFP4 call on a device must come before a graph capture")
-                t = torch.zeros(1, dtype=torch.int32, device=device)
+                with torch.inference_mode(False):  # cleared later, also outside the mode of the first call
+                    t = torch.zeros(1, dtype=torch.int32, device=device)
                 torch.cuda.current_stream(device).synchronize()
                 _status[device.index] = t
     return t
@@ -420,9 +421,10 @@ class MXFP4Experts:
         def room(*shape):
             return torch.zeros(*shape, dtype=torch.uint8, device=device)
 
-        self._set_up(room(experts, inter, hidden // 2), room(experts, inter, hidden // 2),
-                     room(experts, hidden, inter // 2), room(experts, inter // 128, hidden // 128, 2, 512),
-                     room(experts, -(-hidden // 256), inter // 128, 2, 512), True)
+        with torch.inference_mode(False):  # _write may come outside the caller's mode
+            self._set_up(room(experts, inter, hidden // 2), room(experts, inter, hidden // 2),
+                         room(experts, hidden, inter // 2), room(experts, inter // 128, hidden // 128, 2, 512),
+                         room(experts, -(-hidden // 256), inter // 128, 2, 512), True)
         return self
 
     def _write(self, slot: int, gate, up, down) -> None:
