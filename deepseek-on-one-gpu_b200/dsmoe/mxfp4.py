@@ -19,7 +19,8 @@ users who halve the expert memory and the bytes a decode step reads:
 ``moe_layer_ffn`` run on 4-bit experts. Every call goes through
 ``libdsmoe.so`` on the current stream of the tensors' device, with scratch
 from torch's allocator (private to the call, also in a captured graph). There
-is no CPU path and no backward: tensors that require a gradient are rejected.
+is no CPU path and no derivative: tensors that require a gradient or carry a
+forward-mode tangent are rejected.
 """
 from __future__ import annotations
 
@@ -27,6 +28,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib, ptr
@@ -91,6 +93,7 @@ def _call(device: torch.device, name: str, *args) -> None:
 
 def _require(what: str, *tensors: torch.Tensor) -> None:
     dev, grad = None, torch.is_grad_enabled()
+    dual = forward_ad._current_level >= 0  # inside a forward-mode level
     for t in tensors:
         if t is None:
             continue
@@ -100,6 +103,8 @@ def _require(what: str, *tensors: torch.Tensor) -> None:
             raise RuntimeError("dsmoe runs on CUDA tensors only (no CPU fallback)")
         if grad and t.requires_grad:
             raise RuntimeError(f"{what} has no backward: detach the inputs or call it under torch.no_grad()")
+        if dual and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no derivative: a tangent would be lost")
         d = t.device
         if dev is None:
             dev = d

@@ -1,10 +1,17 @@
-"""MXFP4 operators under torch's modes."""
+"""MXFP4 operators under torch's modes: inference mode, forward-mode
+differentiation."""
 import subprocess
 import sys
 
 import pytest
+import torch
+from torch.autograd import forward_ad
+
+from dsmoe import (MXFP4Experts, MXFP4Weight, mxfp4_dequantize, mxfp4_grouped_linear, mxfp4_linear, mxfp4_matmul,
+                   mxfp4_moe, mxfp4_quantize)
 
 pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
 
 
 def test_first_call_in_inference_mode():
@@ -33,3 +40,36 @@ def test_first_call_in_inference_mode():
         "assert torch.equal(a, c) and not torch.equal(a, b)\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def weight(*shape):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(sum(shape))
+    return mxfp4_quantize(torch.randn(*shape, generator=g, device=DEV))
+
+
+def test_forward_mode_tangents_are_refused():
+    """The operators have no derivative of either kind: a dual number is not
+    answered with a result that has lost its tangent."""
+    w, st = MXFP4Weight(*weight(64, 256)), MXFP4Weight(*weight(2, 64, 256))
+    ex = MXFP4Experts(MXFP4Weight(*weight(3, 128, 256)), MXFP4Weight(*weight(3, 128, 256)),
+                      MXFP4Weight(*weight(3, 256, 128)))
+    x = torch.ones(4, 256, dtype=torch.bfloat16, device=DEV)
+    off = torch.tensor([0, 1, 4], dtype=torch.int32, device=DEV)
+    idx, tw = torch.zeros(4, 2, dtype=torch.int64, device=DEV), torch.ones(4, 2, device=DEV)
+    pair = mxfp4_quantize(x)
+
+    def calls(x, tw):
+        return [lambda: mxfp4_quantize(x), lambda: mxfp4_linear(x, w), lambda: mxfp4_grouped_linear(x, st, off),
+                lambda: mxfp4_moe(x, idx, tw, ex)]
+
+    want = [f() for f in calls(x, tw)]
+    with forward_ad.dual_level():
+        dual, dual_tw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, tw))
+        for f in calls(dual, tw) + calls(x, dual_tw)[3:]:
+            with pytest.raises(RuntimeError, match="tangent"):
+                f()
+        for f, y in zip(calls(x, tw), want):  # numbers without a tangent are taken as ever
+            got = f()
+            assert all(torch.equal(a, b) for a, b in zip(got, y)) if isinstance(y, tuple) else torch.equal(got, y)
+        mxfp4_matmul(*pair, w), mxfp4_dequantize(*pair)
