@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib, ptr, require_cuda, stream_handle
-from .mxfp4 import MXFP4LayerBank, moe_forward
+from .mxfp4 import MXFP4LayerBank, _require, moe_forward
 
 
 def _layer_weights(bank, gate_weight, bias) -> _lib.LayerWeights:
@@ -108,6 +108,8 @@ def moe_layer_ffn(hidden: torch.Tensor, layer_idx: int, weight_store, gpu_transf
     _, post_ln = weight_store.get_layer_norm_weights(layer_idx)
     eps = float(getattr(config, "rms_norm_eps", 1e-6))
     bank = gpu_transfer.bank(layer_idx)
+    if isinstance(bank, MXFP4LayerBank):
+        _require("moe_layer_ffn", x, post_ln)  # the norm would drop a derivative, the residual below keep it
     if not bank.fully_resident or isinstance(bank, MXFP4LayerBank):
         from .ops import rms_norm
         normed = rms_norm(x, post_ln, eps)

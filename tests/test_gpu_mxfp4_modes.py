@@ -7,8 +7,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from dsmoe import (MXFP4Experts, MXFP4Weight, mxfp4_dequantize, mxfp4_grouped_linear, mxfp4_linear, mxfp4_matmul,
-                   mxfp4_moe, mxfp4_quantize)
+from dsmoe import (DeepSeekConfig, GPUTransfer, MXFP4Experts, MXFP4Weight, SyntheticWeightStore, moe_block, moe_layer_ffn,
+                   mxfp4_dequantize, mxfp4_grouped_linear, mxfp4_linear, mxfp4_matmul, mxfp4_moe, mxfp4_quantize)
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -73,3 +73,19 @@ def test_forward_mode_tangents_are_refused():
             got = f()
             assert all(torch.equal(a, b) for a, b in zip(got, y)) if isinstance(y, tuple) else torch.equal(got, y)
         mxfp4_matmul(*pair, w), mxfp4_dequantize(*pair)
+
+
+def test_layer_ffn_has_no_derivative_either():
+    """Not one through its residual alone."""
+    cfg = DeepSeekConfig(hidden_size=256, moe_intermediate_size=128)
+    store = SyntheticWeightStore(cfg, seed=2, device=DEV, pin_memory=False, gen_device="cuda")
+    gt = GPUTransfer(cfg, store, DEV, expert_format="mxfp4")
+    x = torch.ones(4, 256, dtype=torch.bfloat16, device=DEV)
+    want = moe_layer_ffn(x, 3, store, gt, cfg)
+    for call in (moe_layer_ffn, moe_block):
+        with pytest.raises(RuntimeError, match="backward"):
+            call(x.clone().requires_grad_(), 3, store, gt, cfg)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)), 3, store, gt, cfg)
+    with torch.no_grad():
+        assert torch.equal(moe_layer_ffn(x.clone().requires_grad_(), 3, store, gt, cfg), want)
