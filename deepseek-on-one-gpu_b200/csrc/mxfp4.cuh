@@ -76,6 +76,7 @@ struct GemmArgs {
   int K;
   int P;                 // first lo row of the split activations
   int ksplit;            // parts of K per tile, a cluster's CTAs (1 unless g.counts == NULL)
+  int unit0;             // with ksplit > 1, the first unit of this launch: one per CTA from there on
   // Scale atoms of the weights, a unit's two A tiles together: [group][pair of
   // tiles][K/128][2][512], SwiGLU [group][tile][K/128][gate, up][512].
   const uint8_t* sfa;

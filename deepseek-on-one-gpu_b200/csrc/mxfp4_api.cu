@@ -238,9 +238,18 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
     if (tile > 64 &&  // smaller ones never load as one box
         (r = make_tma_map(&m_x, u8, a.K, x, a.K, rows, 128, tile))) return r;
   }
-  // A split tile is a cluster, one unit per CTA; otherwise persistent CTAs.
-  const int g = a.ksplit > 1 ? static_cast<int>(max_units) : gemm_grid();
-  MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, m_x8, a, tile, max_units < g ? static_cast<int>(max_units) : g, s));
+  // Persistent CTAs, or clusters of one tile each, one unit per CTA. All clusters fit
+  // the device (pick_ksplit); where fewer SMs may be used they come in several
+  // launches of as many whole clusters as fit, at least one: the split, and so the
+  // order of the sums, stays.
+  const int sms = gemm_grid();
+  const long long most = a.ksplit == 1 ? sms : sms < a.ksplit ? a.ksplit : sms / a.ksplit * a.ksplit;
+  const long long end = a.ksplit == 1 ? 1 : max_units;
+  for (long long u = 0; u < end; u += most) {
+    a.unit0 = static_cast<int>(u);
+    const int grid = static_cast<int>(max_units - u < most ? max_units - u : most);
+    MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, m_x8, a, tile, grid, s));
+  }
   return DSMOE_OK;
 }
 

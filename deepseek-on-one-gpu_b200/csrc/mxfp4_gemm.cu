@@ -404,9 +404,10 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
       }
       tiles = tab.tiles[p.g.n];
     }
-    const int total = tiles * (SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM)) * p.ksplit;
+    const int total = p.ksplit > 1 ? p.unit0 + static_cast<int>(gridDim.x)
+                                   : tiles * (SWIGLU ? (p.M + BM - 1) / BM : (p.M + 2 * BM - 1) / (2 * BM));
     if (lane == 0) {
-      int u = blockIdx.x;
+      int u = p.unit0 + static_cast<int>(blockIdx.x);
       for (int i = 0;; ++i) {
         Unit e;
         e.ncols = 0;  // the end
