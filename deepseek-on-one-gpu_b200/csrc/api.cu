@@ -408,7 +408,8 @@ int route_private(const dsmoe_moe_config_t* c, const void* hidden, const void* g
 }
 
 int sm_count() { return num_sms(); }
-int gemm_grid() { return g_gemm_ctas > 0 && g_gemm_ctas < num_sms() ? g_gemm_ctas : num_sms(); }
+bool gemm_limited() { return g_gemm_ctas > 0 && g_gemm_ctas < num_sms(); }
+int gemm_grid() { return gemm_limited() ? g_gemm_ctas : num_sms(); }
 
 }  // namespace dsmoe
 

@@ -24,6 +24,7 @@ int route_private(const dsmoe_moe_config_t* c, const void* hidden, const void* g
                   int64_t* idx64, float* w, void* scratch, int* status, cudaStream_t s);
 int sm_count();   // SMs of the current device
 int gemm_grid();  // CTAs of a persistent GEMM launch (dsmoe_set_gemm_sm_limit)
+bool gemm_limited();  // fewer than the device's SMs
 // Device address of the current device's allocation-free scratch status word
 // (noalloc.cu); nullptr with the reason in *err on failure.
 void* noalloc_status_word(const char** err);

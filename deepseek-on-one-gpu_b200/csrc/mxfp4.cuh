@@ -153,7 +153,9 @@ __device__ __forceinline__ void split_cols(const Cols& q, uint32_t* hw, uint32_t
 // first one is launched normally, so everything enqueued before the call is
 // done when it starts; a later one may start while its predecessor runs and
 // waits (dependency_wait) before it touches anything an earlier one of the
-// chain reads or writes.
+// chain reads or writes. Under dsmoe_set_gemm_sm_limit a product and the combine
+// are launched normally: waiting on the SMs left free, they would keep another
+// stream's kernels off them.
 __device__ __forceinline__ void dependency_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("fence.proxy.async.global;" ::: "memory");  // its data may be read by TMA next
@@ -233,17 +235,17 @@ cudaError_t launch_segments_split(const __nv_bfloat16* x, long long row_stride, 
                                   int32_t* next, int* status, uint8_t* xq, uint8_t* sf, __nv_bfloat16* zero_out, int M,
                                   cudaStream_t s);
 // out[t] = bf16(shared row + scale * sum_k w[t][k] y[pos[t][k]]), summed in fp32
-cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
-                           int shared, float scale, __nv_bfloat16* out, cudaStream_t s);
+cudaError_t launch_combine(bool chained, const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w,
+                           int top_k, int shared, float scale, __nv_bfloat16* out, cudaStream_t s);
 
 // --------------------------------------------------------- mxfp4_gemm.cu
 // K split of a single-group product of `units` (feature tile pair, token tile)
 // pairs on the current device.
 int pick_ksplit(bool fp4, int tile, int units, int kblocks);
 // x: rows in boxes of the token tile, x32 and x8: of 32 and 8.
-cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
-                        const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a, int tile, int grid,
-                        cudaStream_t s);
+cudaError_t launch_gemm(bool chained, bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1,
+                        const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a,
+                        int tile, int grid, cudaStream_t s);
 
 }  // namespace mx
 }  // namespace dsmoe

@@ -248,7 +248,7 @@ int run_gemm(bool fp4, bool swiglu, const void* w0, const void* w1, int mats, co
   for (long long u = 0; u < end; u += most) {
     a.unit0 = static_cast<int>(u);
     const int grid = static_cast<int>(max_units - u < most ? max_units - u : most);
-    MX_CUDA(mx::launch_gemm(fp4, swiglu, m_w0, m_w1, m_x, m_x32, m_x8, a, tile, grid, s));
+    MX_CUDA(mx::launch_gemm(!gemm_limited(), fp4, swiglu, m_w0, m_w1, m_x, m_x32, m_x8, a, tile, grid, s));
   }
   return DSMOE_OK;
 }
@@ -529,7 +529,7 @@ int dsmoe_mxfp4_moe(const void* hidden, int64_t row_stride, int32_t tokens, cons
   if ((r = run_gemm(false, false, w->down_codes, w->down_codes, G, at<uint8_t>(workspace, L.hq), a, L.tile,
                     L.tiles * ceil_div(H, 256), s)))
     return r;
-  MX_CUDA(mx::launch_combine(a.y, tokens, H, pos, topk_w, top_k, shared, scale, static_cast<__nv_bfloat16*>(out), s));
+  MX_CUDA(mx::launch_combine(!gemm_limited(), a.y, tokens, H, pos, topk_w, top_k, shared, scale, static_cast<__nv_bfloat16*>(out), s));
   return DSMOE_OK;
 }
 

@@ -860,14 +860,14 @@ cudaError_t prepare(int* dev) {
 }
 
 template <class C>
-cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int cluster) {
+cudaLaunchConfig_t config(bool chained, int grid, cudaStream_t s, cudaLaunchAttribute* at, int cluster) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = THREADS;
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = at;
-  if (!C::RAW) {  // else it is the call's first kernel
+  if (chained && !C::RAW) {  // RAW: it is the call's first kernel
     at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
@@ -881,13 +881,13 @@ cudaLaunchConfig_t config(int grid, cudaStream_t s, cudaLaunchAttribute* at, int
 }
 
 template <class C, bool SWIGLU>
-cudaError_t launch(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& x32,
-                   const CUtensorMap& x8, const GemmArgs& a, int grid, cudaStream_t s) {
+cudaError_t launch(bool chained, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
+                   const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a, int grid, cudaStream_t s) {
   int dev = 0;
   const cudaError_t e = prepare<C, SWIGLU>(&dev);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute at[2];
-  const cudaLaunchConfig_t cfg = config<C>(grid, s, at, a.ksplit);
+  const cudaLaunchConfig_t cfg = config<C>(chained, grid, s, at, a.ksplit);
   return cudaLaunchKernelEx(&cfg, mx_gemm_kernel<C, SWIGLU>, w0, w1, x, x32, x8, a);
 }
 
@@ -900,7 +900,7 @@ int resident_clusters(int split) {
   int& n = cache[dev][split];
   if (n == 0) {
     cudaLaunchAttribute at[2];
-    cudaLaunchConfig_t cfg = config<C>(split, nullptr, at, split);
+    cudaLaunchConfig_t cfg = config<C>(true, split, nullptr, at, split);
     if (cudaOccupancyMaxActiveClusters(&n, mx_gemm_kernel<C, false>, &cfg) != cudaSuccess) n = -1;
   }
   return n;
@@ -923,31 +923,31 @@ int pick_ksplit(bool fp4, int tile, int units, int kblocks) {
   return best;
 }
 
-cudaError_t launch_gemm(bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x,
-                        const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a, int tile, int grid,
-                        cudaStream_t s) {
+cudaError_t launch_gemm(bool chained, bool fp4, bool swiglu, const CUtensorMap& w0, const CUtensorMap& w1,
+                        const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& x8, const GemmArgs& a,
+                        int tile, int grid, cudaStream_t s) {
   if (fp4) {
     switch (tile) {
-      case 64: return launch<Cfg<true, 64, 4, true>, false>(w0, w1, x, x32, x8, a, grid, s);
-      case 160: return launch<Cfg<true, 160, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
+      case 64: return launch<Cfg<true, 64, 4, true>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
+      case 160: return launch<Cfg<true, 160, 4>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
       default: return cudaErrorInvalidValue;
     }
   }
   switch (tile) {
     case 16:  // single-group products of up to 16 rows only
-      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 16, 6, true>, false>(w0, w1, x, x32, x8, a, grid, s);
+      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 16, 6, true>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
     case 32:
-      if (a.raw) return launch<Cfg<false, 32, 5, true>, false>(w0, w1, x, x32, x8, a, grid, s);
-      return swiglu ? launch<Cfg<false, 32, 5>, true>(w0, w1, x, x32, x8, a, grid, s)
-                    : launch<Cfg<false, 32, 5>, false>(w0, w1, x, x32, x8, a, grid, s);
+      if (a.raw) return launch<Cfg<false, 32, 5, true>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
+      return swiglu ? launch<Cfg<false, 32, 5>, true>(chained, w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 32, 5>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
     case 64:
-      return swiglu ? launch<Cfg<false, 64, 4>, true>(w0, w1, x, x32, x8, a, grid, s)
-                    : launch<Cfg<false, 64, 4>, false>(w0, w1, x, x32, x8, a, grid, s);
+      return swiglu ? launch<Cfg<false, 64, 4>, true>(chained, w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 64, 4>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
     case 128:  // single-group products only
-      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 128, 3>, false>(w0, w1, x, x32, x8, a, grid, s);
+      return swiglu ? cudaErrorInvalidValue : launch<Cfg<false, 128, 3>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
     case 160:
-      return swiglu ? launch<Cfg<false, 160, 3>, true>(w0, w1, x, x32, x8, a, grid, s)
-                    : launch<Cfg<false, 160, 3>, false>(w0, w1, x, x32, x8, a, grid, s);
+      return swiglu ? launch<Cfg<false, 160, 3>, true>(chained, w0, w1, x, x32, x8, a, grid, s)
+                    : launch<Cfg<false, 160, 3>, false>(chained, w0, w1, x, x32, x8, a, grid, s);
     default: return cudaErrorInvalidValue;
   }
 }

@@ -612,11 +612,11 @@ cudaError_t launch_segments_split(const __nv_bfloat16* x, long long row_stride, 
   }
 }
 
-cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w, int top_k,
-                           int shared, float scale, __nv_bfloat16* out, cudaStream_t s) {
+cudaError_t launch_combine(bool chained, const __nv_bfloat16* y, int T, int H, const int32_t* pos, const float* w,
+                           int top_k, int shared, float scale, __nv_bfloat16* out, cudaStream_t s) {
   // Few tokens: a block per 2048 columns; many: one per token.
   const dim3 grid(T, T < 512 ? (H + 2047) / 2048 : 1);
-  return launch_chained(true, combine_kernel, grid, 256, 0, s, y, T, H, pos, w, top_k, shared, scale, out);
+  return launch_chained(chained, combine_kernel, grid, 256, 0, s, y, T, H, pos, w, top_k, shared, scale, out);
 }
 
 }  // namespace mx

@@ -205,8 +205,9 @@ DSMOE_API int dsmoe_read_ranges(int32_t n, const char* const* paths, const uint6
  * launches at max_ctas CTAs (one per SM), leaving the other SMs free for a
  * collective running concurrently on another stream (the expert-parallel
  * all-to-all). 0 (the default) uses every SM. Results do not depend on it.
- * The MXFP4 products keep to it too; one whose K is split over a cluster of up
- * to 8 CTAs runs as many clusters at a time as fit, but at least one.
+ * The MXFP4 products keep to it too, and do not start before the kernel in front
+ * of them has ended; one whose K is split over a cluster of up to 8 CTAs runs as
+ * many clusters at a time as fit, but at least one.
  */
 DSMOE_API int dsmoe_set_gemm_sm_limit(int32_t max_ctas);
 

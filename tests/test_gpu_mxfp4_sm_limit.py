@@ -2,6 +2,7 @@
 from its captured graph. A CTA of a product takes a whole SM's shared memory
 (one CTA per SM), so that its grid is the number of SMs it holds."""
 import ctypes
+import itertools
 
 import pytest
 import torch
@@ -110,3 +111,21 @@ def test_the_limit_holds(limit):
             assert all(k[0] <= limit for k in gemms), (name, gemms)
         assert torch.equal(got, want), name
     assert mxfp4_status(DEV) == 0
+
+
+@pytest.mark.parametrize("limit", [5, 100])
+def test_no_kernel_of_a_capped_call_waits_on_the_other_sms(limit):
+    """Launched before its predecessor has ended, a kernel would hold the SMs
+    that the limit leaves free while it waits: a capped call's products and what
+    comes behind them start in turn."""
+    for name, fn in cases().items():
+        free, _ = launches(fn)
+        try:
+            set_gemm_sm_limit(limit)
+            capped, _ = launches(fn)
+        finally:
+            set_gemm_sm_limit(0)
+        behind = list(itertools.dropwhile(lambda k: k[1] != GEMM_THREADS, capped))
+        assert behind and not any(early for _, _, early in behind), (name, capped)
+        if "ffn" in name:  # chained where nothing is to be left free
+            assert any(early for _, threads, early in free if threads == GEMM_THREADS)
