@@ -118,12 +118,8 @@ cudaError_t launch_combine(const __nv_bfloat16* y, int T, int H, const int32_t* 
   if (T == 0) return cudaSuccess;
   int grid = T;
   if (peer_out) {
-    static int n_sm[64] = {0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (n_sm[dev] == 0 && cudaDeviceGetAttribute(&n_sm[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-      return cudaErrorInvalidDevice;
-    grid = T < 4 * n_sm[dev] ? T : 4 * n_sm[dev];
+    const int most = 4 * sm_count();
+    grid = T < most ? T : most;
   }
   cb::combine_kernel<<<grid, 256, 0, stream>>>(y, T, H, pos, w, top_k, row_start, scale, has_shared, residual, out,
                                             origin, peer_out, me, cap, n_rows);

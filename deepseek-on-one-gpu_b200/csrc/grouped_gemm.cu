@@ -49,6 +49,8 @@
 // Work unit = (group, 128-feature tile, BN-token tile); units are ordered
 // group-major, then feature tile, then token tile; CTA b takes units b,
 // b + gridDim.x, ...
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -448,7 +450,7 @@ template <int BN, int STAGES, int NBUF, bool NCAT, int EPI_WARPS>
 cudaError_t launch_cfg(const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& x, const CUtensorMap& x32,
                        const GemmParams& p, int grid, cudaStream_t stream) {
   using C = Cfg<BN, STAGES, NBUF, NCAT, EPI_WARPS>;
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];
   int dev = 0;
   const cudaError_t de = cudaGetDevice(&dev);
   if (de != cudaSuccess) return de;

@@ -44,6 +44,8 @@
 // SM clock falls to 1.39 GHz with the pipe 87% busy), and 4-bit rows x 18432 x 7168
 // 211 us (5.1 PFLOP/s). A stage's copies take ~2000 cycles from issue to use; three
 // stages of 76 KB hide them at 1280 MMA cycles a stage.
+#include <atomic>
+
 #include "common.cuh"
 #include "mxfp4.cuh"
 
@@ -847,7 +849,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
 
 template <class C, bool SWIGLU>
 cudaError_t prepare(int* dev) {
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];  // threads that come together set it twice
   cudaError_t e = cudaGetDevice(dev);
   if (e != cudaSuccess) return e;
   if (*dev < 0 || *dev >= 64) return cudaErrorInvalidDevice;
@@ -894,14 +896,15 @@ cudaError_t launch(bool chained, const CUtensorMap& w0, const CUtensorMap& w1, c
 // Clusters of `split` CTAs that run at the same time on the current device.
 template <class C>
 int resident_clusters(int split) {
-  static int cache[64][kMaxSplit + 1] = {};
+  static std::atomic<int> cache[64][kMaxSplit + 1];
   int dev = 0;
   if (prepare<C, false>(&dev) != cudaSuccess) return 0;
-  int& n = cache[dev][split];
+  int n = cache[dev][split].load(std::memory_order_relaxed);
   if (n == 0) {
     cudaLaunchAttribute at[2];
     cudaLaunchConfig_t cfg = config<C>(true, split, nullptr, at, split);
     if (cudaOccupancyMaxActiveClusters(&n, mx_gemm_kernel<C, false>, &cfg) != cudaSuccess) n = -1;
+    cache[dev][split].store(n, std::memory_order_relaxed);
   }
   return n;
 }

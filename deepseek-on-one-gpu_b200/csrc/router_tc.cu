@@ -11,6 +11,8 @@
 // operand, all experts (up to 256) are the N operand, K advances 64 elements
 // (128 bytes) per stage. Warp 0 issues TMA, warp 1 allocates TMEM and issues
 // the MMAs, warps 2-5 read the 128 x E accumulator back and store it.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -149,7 +151,7 @@ int router_tc_ksplit(int T, int H, int num_sms) {
 cudaError_t launch_router_logits_tc(const CUtensorMap& tm_x, const CUtensorMap& tm_g, float* partial, int T, int H,
                                     int E, int ksplit, int* status, cudaStream_t stream) {
   if (E > rtc::MAX_E || E % 16 || H % rtc::BKE) return cudaErrorInvalidValue;
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];
   int dev = 0;
   const cudaError_t de = cudaGetDevice(&dev);
   if (de != cudaSuccess) return de;

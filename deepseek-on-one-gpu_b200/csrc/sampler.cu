@@ -40,6 +40,7 @@
 // counting as the maximum). For temperature > 0, a row whose maximum logit is
 // not finite (a NaN anywhere, or +-inf, where the reference's softmax yields
 // NaN) gets token -1.
+#include <atomic>
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -605,7 +606,7 @@ cudaError_t launch_top_p(const float* logits, int rows, int V, long long ld, flo
   if (rows <= 0) return cudaSuccess;
   const int ncta = (V + smp::CHUNK - 1) / smp::CHUNK;
   if (V <= 0 || ncta > smp::MAX_CTAS || rows > 65535) return cudaErrorInvalidValue;
-  static bool attr[64] = {false};
+  static std::atomic<bool> attr[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
