@@ -21,6 +21,7 @@
 // e4m3: 135 us, 5.3 TB/s (16 numbers per thread, each rounded to odd: 225 us, at
 // 70% of the issue slots).
 #include "common.cuh"
+#include "kernels.h"
 #include "mxfp4.cuh"
 
 #include <cuda_fp16.h>
@@ -334,8 +335,8 @@ __global__ void __launch_bounds__(256) tile_scales_kernel(const uint32_t* __rest
 // 64 per SM (a few waves hide one another's ends, and constants are made once for
 // several steps; 16 per SM 4% slower, no limit 12%). Dequantise: no limit (16 per
 // SM 18% slower).
-constexpr uint64_t kQuantBlocks = 148 * 64;
-int grid_for(uint64_t units, int per_block, uint64_t most = kQuantBlocks) {
+uint64_t quant_blocks() { return 64ull * sm_count(); }
+int grid_for(uint64_t units, int per_block, uint64_t most) {
   const uint64_t b = (units + per_block - 1) / per_block;
   return static_cast<int>(b < most ? (b ? b : 1) : most);
 }
@@ -348,7 +349,7 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
   if (type == kTypeE4m3) {
     const FastDiv per_row(K / 32), rpm(static_cast<uint32_t>(rows_per_mat));
     const uint64_t blocks = static_cast<uint64_t>(rows) * per_row.d;
-    quantize_fp8_kernel<<<grid_for(blocks, 256), 256, 0, s>>>(
+    quantize_fp8_kernel<<<grid_for(blocks, 256, quant_blocks()), 256, 0, s>>>(
         static_cast<const __nv_fp8_e4m3*>(x), static_cast<uint32_t>(blocks), per_row, row_stride, scale_inv, rpm,
         static_cast<uint32_t>((rows_per_mat + 127) / 128), (K + 127) / 128, codes, scales);
     return cudaGetLastError();
@@ -358,8 +359,8 @@ cudaError_t launch_quantize(const void* x, int type, long long rows, int K, long
     constexpr bool ROWS = decltype(with_rows)::value;
     const FastDiv per_row(K / Form<T>::N);
     const uint64_t units = static_cast<uint64_t>(rows) * per_row.d;
-    quantize_kernel<T, ROWS><<<grid_for(units, 256), 256, 0, s>>>(p, static_cast<uint32_t>(units), per_row, row_stride,
-                                                                  codes, scales);
+    quantize_kernel<T, ROWS><<<grid_for(units, 256, quant_blocks()), 256, 0, s>>>(
+        p, static_cast<uint32_t>(units), per_row, row_stride, codes, scales);
   };
   auto either = [&](auto* p) {
     if (rows == 1 || row_stride == K) go(p, std::false_type{});
