@@ -40,9 +40,9 @@
 // What bounds it. Few rows: the weights' bytes from HBM (512 rows over 256
 // experts of 7168 x 2048: 255 to 259 us, 6.7 TB/s; gate and up of a 64-token FFN
 // 570 to 585 us, 6.0 TB/s). Many: the tensor pipe under the power limit. T=4096 x
-// 7168 x 18432 takes 680 to 700 us (1545 to 1590 TFLOP/s in useful operations; the
-// SM clock falls to 1.39 GHz with the pipe 87% busy), and 4-bit rows x 18432 x 7168
-// 211 us (5.1 PFLOP/s). A stage's copies take ~2000 cycles from issue to use; three
+// 7168 x 18432 takes 680 to 700 us by itself (1545 to 1590 TFLOP/s in useful
+// operations, the pipe 89% busy at 1.51 GHz; in long runs the clock falls to 1.17),
+// and 4-bit rows x 18432 x 7168 211 us (5.1 PFLOP/s, 66% at 1.65 GHz). A stage's copies take ~2000 cycles from issue to use; three
 // stages of 76 KB hide them at 1280 MMA cycles a stage.
 #include <atomic>
 
@@ -721,7 +721,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tm_w0, const __grid_constant_
             float g[CHUNK], up[CHUNK];
             load(d0, column(j), g);
             load(d1, column(j), up);
-            // silu in fp32 with the fast exp and divide (a few fp32 ulp)
+            // silu in fp32 with the fast exp and divide. __expf is off by 2 +
+            // 1.173 |g| units in the last place, the divide by 2: relative error up
+            // to (5 + 1.2 |g|) 2^-23 (29 units at g = -20, 101 at -80). Where 1 +
+            // e^-g passes 2^126 (g below -87.3) the divide may give 0, of a silu
+            // below 2^-119. All far below the 2^-9 that the split keeps.
 #pragma unroll
             for (int t = 0; t < CHUNK; ++t) h[j * CHUNK + t] = __fdividef(g[t], 1.0f + __expf(-g[t])) * up[t];
           }

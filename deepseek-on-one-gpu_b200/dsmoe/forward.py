@@ -98,9 +98,10 @@ def moe_layer_ffn(hidden: torch.Tensor, layer_idx: int, weight_store, gpu_transf
     """The FFN half of a MoE transformer layer (``inference/forward.py:97-109``
     for ``layer_idx >= first_k_dense_replace``):
     ``hidden + moe_block(rms_norm(hidden, post_attention_layernorm))``, bf16.
-    With every expert of the layer resident this is one library call
+    With every FP8 expert of the layer resident this is one library call
     (``dsmoe_moe_layer_ffn``: the norm kernel, the MoE kernels, and the
-    residual add inside the combine)."""
+    residual add inside the combine); otherwise, and with MXFP4 experts, it is
+    ``rms_norm``, ``moe_block`` and an addition, each rounded to bf16."""
     H = hidden.shape[-1]
     x = hidden.reshape(-1, H).contiguous()
     if x.dtype != torch.bfloat16:

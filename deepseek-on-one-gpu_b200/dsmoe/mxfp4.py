@@ -146,8 +146,8 @@ def _quantize_into(x: torch.Tensor, scale_inv: torch.Tensor | None, codes: torch
 def mxfp4_quantize(x: torch.Tensor, scale_inv: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``x`` [..., K] (K a multiple of 32) -> codes uint8 [..., K/2] and scales
     uint8 [..., K/32]. Per block of 32 numbers with largest magnitude a:
-    scale 2^(floor(log2 a) - 2), codes rounded to nearest even, saturating at
-    6; a block with an infinity or a NaN becomes NaN.
+    scale 2^(floor(log2 a) - 2), from 2^-127 to 2^127, codes rounded to nearest
+    even, saturating at 6; a block with an infinity or a NaN becomes NaN.
 
     ``x`` is bf16, fp16 or fp32, or e4m3 [..., O, I] with the checkpoint's
     ``scale_inv`` fp32 [..., ceil(O/128), ceil(I/128)] (the products are
@@ -300,8 +300,10 @@ def _check_x(what: str, x: torch.Tensor, K: int, device: torch.device, *others: 
 
 
 def mxfp4_linear(x: torch.Tensor, weight: MXFP4Weight) -> torch.Tensor:
-    """``bf16(x @ W.T)`` for bf16 ``x`` [..., in], fp32 sums. A row with an
-    infinity or a NaN comes out as NaN."""
+    """``bf16(x @ W.T)`` for bf16 ``x`` [..., in], fp32 sums. Numbers of ``x``
+    below 2^-9 of the largest of their block of 32 are taken with an error of at
+    most 2^-17 of it, all others exactly. A row with an infinity or a NaN comes
+    out as NaN."""
     _check_weight("mxfp4_linear", weight, False)
     K, N = weight.in_features, weight.out_features
     _check_x("mxfp4_linear", x, K, weight.device)
@@ -343,7 +345,8 @@ def mxfp4_grouped_linear(x: torch.Tensor, weight: MXFP4Weight, offsets: torch.Te
     [R, in] (bf16) times expert e's weight -> bf16 [R, out]. ``offsets`` is
     int32 [E + 1] on the device, never read by the host. Rows outside every
     segment are zero in a new output and left as they are in ``out`` (dense
-    bf16 [R, out], which must not overlap ``x``)."""
+    bf16 [R, out], which must not overlap ``x``). Small numbers of a row and
+    infinities and NaN are as in ``mxfp4_linear``."""
     _check_weight("mxfp4_grouped_linear", weight, True)
     _check_x("mxfp4_grouped_linear", x, weight.in_features, weight.device, offsets, out)
     if x.dim() != 2:
@@ -460,8 +463,10 @@ def mxfp4_moe(hidden: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor
     and ``topk_w`` fp32, [..., top_k], top_k <= 8):
     ``bf16(scale * sum_k w_k E_k(hidden) + E_shared(hidden))``,
     ``E(x) = down(silu(gate(x)) * up(x))``, for bf16 ``hidden`` [..., hidden].
-    silu and the sum over experts are fp32; each expert's output row is
-    rounded to bf16. An id outside the routed experts adds nothing."""
+    silu, its product with up and the sum over experts are fp32; in between, the
+    down projection takes that product to 8 or 9 significant bits (two e4m3 terms,
+    as ``mxfp4_linear`` takes bf16, by way of fp16) and each expert's output row
+    is rounded to bf16. An id outside the routed experts adds nothing."""
     if not isinstance(experts, MXFP4Experts):
         raise TypeError("mxfp4_moe expects MXFP4Experts")
     _check_x("mxfp4_moe", hidden, experts.hidden, experts.device, topk_idx, topk_w)

@@ -442,13 +442,13 @@ enum { DSMOE_BF16 = 0, DSMOE_F16 = 1, DSMOE_F32 = 2, DSMOE_E4M3 = 3 };
 /*
  * x [rows][row_stride], cols (% 32 == 0) numbers per row -> codes [rows][cols/2],
  * scales [rows][cols/32]. Per block of 32, with a = max|v|:
- * scale = 2^max(floor(log2 a) - 2, -127), codes rounded to nearest even and
- * saturated at 6. A block with an infinity or a NaN gets scale byte 255 and
+ * scale = 2^(floor(log2 a) - 2), in [2^-127, 2^127], codes rounded to nearest
+ * even and saturated at 6. A block with an infinity or a NaN gets scale byte 255 and
  * codes 0, a zero block scale byte 0. DSMOE_E4M3 takes the checkpoint's form:
  * scale_inv fp32 [rows / rows_per_matrix][ceil(rows_per_matrix/128)][ceil(cols/128)]
- * multiplies 128x128 blocks, and the exact products are rounded (a product
- * beyond fp32's largest number saturates there). Rows start on 16 bytes; codes
- * are 8-byte aligned.
+ * multiplies 128x128 blocks, and the exact products are rounded, those beyond
+ * fp32's largest number too (scale bytes 253 and 254, the latter saturating at
+ * 6 * 2^127). Rows start on 16 bytes; codes are 8-byte aligned.
  */
 DSMOE_API int dsmoe_mxfp4_quantize(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t row_stride,
                                    const float* scale_inv, int64_t rows_per_matrix, void* codes, void* scales,
@@ -472,7 +472,7 @@ DSMOE_API int dsmoe_mxfp4_scale_atoms(const void* scales, int32_t matrices, int3
 /*
  * out[t][o] = bf16( sum_i x[t][i] * weight[o][i] ), x bf16, weight MXFP4 (codes
  * 32-byte aligned), fp32 sums. in features a multiple of 128 up to 32768, out
- * features a multiple of 8. A row of x with an infinity or a NaN comes out as
+ * features a multiple of 8 up to 2^18, up to 2^22 rows (here and below). A row of x with an infinity or a NaN comes out as
  * NaN. Numbers below 2^-9 of the largest of their block of 32 are taken with an
  * error of at most 2^-17 of it, all others exactly.
  */
@@ -506,9 +506,10 @@ DSMOE_API int dsmoe_mxfp4_grouped_linear(const void* x, int64_t row_stride, int3
  *   out[t] = bf16( scale * sum_k topk_w[t][k] E_{topk_idx[t][k]}(hidden[t]) + E_shared(hidden[t]) ),
  *   E(x) = down(silu(gate(x)) * up(x)).
  * Matrices: the shared expert first (if shared == 1), then the routed experts.
- * silu and the product stay in fp32 and are split like activations; each
- * expert's output row is rounded to bf16, the sum over experts is fp32 in
- * top-k order. An id outside [0, n_routed) adds nothing. top_k <= 8.
+ * silu and the product stay in fp32 and are split like activations, to 8 or 9
+ * bits, for the down projection; each expert's output row is rounded to bf16,
+ * the sum over experts is fp32 in top-k order. An id outside [0, n_routed) adds
+ * nothing. top_k <= 8.
  */
 typedef struct {
   int32_t hidden;    /* multiples of 128 */
